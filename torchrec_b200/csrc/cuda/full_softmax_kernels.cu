@@ -1,0 +1,1122 @@
+// Cross entropy of a softmax over a whole catalogue, with its gradient, without keeping the scores.  For the rows i whose target is
+// not ignored (z = h W^T + b, all sums in fp32, operands bf16):
+//   loss_i = log sum_v exp z_iv - z_i,t          dW = G^T h,  db = sum_i G,  dh = G W,   G_iv = g_i (exp(z_iv - lse_i) - [v = t_i]).
+// A library route writes the [P, V] scores and reads them back several times; here a 128 x 128 tile of them lives in tensor memory.
+//
+// One kernel, three forms.  128 rows X stay in shared memory, 128-row tiles Y are streamed past them:
+//   S = X Y^T (tcgen05, fp32 in TMEM) -> E = f(S) in registers, rounded to bf16, written back over S -> ACC += E Y (A operand in TMEM).
+//   FWD  X = rows of h, Y = W.   f is the running softmax, so that ACC / sum is the expectation of W under the softmax: the forward
+//        already holds dh up to the upstream factor, and no pass over the scores is spent on dh in the backward.
+//   LSE  the same without ACC (no gradient wanted).
+//   BWD  X = rows of W, Y = h.   f uses the known log sum, so ACC = dW of the 128 items; nothing is added up across blocks.
+// That is 8 P V D operations for the step, of which 2 P V D recompute the scores, and two exponentials per score.
+// The target's own term never enters the rounded sums: with w = 1 - p_t (from the sum over the others), dh = w (ACC / sum - W_t) and
+// G_it = -w, so rows that the model already predicts well keep their relative accuracy.
+//
+// Both products want the streamed tile, once K-major (S) and once MN-major (ACC); one copy in shared memory serves both up to
+// D = 256, where ACC takes the 256 TMEM columns that two S tiles leave.  Wider rows are cut into pieces of 256 columns that
+// recompute S (and load the tile twice).
+// The maximum is raised lazily: ACC and the sum are rescaled only when a row's maximum grew by more than 2^8 (the rounded terms stay
+// below 2^8, which bf16 holds with its usual relative error).
+// Ignored rows are left out at the start (their h is never multiplied, so NaN or infinity in padding does not spread) and cost nothing.
+// All sums run in a fixed order: pieces of the streamed axis go to a workspace and are joined by a second kernel.
+// Every wait is bounded (tcgen05.cuh); a block that gives up raises an error word and returns.
+//
+// (The reference ends BERT4Rec in a dense projection over the vocabulary and nn.CrossEntropyLoss, examples/bert4rec/bert4rec_main.py.)
+#include <ATen/ATen.h>
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <torch/library.h>
+
+#include <cmath>
+
+#include "common.cuh"
+#include "tcgen05.cuh"
+
+namespace trb {
+
+constexpr int kFsTile = 128;                        // rows of X, and of a streamed tile
+constexpr int kFsThreads = 320;                     // TMA warp, MMA warp, 8 softmax warps
+constexpr int kFsSlotBytes = kFsTile * 128;         // 128 rows x 64 bf16
+constexpr int kFsSlots = 14;                        // X and the ring of streamed blocks
+constexpr int kFsMaxUnits = 13;
+constexpr int kFsMaxD = 1024;
+constexpr int kFsAcc = 256;                         // accumulator columns
+constexpr int kFsExtra = 3072;                      // per-column values of a tile, exchange of maxima, barriers
+constexpr int kFsSmem = kFsSlots * kFsSlotBytes + kFsExtra;
+constexpr int kFsItemsPerSm = 4;                    // bounds the workspace of partial results
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr float kRaise = 8.f;                       // base-2 growth of the maximum that forces a rescale
+
+enum FsMode : int { FS_LSE = 0, FS_FWD = 1, FS_BWD = 2 };
+enum FsErr : int { FS_ERR_EMPTY = 1, FS_ERR_FULL = 2, FS_ERR_X = 3, FS_ERR_S = 4, FS_ERR_P = 5, FS_ERR_ACC = 6, FS_ERR_COL = 7, FS_ERR_XCH = 8, FS_ERR_SMEM = 9, FS_ERR_TARGET = 16 };
+
+__device__ int g_fs_error = 0;  // one word per device; never allocated, so it may first be touched inside a graph capture
+
+// How the tiles of X, pieces of the accumulator's columns and pieces of the streamed axis are dealt to the blocks.  Computed alike by
+// every block (the number of rows that are not ignored is only known on the device).
+struct FsSchedule {
+  int tx, ty, pieces, splits, per, items;
+};
+
+__host__ __device__ inline FsSchedule fs_schedule(int nx, int ny, int pieces, int grid) {
+  FsSchedule s;
+  s.tx = (nx + kFsTile - 1) / kFsTile;
+  s.ty = (ny + kFsTile - 1) / kFsTile;
+  s.pieces = pieces;
+  s.splits = 1;
+  s.per = s.ty;
+  const int base = s.tx * pieces;
+  if (base > 0 && s.ty > 1) {
+    // rounds of blocks x (tiles of an item + its start, end and share of the join).  Candidates fill 1..4 rounds.
+    const int most = s.tx > 0 ? (kFsItemsPerSm * grid) / s.tx : 1;
+    float best = float((base + grid - 1) / grid) * (s.ty + 2.f);
+    for (int r = 1; r <= kFsItemsPerSm; ++r) {
+      int c = r * grid / base;
+      c = c < s.ty ? c : s.ty;
+      c = c < most ? c : most;
+      if (c <= 1) continue;
+      const int per = (s.ty + c - 1) / c, eff = (s.ty + per - 1) / per;
+      const float cost = float((base * eff + grid - 1) / grid) * (per + 5.f);
+      if (cost < best) {
+        best = cost;
+        s.splits = eff;
+        s.per = per;
+      }
+    }
+  }
+  s.items = base * s.splits;
+  return s;
+}
+
+// rows of partial results that any schedule for at most `nx` rows of X needs
+static int64_t fs_partial_rows(int64_t nx, int64_t ny, int grid) {
+  const int64_t tx = (nx + kFsTile - 1) / kFsTile, ty = std::max<int64_t>(1, (ny + kFsTile - 1) / kFsTile);
+  return std::max(tx, std::min<int64_t>(tx * ty, int64_t(kFsItemsPerSm) * grid)) * kFsTile;
+}
+
+struct FsParams {
+  const int* n_valid;      // rows of h that take part
+  int V, D;
+  int kb;                  // blocks of 64 columns
+  int x_resident, hold;    // X stays in shared memory; a streamed tile stays until ACC has read it
+  int grid;
+  const int* target;       // [Ppad] targets of the compacted rows
+  const float* bias;       // [Vpad] (-inf behind V), or null
+  float* part_acc;         // [splits, tx * 128, D]
+  float* part_m;           // [splits, 2, tx * 128]  running maximum (base 2) of a row's half tiles
+  float* part_l;           // [splits, 2, tx * 128]  sum; BWD: db
+  float* zt;               // [Ppad] score of the target (base 2)
+  const float* lse2;       // BWD [Ppad] (+inf behind n_valid)
+  const float* wex;        // BWD [Ppad] 1 - p_t
+  const float* gcol;       // BWD [Ppad] upstream gradient of every row, or null
+  const float* dloss;      // BWD scalar upstream gradient (with gcol: unused)
+  int mean;                // BWD: divide by n_valid
+  void* dw;                // BWD [V, D]
+  int dw_fp32;
+};
+
+__device__ __forceinline__ float fs_ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ uint32_t fs_pack(float lo, float hi) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+__device__ __forceinline__ void fs_bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)), "l"(src), "r"(bytes),
+               "r"(smem_u32(bar))
+               : "memory");
+}
+
+__host__ __device__ constexpr uint32_t fs_idesc(int n, bool b_mn) {
+  return (1u << 4) | (1u << 7) | (1u << 10) | (uint32_t(b_mn) << 16) | (uint32_t(n >> 3) << 17) | (uint32_t(kFsTile >> 4) << 24);
+}
+
+struct FsBars {
+  uint64_t full[kFsMaxUnits], empty[kFsMaxUnits];
+  uint64_t x_full, x_empty;
+  uint64_t s_full[2], p_full[2];
+  uint64_t acc_done[2], o_empty;  // acc_done by the tile's parity: a waiter may be one tile behind the last commit
+  uint64_t c_full[2], c_empty[2];
+  uint64_t xch[4], drain;
+  uint32_t tmem_base;
+  int abort_flag;
+};
+static_assert(sizeof(FsBars) + 2048 <= kFsExtra, "the shared memory behind the slots is too small");
+
+template <int MODE, bool BIAS, bool ROWG>
+__global__ void __launch_bounds__(kFsThreads, 1)
+full_softmax_kernel(const __grid_constant__ CUtensorMap tmapX, const __grid_constant__ CUtensorMap tmapY, const FsParams p) {
+  constexpr bool kAcc = MODE != FS_LSE;
+  constexpr uint32_t kTmemCols = kAcc ? 512 : 256;
+  extern __shared__ __align__(1024) uint8_t fs_smem[];
+  float* cols = reinterpret_cast<float*>(fs_smem + kFsSlots * kFsSlotBytes);  // 512 floats: FWD maxima [2][8][32]; BWD lse2 [2][128], g [2][128]
+  FsBars* B = reinterpret_cast<FsBars*>(cols + 512);
+  volatile int* abort_flag = &B->abort_flag;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int n_valid = *p.n_valid;
+  const int nx = MODE == FS_BWD ? p.V : n_valid, ny = MODE == FS_BWD ? n_valid : p.V;
+  const FsSchedule sc = fs_schedule(nx, ny, kAcc ? (p.D + kFsAcc - 1) / kFsAcc : 1, p.grid);
+  const int spu = p.kb == 1 ? 1 : 2;                       // slots of a unit of the ring
+  const int upt = (p.kb + spu - 1) / spu;                  // units of a streamed tile
+  const int x_slots = p.x_resident ? p.kb : 0;
+  const int units = min((kFsSlots - x_slots) / spu, kFsMaxUnits);
+  uint8_t* ring = fs_smem + x_slots * kFsSlotBytes;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kFsMaxUnits; ++i) {
+      mbar_init(&B->full[i], 1);
+      mbar_init(&B->empty[i], 1);
+    }
+    mbar_init(&B->x_full, 1);
+    mbar_init(&B->x_empty, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&B->s_full[i], 1);
+      mbar_init(&B->p_full[i], 8);
+      mbar_init(&B->acc_done[i], 1);
+      mbar_init(&B->c_full[i], 1);
+      mbar_init(&B->c_empty[i], 8);
+    }
+    mbar_init(&B->o_empty, 8);
+    for (int i = 0; i < 4; ++i) mbar_init(&B->xch[i], 2);
+    mbar_init(&B->drain, 1);
+    *abort_flag = 0;
+    // the swizzled descriptors want slots on 1024-byte boundaries
+    if ((smem_u32(fs_smem) & 1023) != 0) {
+      *abort_flag = 1;
+      atomicCAS(&g_fs_error, 0, FS_ERR_SMEM);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&B->tmem_base)), "r"(kTmemCols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tcgen05_fence_before();
+  __syncthreads();
+  tcgen05_fence_after();
+  const uint32_t tmem = B->tmem_base;
+  bool ok = *abort_flag == 0;
+
+  // item -> (tile of X, piece of the accumulator's columns, split of the streamed axis).  The split is the slow index: blocks that run
+  // together stream the same tiles, which then come from L2.
+  const int base = sc.tx * sc.pieces;
+
+  if (warp == 0) {
+    // ---------------- TMA producer ----------------
+    if (lane == 0) {
+      uint32_t uc = 0, item = 0, tc = 0;
+      auto load_unit = [&](const CUtensorMap* map, int u, int row) {
+        const uint32_t s = uc % units, ph = (uc / units) & 1;
+        if (!mbar_wait(&B->empty[s], ph ^ 1, abort_flag, &g_fs_error, FS_ERR_EMPTY)) return false;
+        const int n = min(spu, p.kb - u * spu);
+        mbar_expect_tx(&B->full[s], n * kFsSlotBytes);
+        for (int k = 0; k < n; ++k) tma_load_2d(ring + (s * spu + k) * kFsSlotBytes, map, &B->full[s], (u * spu + k) * 64, row);
+        ++uc;
+        return true;
+      };
+      for (int w = blockIdx.x; w < sc.items && ok; w += gridDim.x, ++item) {
+        const int split = w / base, rem = w - split * base, x = rem % sc.tx, piece = rem / sc.tx;
+        const int t0 = split * sc.per, nt = min(sc.ty, t0 + sc.per) - t0;
+        if (p.x_resident && nt > 0) {
+          if (item > 0 && !mbar_wait(&B->x_empty, (item - 1) & 1, abort_flag, &g_fs_error, FS_ERR_X)) { ok = false; break; }
+          mbar_expect_tx(&B->x_full, p.kb * kFsSlotBytes);
+          for (int k = 0; k < p.kb; ++k) tma_load_2d(fs_smem + k * kFsSlotBytes, &tmapX, &B->x_full, k * 64, x * kFsTile);
+        }
+        const int pu0 = piece * (kFsAcc / 128), pu1 = min(upt, pu0 + kFsAcc / 128);
+        for (int t = 0; t <= nt && ok; ++t) {
+          if (t < nt) {
+            if constexpr (MODE == FS_BWD) {
+              const int b = tc & 1;
+              if (!mbar_wait(&B->c_empty[b], ((tc >> 1) & 1) ^ 1, abort_flag, &g_fs_error, FS_ERR_COL)) { ok = false; break; }
+              mbar_expect_tx(&B->c_full[b], ROWG ? 1024 : 512);
+              fs_bulk_load(cols + b * 128, p.lse2 + int64_t(t0 + t) * kFsTile, 512, &B->c_full[b]);
+              if constexpr (ROWG) fs_bulk_load(cols + 256 + b * 128, p.gcol + int64_t(t0 + t) * kFsTile, 512, &B->c_full[b]);
+              ++tc;
+            }
+            for (int u = 0; u < upt && ok; ++u) {
+              if (!p.x_resident) ok = load_unit(&tmapX, u, x * kFsTile);
+              ok = ok && load_unit(&tmapY, u, (t0 + t) * kFsTile);
+            }
+          }
+          if (kAcc && !p.hold && t > 0)
+            for (int u = pu0; u < pu1 && ok; ++u) ok = load_unit(&tmapY, u, (t0 + t - 1) * kFsTile);
+        }
+      }
+      if (!ok) {
+        // copies may still be on their way into shared memory: give them a bounded time to land before the block may exit
+        const long long begin = clock64();
+        for (uint32_t j = uc > uint32_t(units) ? uc - units : 0; j < uc; ++j)
+          while (!mbar_try_wait(&B->full[j % units], (j / units) & 1) && clock64() - begin < kWaitCycles) {
+          }
+        if (p.x_resident && item < uint32_t(sc.items))
+          while (!mbar_try_wait(&B->x_full, item & 1) && clock64() - begin < kWaitCycles) {
+          }
+        if constexpr (MODE == FS_BWD)
+          for (uint32_t j = tc > 2 ? tc - 2 : 0; j < tc; ++j)
+            while (!mbar_try_wait(&B->c_full[j & 1], (j >> 1) & 1) && clock64() - begin < kWaitCycles) {
+            }
+      }
+    }
+  } else if (warp == 1) {
+    // ---------------- MMA issuer ----------------
+    // S(t + 1) is issued before ACC(t), so the tensor cores work while the softmax warps turn S(t) into E(t).
+    if (lane == 0) {
+      uint32_t uc = 0, item = 0, tc = 0;  // tc: tile whose S is issued next
+      constexpr uint32_t idesc_s = fs_idesc(kFsTile, false);
+      for (int w = blockIdx.x; w < sc.items && ok; w += gridDim.x, ++item) {
+        const int split = w / base, rem = w - split * base, piece = rem / sc.tx;
+        const int t0 = split * sc.per, nt = min(sc.ty, t0 + sc.per) - t0;
+        if (p.x_resident && nt > 0 && !mbar_wait(&B->x_full, item & 1, abort_flag, &g_fs_error, FS_ERR_X)) { ok = false; break; }
+        const int pu0 = piece * (kFsAcc / 128), pu1 = min(upt, pu0 + kFsAcc / 128);
+        uint32_t held[2] = {0, 0};  // first unit of a held tile
+        for (int t = 0; t <= nt && ok; ++t) {
+          if (t < nt) {
+            const int b = tc & 1;
+            // the buffer's previous tile: with ACC its E was consumed by an MMA issued before this one; without, its readers must be done
+            if (!kAcc && tc >= 2 && !mbar_wait(&B->p_full[b], ((tc >> 1) - 1) & 1, abort_flag, &g_fs_error, FS_ERR_P)) { ok = false; break; }
+            tcgen05_fence_after();
+            const uint32_t d = tmem + b * kFsTile;
+            held[t & 1] = uc;
+            for (int u = 0; u < upt && ok; ++u) {
+              const uint32_t xs = uc % units;
+              if (!p.x_resident) {
+                if (!mbar_wait(&B->full[xs], (uc / units) & 1, abort_flag, &g_fs_error, FS_ERR_FULL)) { ok = false; break; }
+                ++uc;
+              }
+              const uint32_t ys = uc % units;
+              if (!mbar_wait(&B->full[ys], (uc / units) & 1, abort_flag, &g_fs_error, FS_ERR_FULL)) { ok = false; break; }
+              ++uc;
+              tcgen05_fence_after();
+              const int n = min(spu, p.kb - u * spu);
+              for (int k = 0; k < n; ++k) {
+                const int col0 = (u * spu + k) * 64;
+                const uint32_t ax = smem_u32(p.x_resident ? fs_smem + (u * spu + k) * kFsSlotBytes : ring + (xs * spu + k) * kFsSlotBytes);
+                const uint32_t by = smem_u32(ring + (ys * spu + k) * kFsSlotBytes);
+                const int steps = min(4, (p.D - col0 + 15) / 16);
+                for (int i = 0; i < steps; ++i)
+                  umma_bf16(d, make_smem_desc(ax + i * 32, 16, 1024), make_smem_desc(by + i * 32, 16, 1024), idesc_s, (col0 > 0 || i > 0) ? 1u : 0u);
+              }
+              if (!p.x_resident) tcgen05_commit(&B->empty[xs]);
+              if (!p.hold) tcgen05_commit(&B->empty[ys]);
+            }
+            if (!ok) break;
+            tcgen05_commit(&B->s_full[b]);
+            if (p.x_resident && t == nt - 1) tcgen05_commit(&B->x_empty);
+            ++tc;
+          }
+          if (kAcc && t > 0) {
+            const uint32_t tt = (t < nt) ? tc - 2 : tc - 1;  // tile whose E is multiplied now
+            if (t == 1 && item > 0 && !mbar_wait(&B->o_empty, (item - 1) & 1, abort_flag, &g_fs_error, FS_ERR_ACC)) { ok = false; break; }
+            if (!mbar_wait(&B->p_full[tt & 1], (tt >> 1) & 1, abort_flag, &g_fs_error, FS_ERR_P)) { ok = false; break; }
+            tcgen05_fence_after();
+            const uint32_t e = tmem + (tt & 1) * kFsTile;
+            for (int u = pu0; u < pu1 && ok; ++u) {
+              uint32_t s;
+              if (p.hold) {
+                s = (held[(t - 1) & 1] + u) % units;
+              } else {
+                s = uc % units;
+                if (!mbar_wait(&B->full[s], (uc / units) & 1, abort_flag, &g_fs_error, FS_ERR_FULL)) { ok = false; break; }
+                ++uc;
+                tcgen05_fence_after();
+              }
+              const int n = min(64 * spu, (p.D - u * 64 * spu + 15) / 16 * 16);
+              const uint32_t idesc = fs_idesc(n, true);
+              const uint32_t by = smem_u32(ring + s * spu * kFsSlotBytes);
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+                umma_bf16_ts(tmem + 256 + (u - pu0) * 128, e + (i < 4 ? i * 8 : 64 + (i - 4) * 8), make_smem_desc(by + i * 2048, kFsSlotBytes, 1024), idesc,
+                             (t > 1 || i > 0) ? 1u : 0u);
+              tcgen05_commit(&B->empty[s]);
+            }
+            if (ok) tcgen05_commit(&B->acc_done[tt & 1]);
+          }
+        }
+      }
+      if (!ok) {  // products already issued must end before the tensor memory is freed
+        tcgen05_commit(&B->drain);
+        const long long begin = clock64();
+        while (!mbar_try_wait(&B->drain, 0) && clock64() - begin < kWaitCycles) {
+        }
+      }
+    }
+  } else {
+    // ---------------- softmax warps (2..9) ----------------
+    // Two warps share the 32 rows of a TMEM lane quarter (warp % 4) and take 64 columns each; a thread owns one row.
+    const int q = warp & 3, half = (warp - 2) >> 2, ew = warp - 2;
+    const uint32_t lanes = uint32_t(q * 32) << 16;
+    uint32_t item = 0, tc = 0;
+    auto wait_all = [&](uint64_t* bar, uint32_t parity, int code) {
+      return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, &g_fs_error, code)) != 0;
+    };
+    for (int w = blockIdx.x; w < sc.items && ok; w += gridDim.x, ++item) {
+      const int split = w / base, rem = w - split * base, x = rem % sc.tx, piece = rem / sc.tx;
+      const int t0 = split * sc.per, nt = min(sc.ty, t0 + sc.per) - t0;
+      const int row = x * kFsTile + q * 32 + lane;  // FWD: compacted row of h; BWD: item
+      const int64_t prow = int64_t(sc.tx) * kFsTile;  // rows of one split's partial results
+      int tgt = -1;
+      float bias_row = 0.f;
+      if constexpr (MODE == FS_BWD) {
+        if constexpr (BIAS) bias_row = p.bias[row] * kLog2e;  // padded to whole tiles
+      } else {
+        tgt = p.target[row];
+      }
+      float m2 = -INFINITY, l = 0.f;
+      for (int t = 0; t < nt && ok; ++t, ++tc) {
+        const int b = tc & 1;
+        const int col0 = (t0 + t) * kFsTile + half * 64;  // first of this warp's 64 columns
+        int tc0 = -1, tc1 = -1;
+        if constexpr (MODE == FS_BWD) {  // targets of the 64 rows of h, two per lane
+          tc0 = p.target[col0 + lane];
+          tc1 = p.target[col0 + 32 + lane];
+        }
+        if (!wait_all(&B->s_full[b], (tc >> 1) & 1, FS_ERR_S)) { ok = false; break; }
+        tcgen05_fence_after();
+        const uint32_t ts = tmem + lanes + b * kFsTile + half * 64;
+        uint32_t r0[32], r1[32];
+        tmem_ld_32x32_issue(ts, r0);
+        tmem_ld_32x32_issue(ts + 32, r1);
+        tmem_ld_wait(r0);
+        tmem_ld_wait(r1);
+        if constexpr (!kAcc) {
+          tcgen05_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&B->p_full[b]);
+        }
+        float z[64];
+#pragma unroll
+        for (int j = 0; j < 32; ++j) {
+          z[j] = __uint_as_float(r0[j]);
+          z[32 + j] = __uint_as_float(r1[j]);
+        }
+        if constexpr (MODE != FS_BWD) {
+          if constexpr (BIAS) {
+            const float4* bp = reinterpret_cast<const float4*>(p.bias + col0);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              const float4 v = __ldg(bp + j);
+              z[4 * j] += v.x;
+              z[4 * j + 1] += v.y;
+              z[4 * j + 2] += v.z;
+              z[4 * j + 3] += v.w;
+            }
+          } else if (col0 + 64 > p.V) {
+#pragma unroll
+            for (int j = 0; j < 64; ++j)
+              if (col0 + j >= p.V) z[j] = -INFINITY;
+          }
+          const int rel = tgt - col0;
+          const bool hit = rel >= 0 && rel < 64 && tgt >= 0;
+          if (__any_sync(0xffffffffu, hit)) {
+#pragma unroll
+            for (int j = 0; j < 64; ++j)
+              if (hit && j == rel) {
+                if (piece == 0) p.zt[row] = z[j] * kLog2e;
+                z[j] = -INFINITY;
+              }
+          }
+          float mx[4] = {z[0], z[1], z[2], z[3]};
+#pragma unroll
+          for (int j = 4; j < 64; ++j) mx[j & 3] = fmaxf(mx[j & 3], z[j]);
+          float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * kLog2e;
+          if constexpr (MODE == FS_FWD) {
+            // both halves of a row scale by the same maximum
+            cols[(b * 8 + ew) * 32 + lane] = mt;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&B->xch[q]);
+            if (!wait_all(&B->xch[q], tc & 1, FS_ERR_XCH)) { ok = false; break; }
+            mt = fmaxf(mt, cols[(b * 8 + (ew ^ 4)) * 32 + lane]);
+            const bool raise = mt > m2 + kRaise || (t == 0);
+            if (__any_sync(0xffffffffu, raise)) {
+              const float mn = raise ? fmaxf(mt, m2) : m2;
+              const float f = (m2 == mn) ? 1.f : fs_ex2(m2 - mn);
+              l *= f;
+              m2 = mn;
+              if (t > 0) {
+                // rescale this warp's share of the accumulator: every ACC up to the previous tile has to be complete
+                if (!wait_all(&B->acc_done[(tc - 1) & 1], ((tc - 1) >> 1) & 1, FS_ERR_ACC)) { ok = false; break; }
+                tcgen05_fence_after();
+                const int groups = (min(kFsAcc, p.D - piece * kFsAcc) + 31) / 32;
+                for (int g = half; g < groups; g += 2) {
+                  const uint32_t to = tmem + lanes + 256 + g * 32;
+                  uint32_t a[32];
+                  tmem_ld_32x32_issue(to, a);
+                  tmem_ld_wait(a);
+#pragma unroll
+                  for (int j = 0; j < 32; ++j) a[j] = __float_as_uint(__uint_as_float(a[j]) * f);
+                  tmem_st_32x32(to, a);
+                }
+                tmem_st_wait();
+              }
+            }
+          } else {
+            const float mn = fmaxf(m2, mt);
+            if (mn > m2) l *= fs_ex2(m2 - mn);
+            m2 = mn;
+          }
+          const float ms = m2 == -INFINITY ? 0.f : m2;
+          float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int j = 0; j < 64; ++j) {
+            z[j] = fs_ex2(fmaf(z[j], kLog2e, -ms));
+            sum[j & 3] += z[j];
+          }
+          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        } else {
+          if (!wait_all(&B->c_full[b], (tc >> 1) & 1, FS_ERR_COL)) { ok = false; break; }
+          const float4* lp = reinterpret_cast<const float4*>(cols + b * 128 + half * 64);
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            const float4 v = lp[j];
+            z[4 * j] = fs_ex2(fmaf(z[4 * j], kLog2e, bias_row) - v.x);
+            z[4 * j + 1] = fs_ex2(fmaf(z[4 * j + 1], kLog2e, bias_row) - v.y);
+            z[4 * j + 2] = fs_ex2(fmaf(z[4 * j + 2], kLog2e, bias_row) - v.z);
+            z[4 * j + 3] = fs_ex2(fmaf(z[4 * j + 3], kLog2e, bias_row) - v.w);
+          }
+          // entries (item, row of h) with the row's target: p - 1 = -(1 - p_t)
+          const int v0 = x * kFsTile + q * 32;
+          uint32_t h0 = __ballot_sync(0xffffffffu, tc0 >= v0 && tc0 < v0 + 32), h1 = __ballot_sync(0xffffffffu, tc1 >= v0 && tc1 < v0 + 32);
+          if (h0 | h1) {
+#pragma unroll
+            for (int j = 0; j < 64; ++j) {
+              if (((j < 32 ? h0 : h1) >> (j & 31)) & 1u) {
+                const int owner = __shfl_sync(0xffffffffu, j < 32 ? tc0 : tc1, j & 31) - v0;
+                if (lane == owner) z[j] = -__ldg(p.wex + col0 + j);
+              }
+            }
+          }
+          if constexpr (ROWG) {
+            const float4* gp = reinterpret_cast<const float4*>(cols + 256 + b * 128 + half * 64);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              const float4 v = gp[j];
+              z[4 * j] *= v.x;
+              z[4 * j + 1] *= v.y;
+              z[4 * j + 2] *= v.z;
+              z[4 * j + 3] *= v.w;
+            }
+          }
+          if constexpr (BIAS) {
+            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int j = 0; j < 64; ++j) sum[j & 3] += z[j];
+            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&B->c_empty[b]);
+        }
+        if constexpr (kAcc) {
+          // E in bf16 over the first half of the score columns that this warp read
+          uint32_t e[32];
+#pragma unroll
+          for (int j = 0; j < 32; ++j) e[j] = fs_pack(z[2 * j], z[2 * j + 1]);
+          tmem_st_32x32(ts, e);
+          tmem_st_wait();
+          tcgen05_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&B->p_full[b]);
+        }
+      }
+      if (!ok) break;
+      // ---- end of the item ----
+      if (piece == 0 && (MODE != FS_BWD || BIAS)) {
+        const int64_t at = (int64_t(split) * 2 + half) * prow + row;
+        p.part_l[at] = l;
+        if constexpr (MODE != FS_BWD) p.part_m[at] = m2;
+      }
+      if constexpr (kAcc) {
+        if (nt > 0) {
+          if (!wait_all(&B->acc_done[(tc - 1) & 1], ((tc - 1) >> 1) & 1, FS_ERR_ACC)) { ok = false; break; }
+          tcgen05_fence_after();
+        }
+        const int width = min(kFsAcc, p.D - piece * kFsAcc);
+        const bool direct = MODE == FS_BWD && sc.splits == 1;
+        float scale = 1.f;
+        if (direct && !ROWG) scale = *p.dloss / (p.mean ? float(max(n_valid, 1)) : 1.f);
+        for (int g = half; g * 32 < width; g += 2) {
+          uint32_t a[32];
+          if (nt > 0) {
+            tmem_ld_32x32_issue(tmem + lanes + 256 + g * 32, a);
+            tmem_ld_wait(a);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) a[j] = 0u;
+          }
+          const int c0 = piece * kFsAcc + g * 32;
+#pragma unroll
+          for (int j = 0; j < 32; j += 8) {
+            if (row >= nx || c0 + j >= p.D) continue;  // D % 8 == 0
+            float v[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = __uint_as_float(a[j + k]) * scale;
+            if (!direct || p.dw_fp32) {
+              float* o = direct ? reinterpret_cast<float*>(p.dw) + int64_t(row) * p.D + c0 + j : p.part_acc + (int64_t(split) * prow + row) * p.D + c0 + j;
+              *reinterpret_cast<float4*>(o) = make_float4(v[0], v[1], v[2], v[3]);
+              *reinterpret_cast<float4*>(o + 4) = make_float4(v[4], v[5], v[6], v[7]);
+            } else {
+              uint4 o = make_uint4(fs_pack(v[0], v[1]), fs_pack(v[2], v[3]), fs_pack(v[4], v[5]), fs_pack(v[6], v[7]));
+              *reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(p.dw) + int64_t(row) * p.D + c0 + j) = o;
+            }
+          }
+          __syncwarp();
+        }
+        tcgen05_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&B->o_empty);
+      }
+    }
+  }
+
+  tcgen05_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tcgen05_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+  }
+}
+
+// ---- before the forward -----------------------------------------------------------------------------
+// Blocks 0..row_blocks-1 put the rows whose target counts one behind the other (in their order), as bf16 with zero columns up to Dp;
+// slot[i] is row i's place or -1.  The remaining blocks copy the bias with -inf behind V.  Every row block counts the targets before
+// its own itself: P targets are at most a few hundred KB in L2, cheaper than another launch.
+constexpr int kPrepRows = 512;
+
+struct PrepParams {
+  const void* h;
+  int64_t h_row, h_col;  // strides
+  int h_fp32, vec;
+  const int64_t* targets;
+  int64_t t_stride, ignore;
+  int P, V, D, Dp;
+  __nv_bfloat16* hc;
+  int* n_valid;
+  int* slot;
+  int* target;
+  float* loss_rows;
+  const float* bias_in;
+  float* bias_out;
+  int row_blocks;
+};
+
+__device__ __forceinline__ int fs_target_kind(int64_t t, const PrepParams& p) { return t == p.ignore ? 0 : (t < 0 || t >= p.V ? 2 : 1); }
+
+__global__ void __launch_bounds__(kPrepRows) full_softmax_prep_kernel(const PrepParams p) {
+  if (int(blockIdx.x) >= p.row_blocks) {
+    const int vpad = (p.V + kFsTile - 1) / kFsTile * kFsTile;
+    for (int v = (blockIdx.x - p.row_blocks) * kPrepRows + threadIdx.x; v < vpad; v += (gridDim.x - p.row_blocks) * kPrepRows)
+      p.bias_out[v] = v < p.V ? p.bias_in[v] : -INFINITY;
+    return;
+  }
+  __shared__ int counts[kPrepRows / 32];
+  __shared__ int slots[kPrepRows];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int begin = blockIdx.x * kPrepRows, row = begin + threadIdx.x;
+  int before = 0;
+  for (int i = threadIdx.x; i < begin; i += kPrepRows) before += fs_target_kind(p.targets[i * p.t_stride], p) == 1;
+  const int64_t t = row < p.P ? p.targets[row * p.t_stride] : p.ignore;
+  const int kind = row < p.P ? fs_target_kind(t, p) : 0;
+  const uint32_t mine = __ballot_sync(0xffffffffu, kind == 1);
+  const int in_warp = __popc(mine & ((1u << lane) - 1));
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
+  // base of the block: the sum of every warp's `before`; base of the warp: the valid rows of the warps in front
+  if (lane == 0) {
+    counts[warp] = __popc(mine);
+    slots[warp] = before;
+  }
+  __syncthreads();
+  int first = 0, total = 0;
+#pragma unroll
+  for (int w = 0; w < kPrepRows / 32; ++w) {
+    total += slots[w];
+    if (w < warp) first += counts[w];
+  }
+  int block_valid = 0;
+#pragma unroll
+  for (int w = 0; w < kPrepRows / 32; ++w) block_valid += counts[w];
+  __syncthreads();
+  const int at = kind == 1 ? total + first + in_warp : -1;
+  slots[threadIdx.x] = at;
+  if (row < p.P) {
+    p.slot[row] = at;
+    if (at >= 0) p.target[at] = int(t);
+    p.loss_rows[row] = kind == 2 ? __int_as_float(0x7fc00000) : 0.f;
+    if (kind == 2) atomicCAS(&g_fs_error, 0, FS_ERR_TARGET);
+  }
+  __syncthreads();
+  const bool last = int(blockIdx.x) == p.row_blocks - 1;
+  const int n = total + block_valid, padded = (n + kFsTile - 1) / kFsTile * kFsTile;
+  if (last) {
+    if (threadIdx.x == 0) *p.n_valid = n;
+    if (n + int(threadIdx.x) < padded) p.target[n + threadIdx.x] = -1;
+  }
+  const int vecs = p.Dp / 8;
+  const int rows = min(kPrepRows, p.P - begin);
+  // eight columns at a time
+  for (int i = threadIdx.x; i < rows * vecs; i += kPrepRows) {
+    const int r = i / vecs, c = (i - r * vecs) * 8, to = slots[r];
+    if (to < 0) continue;
+    uint4 o;
+    if (p.vec && !p.h_fp32) {
+      o = *reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(p.h) + int64_t(begin + r) * p.h_row + c);
+    } else {
+      float v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int64_t e = int64_t(begin + r) * p.h_row + int64_t(c + k) * p.h_col;
+        v[k] = c + k < p.D ? (p.h_fp32 ? reinterpret_cast<const float*>(p.h)[e] : __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p.h)[e])) : 0.f;
+      }
+      o = make_uint4(fs_pack(v[0], v[1]), fs_pack(v[2], v[3]), fs_pack(v[4], v[5]), fs_pack(v[6], v[7]));
+    }
+    *reinterpret_cast<uint4*>(p.hc + int64_t(to) * p.Dp + c) = o;
+  }
+  if (last)
+    for (int i = threadIdx.x; i < (padded - n) * vecs; i += kPrepRows) *reinterpret_cast<uint4*>(p.hc + int64_t(n) * p.Dp + int64_t(i) * 8) = make_uint4(0, 0, 0, 0);
+}
+
+// ---- after the forward: join the splits of every row --------------------------------------------------
+// One block per row: the splits' weights 2^(m_s - max) go to shared memory, then the threads walk (group of splits, 4 columns).
+constexpr int kJoinThreads = 128;
+
+template <bool ACC>
+__global__ void __launch_bounds__(kJoinThreads) full_softmax_join_kernel(const int* __restrict__ n_valid_p, int V, int D, int grid, int pieces, const float* __restrict__ part_acc,
+                                                                         const float* __restrict__ part_m, const float* __restrict__ part_l, const float* __restrict__ zt,
+                                                                         const int* __restrict__ target, const __nv_bfloat16* __restrict__ W, int64_t ldw,
+                                                                         float* __restrict__ lse2, float* __restrict__ wex, float* __restrict__ loss_c, float* __restrict__ unit) {
+  extern __shared__ __align__(16) float js[];  // [splits] weights, then [threads * 4] partial sums
+  const int n = *n_valid_p, row = blockIdx.x;
+  const int padded = (n + kFsTile - 1) / kFsTile * kFsTile;
+  if (row >= padded) return;
+  if (row >= n) {  // a streamed row of zeros: exp(0 - inf) = 0
+    if (threadIdx.x == 0) lse2[row] = INFINITY;
+    return;
+  }
+  const FsSchedule sc = fs_schedule(n, V, pieces, grid);
+  const int64_t prow = int64_t(sc.tx) * kFsTile;
+  __shared__ float red[kJoinThreads / 32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  float m = -INFINITY;
+  for (int s = threadIdx.x; s < 2 * sc.splits; s += kJoinThreads) m = fmaxf(m, part_m[s * prow + row]);
+  m = warp_max(m);
+  if (lane == 0) red[warp] = m;
+  __syncthreads();
+  m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  __syncthreads();
+  const float ms = m == -INFINITY ? 0.f : m;
+  float l = 0.f;
+  for (int s = threadIdx.x; s < 2 * sc.splits; s += kJoinThreads) {
+    const float f = exp2f(part_m[s * prow + row] - ms);
+    l += f * part_l[s * prow + row];
+    if (ACC && !(s & 1)) js[s >> 1] = f;
+  }
+  l = warp_sum(l);
+  if (lane == 0) red[warp] = l;
+  __syncthreads();
+  l = (red[0] + red[1]) + (red[2] + red[3]);
+  // others' log sum a, target's score z (base 2): lse = max + log2(1 + 2^-|a - z|)
+  const float a = ms + log2f(l), z = zt[row], d = a - z;
+  const float tail = log1pf(exp2f(-fabsf(d)));
+  const float loss = (d > 0.f ? d * kLn2 : 0.f) + tail;
+  const float w = d > 0.f ? 1.f / (1.f + exp2f(-d)) : exp2f(d) / (1.f + exp2f(d));  // 1 - p_t
+  if (threadIdx.x == 0) {
+    lse2[row] = fmaxf(a, z) + tail * kLog2e;
+    wex[row] = w;
+    loss_c[row] = d != d ? d : loss;
+  }
+  if constexpr (ACC) {
+    float4* buf = reinterpret_cast<float4*>(js + ((sc.splits + 3) & ~3));
+    const int vecs = D / 4;
+    int lanes = 1;
+    while (lanes < vecs && lanes < kJoinThreads) lanes <<= 1;
+    const int groups = sc.splits > 1 ? kJoinThreads / lanes : 1;
+    const int g = threadIdx.x / lanes, c = threadIdx.x % lanes;
+    const float inv = l > 0.f ? w / l : (l == 0.f ? 0.f : l);
+    const int64_t t = target[row];
+    for (int v0 = 0; v0 < vecs; v0 += lanes) {
+      const int v = v0 + c;
+      float4 s4 = f4zero();
+      if (v < vecs && g < groups)
+        for (int s = g; s < sc.splits; s += groups) {
+          const float4 x = *reinterpret_cast<const float4*>(part_acc + (s * prow + row) * D + v * 4);
+          const float f = js[s];
+          s4.x += f * x.x;
+          s4.y += f * x.y;
+          s4.z += f * x.z;
+          s4.w += f * x.w;
+        }
+      if (groups > 1) {
+        buf[threadIdx.x] = s4;
+        __syncthreads();
+        if (g == 0)
+          for (int k = 1; k < groups; ++k) {
+            const float4 x = buf[k * lanes + c];
+            s4.x += x.x;
+            s4.y += x.y;
+            s4.z += x.z;
+            s4.w += x.w;
+          }
+        __syncthreads();
+      }
+      if (g == 0 && v < vecs) {
+        const float4 wt = Vec4<__nv_bfloat16>::load(W + t * ldw + v * 4);
+        *reinterpret_cast<float4*>(unit + int64_t(row) * D + v * 4) =
+            make_float4(s4.x * inv - w * wt.x, s4.y * inv - w * wt.y, s4.z * inv - w * wt.z, s4.w * inv - w * wt.w);
+      }
+    }
+  }
+}
+
+// rows' losses at their own places, and their sum in a fixed order (one block: P values)
+__global__ void __launch_bounds__(1024) full_softmax_reduce_kernel(int P, const int* __restrict__ n_valid, const int* __restrict__ slot, const float* __restrict__ loss_c,
+                                                                   float* __restrict__ rows, float* __restrict__ out, int mean) {
+  __shared__ float red[32];
+  float s = 0.f;
+  for (int i = threadIdx.x; i < P; i += 1024) {
+    const int at = slot[i];
+    s += at >= 0 ? loss_c[at] : rows[i];
+  }
+  s = warp_sum(s);
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = s;
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    s = warp_sum(red[threadIdx.x]);
+    if (threadIdx.x == 0) *out = mean ? s / float(max(*n_valid, 1)) : s;
+  }
+}
+
+__global__ void full_softmax_rows_kernel(int P, const int* __restrict__ slot, const float* __restrict__ loss_c, float* __restrict__ rows) {
+  const int i = blockIdx.x * blockDim.x + threadIdx.x;
+  if (i < P && slot[i] >= 0) rows[i] = loss_c[slot[i]];
+}
+
+// ---- backward: dh = g * unit at the rows' own places, and the per-row factors of the compacted rows --------
+template <typename T>
+__global__ void full_softmax_dh_kernel(int P, int D, int Dp, const int* __restrict__ n_valid, const int* __restrict__ slot, const float* __restrict__ unit,
+                                       const float* __restrict__ dloss, int64_t dl_stride, int per_row, int mean, T* __restrict__ dh, float* __restrict__ gcol) {
+  const int vecs = Dp / 8;
+  const int64_t idx = int64_t(blockIdx.x) * blockDim.x + threadIdx.x;
+  const int n = *n_valid;
+  if (gcol != nullptr && blockIdx.x == 0) {
+    const int padded = (n + kFsTile - 1) / kFsTile * kFsTile;
+    if (n + int(threadIdx.x) < padded) gcol[n + threadIdx.x] = 0.f;  // 256 threads cover the at most 127 rows
+  }
+  const int64_t row = idx / vecs;
+  if (row >= P) return;
+  const int c = int(idx - row * vecs) * 8;
+  const int at = slot[row];
+  const float g = per_row ? dloss[row * dl_stride] : *dloss / (mean ? float(max(n, 1)) : 1.f);
+  if (gcol != nullptr && c == 0 && at >= 0) gcol[at] = g;
+  if (dh == nullptr) return;
+  float v[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) v[k] = 0.f;
+  if (at >= 0) {
+    const float4* u = reinterpret_cast<const float4*>(unit + int64_t(at) * Dp + c);
+    const float4 a = u[0], b = u[1];
+    v[0] = a.x * g; v[1] = a.y * g; v[2] = a.z * g; v[3] = a.w * g;
+    v[4] = b.x * g; v[5] = b.y * g; v[6] = b.z * g; v[7] = b.w * g;
+  }
+  T* o = dh + row * D + c;
+  if (D == Dp) {
+    if constexpr (sizeof(T) == 2) {
+      *reinterpret_cast<uint4*>(o) = make_uint4(fs_pack(v[0], v[1]), fs_pack(v[2], v[3]), fs_pack(v[4], v[5]), fs_pack(v[6], v[7]));
+    } else {
+      reinterpret_cast<float4*>(o)[0] = make_float4(v[0], v[1], v[2], v[3]);
+      reinterpret_cast<float4*>(o)[1] = make_float4(v[4], v[5], v[6], v[7]);
+    }
+  } else {
+    for (int k = 0; k < 8 && c + k < D; ++k) o[k] = T(v[k]);
+  }
+}
+
+// ---- backward: join the splits of dW, and db ----------------------------------------------------------------
+template <typename T>
+__global__ void full_softmax_dw_kernel(const int* __restrict__ n_valid, int V, int D, int grid, int pieces, const float* __restrict__ part_acc, const float* __restrict__ dloss,
+                                       int per_row, int mean, T* __restrict__ dw) {
+  const FsSchedule sc = fs_schedule(V, *n_valid, pieces, grid);
+  if (sc.splits == 1) return;  // written by the main kernel
+  const int64_t stride = int64_t(sc.tx) * kFsTile * D;
+  const float scale = per_row ? 1.f : *dloss / (mean ? float(max(*n_valid, 1)) : 1.f);
+  for (int64_t i = (int64_t(blockIdx.x) * blockDim.x + threadIdx.x) * 4; i < int64_t(V) * D; i += int64_t(gridDim.x) * blockDim.x * 4) {
+    float4 s4 = f4zero();
+    for (int s = 0; s < sc.splits; ++s) {
+      const float4 x = *reinterpret_cast<const float4*>(part_acc + s * stride + i);
+      s4.x += x.x;
+      s4.y += x.y;
+      s4.z += x.z;
+      s4.w += x.w;
+    }
+    Vec4<T>::store(dw + i, make_float4(s4.x * scale, s4.y * scale, s4.z * scale, s4.w * scale));
+  }
+}
+
+__global__ void full_softmax_db_kernel(const int* __restrict__ n_valid, int V, int grid, int pieces, const float* __restrict__ part_l, const float* __restrict__ dloss, int per_row,
+                                       int mean, float* __restrict__ db) {
+  const FsSchedule sc = fs_schedule(V, *n_valid, pieces, grid);
+  const int v = blockIdx.x * blockDim.x + threadIdx.x;
+  if (v >= V) return;
+  const int64_t prow = int64_t(sc.tx) * kFsTile;
+  float s = 0.f;
+  for (int k = 0; k < 2 * sc.splits; ++k) s += part_l[k * prow + v];
+  db[v] = per_row ? s : s * (*dloss / (mean ? float(max(*n_valid, 1)) : 1.f));
+}
+
+// ---- host ---------------------------------------------------------------------------------------------------
+static int fs_grid(const at::Device& dev) {
+  return at::cuda::getDeviceProperties(dev.index())->multiProcessorCount;
+}
+
+template <int MODE, bool BIAS, bool ROWG>
+static void fs_launch(const CUtensorMap& tx, const CUtensorMap& ty, const FsParams& p) {
+  auto kernel = full_softmax_kernel<MODE, BIAS, ROWG>;
+  TRB_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kFsSmem));
+  kernel<<<p.grid, kFsThreads, kFsSmem, at::cuda::getCurrentCUDAStream()>>>(tx, ty, p);
+  TRB_CUDA_CHECK(cudaGetLastError());
+}
+
+static void fs_shape(FsParams& p, int64_t V, int64_t D, bool acc) {
+  p.V = int(V);
+  p.D = int(D);
+  p.kb = int((D + 63) / 64);
+  p.x_resident = p.kb <= 8;       // with up to 8 of 14 slots for X the ring keeps three units of two blocks
+  p.hold = acc && p.kb <= 4;      // two tiles of four blocks, X and one more unit fit
+}
+
+constexpr int64_t kFsMaxRows = (int64_t(1) << 31) - 2 * kFsTile;
+
+static void fs_check_weight(const at::Tensor& w) {
+  TORCH_CHECK(w.is_cuda() && w.scalar_type() == at::kBFloat16 && w.dim() == 2 && w.stride(1) == 1 && w.size(0) >= 1 && w.size(0) < kFsMaxRows,
+              "full_softmax: the weight is a bf16 [V, D] matrix with contiguous rows");
+  TORCH_CHECK(w.size(1) >= 8 && w.size(1) % 8 == 0 && w.size(1) <= kFsMaxD && w.stride(0) % 8 == 0 && w.stride(0) >= w.size(1) &&
+                  reinterpret_cast<uintptr_t>(w.data_ptr()) % 16 == 0,
+              "full_softmax: D and the row pitch of the weight are multiples of 8 (D at most ", kFsMaxD, "), its rows start on 16 bytes");
+}
+
+// h [P, D] bf16 or fp32 (any strides), weight [V, Dp] bf16 with Dp = D rounded up to 8 (zero columns behind D), targets [P] int64,
+// bias [V] fp32 or none.  reduction: 0 none, 1 mean, 2 sum.  grad: 0 loss only, 1 prepare the backward of W and b, 2 of h too.
+// Returns (loss, hc, meta, stat, unit): the compacted rows [Ppad, Dp], meta = n_valid (4 ints) | targets [Ppad] | slot [P], stat =
+// lse2 [Ppad] | 1 - p_t [Ppad] | padded bias, unit [Ppad, Dp] = dh without the upstream factor (empty unless grad == 2).
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> full_softmax_fwd(const at::Tensor& h, const at::Tensor& weight, const at::Tensor& targets,
+                                                                                        const c10::optional<at::Tensor>& bias, int64_t ignore_index, int64_t reduction,
+                                                                                        int64_t grad) {
+  fs_check_weight(weight);
+  TORCH_CHECK(h.is_cuda() && h.dim() == 2 && (h.scalar_type() == at::kBFloat16 || h.scalar_type() == at::kFloat), "full_softmax: h is bf16 or fp32 [P, D]");
+  TORCH_CHECK(targets.is_cuda() && targets.dim() == 1 && targets.scalar_type() == at::kLong && targets.size(0) == h.size(0), "full_softmax: targets is int64 [P]");
+  TORCH_CHECK(h.device() == weight.device() && h.device() == targets.device(), "full_softmax: operands on different devices");
+  TORCH_CHECK(reduction >= 0 && reduction <= 2 && grad >= 0 && grad <= 2);
+  const int64_t P = h.size(0), D = h.size(1), V = weight.size(0), Dp = weight.size(1);
+  TORCH_CHECK(P < kFsMaxRows && D >= 1 && D <= Dp && Dp - D < 8, "full_softmax: h and weight differ in width");
+  const bool has_bias = bias.has_value() && bias->defined();
+  if (has_bias)
+    TORCH_CHECK(bias->is_cuda() && bias->device() == h.device() && bias->scalar_type() == at::kFloat && bias->dim() == 1 && bias->size(0) == V && bias->is_contiguous(),
+                "full_softmax: bias is fp32 [V]");
+  c10::cuda::CUDAGuard guard(h.device());
+  auto stream = at::cuda::getCurrentCUDAStream();
+  const int64_t Ppad = (P + kFsTile - 1) / kFsTile * kFsTile, Vpad = (V + kFsTile - 1) / kFsTile * kFsTile;
+  const auto f32 = h.options().dtype(at::kFloat);
+  at::Tensor hc = at::empty({Ppad, Dp}, h.options().dtype(at::kBFloat16));
+  at::Tensor meta = at::empty({4 + Ppad + P}, h.options().dtype(at::kInt));
+  at::Tensor stat = at::empty({2 * Ppad + (has_bias ? Vpad : 0)}, f32);
+  at::Tensor unit = at::empty({grad == 2 ? Ppad : 0, Dp}, f32);
+  at::Tensor rows = at::empty({P}, f32);
+  if (P == 0) {
+    meta.zero_();
+    return {reduction == 0 ? rows : at::zeros({}, f32), hc, meta, stat, unit};
+  }
+  const int grid = fs_grid(h.device());
+  const bool acc = grad == 2;
+  const int pieces = acc ? int((Dp + kFsAcc - 1) / kFsAcc) : 1;
+  const int64_t prows = fs_partial_rows(P, V, grid);
+  at::Tensor part_acc = acc ? at::empty({prows, Dp}, f32) : at::Tensor();
+  at::Tensor part = at::empty({4 * prows + 2 * Ppad}, f32);  // maxima, sums (two halves each); targets' scores, compacted losses
+  float* part_m = part.data_ptr<float>();
+  float* part_l = part_m + 2 * prows;
+  float* zt = part_l + 2 * prows;
+  float* loss_c = zt + Ppad;
+  int* n_valid = meta.data_ptr<int>();
+  int* target = n_valid + 4;
+  int* slot = target + Ppad;
+  float* lse2 = stat.data_ptr<float>();
+  float* wex = lse2 + Ppad;
+  float* bias_ws = has_bias ? wex + Ppad : nullptr;
+  {
+    PrepParams q{};
+    q.h = h.data_ptr();
+    q.h_row = h.stride(0);
+    q.h_col = h.stride(1);
+    q.h_fp32 = h.scalar_type() == at::kFloat;
+    q.vec = !q.h_fp32 && D == Dp && q.h_col == 1 && q.h_row % 8 == 0 && reinterpret_cast<uintptr_t>(q.h) % 16 == 0;
+    q.targets = targets.data_ptr<int64_t>();
+    q.t_stride = targets.stride(0);
+    q.ignore = ignore_index;
+    q.P = int(P);
+    q.V = int(V);
+    q.D = int(D);
+    q.Dp = int(Dp);
+    q.hc = reinterpret_cast<__nv_bfloat16*>(hc.data_ptr());
+    q.n_valid = n_valid;
+    q.slot = slot;
+    q.target = target;
+    q.loss_rows = rows.data_ptr<float>();
+    q.bias_in = has_bias ? bias->data_ptr<float>() : nullptr;
+    q.bias_out = bias_ws;
+    q.row_blocks = int((P + kPrepRows - 1) / kPrepRows);
+    const int bias_blocks = has_bias ? int(std::min<int64_t>((Vpad + kPrepRows - 1) / kPrepRows, 2 * grid)) : 0;
+    full_softmax_prep_kernel<<<q.row_blocks + bias_blocks, kPrepRows, 0, stream>>>(q);
+    TRB_CUDA_CHECK(cudaGetLastError());
+  }
+  FsParams p{};
+  fs_shape(p, V, Dp, acc);
+  p.n_valid = n_valid;
+  p.grid = grid;
+  p.target = target;
+  p.bias = bias_ws;
+  p.part_acc = acc ? part_acc.data_ptr<float>() : nullptr;
+  p.part_m = part_m;
+  p.part_l = part_l;
+  p.zt = zt;
+  const CUtensorMap tx = make_tmap(hc.data_ptr(), Ppad, Dp, Dp, 64, kFsTile);
+  const CUtensorMap ty = make_tmap(weight.data_ptr(), V, Dp, weight.stride(0), 64, kFsTile);
+  if (acc) has_bias ? fs_launch<FS_FWD, true, false>(tx, ty, p) : fs_launch<FS_FWD, false, false>(tx, ty, p);
+  else has_bias ? fs_launch<FS_LSE, true, false>(tx, ty, p) : fs_launch<FS_LSE, false, false>(tx, ty, p);
+  {
+    const int smem = (kFsItemsPerSm * grid + 8) * 4 + kJoinThreads * 16;
+    const auto* w = reinterpret_cast<const __nv_bfloat16*>(weight.data_ptr());
+    auto join = acc ? full_softmax_join_kernel<true> : full_softmax_join_kernel<false>;
+    join<<<unsigned(Ppad), kJoinThreads, smem, stream>>>(n_valid, int(V), int(Dp), grid, pieces, p.part_acc, part_m, part_l, zt, target, w, weight.stride(0), lse2, wex, loss_c,
+                                                         acc ? unit.data_ptr<float>() : nullptr);
+    TRB_CUDA_CHECK(cudaGetLastError());
+  }
+  if (reduction == 0) {
+    full_softmax_rows_kernel<<<unsigned((P + 255) / 256), 256, 0, stream>>>(int(P), slot, loss_c, rows.data_ptr<float>());
+    TRB_CUDA_CHECK(cudaGetLastError());
+    return {rows, hc, meta, stat, unit};
+  }
+  at::Tensor loss = at::empty({}, f32);
+  full_softmax_reduce_kernel<<<1, 1024, 0, stream>>>(int(P), n_valid, slot, loss_c, rows.data_ptr<float>(), loss.data_ptr<float>(), reduction == 1);
+  TRB_CUDA_CHECK(cudaGetLastError());
+  return {loss, hc, meta, stat, unit};
+}
+
+// dloss: fp32, [P] for reduction 0, a scalar otherwise.  Outputs that are not wanted come back empty.  dh [P, D] in bf16 or fp32,
+// dW [V, Dp] in bf16 or fp32, db [V] in fp32.
+std::tuple<at::Tensor, at::Tensor, at::Tensor> full_softmax_bwd(const at::Tensor& dloss, const at::Tensor& weight, const at::Tensor& hc, const at::Tensor& meta, const at::Tensor& stat,
+                                                                const at::Tensor& unit, int64_t P, int64_t D, bool has_bias, int64_t reduction, bool want_h, bool want_w, bool want_b,
+                                                                bool dh_fp32, bool dw_fp32) {
+  fs_check_weight(weight);
+  const int64_t V = weight.size(0), Dp = weight.size(1), Ppad = (P + kFsTile - 1) / kFsTile * kFsTile, Vpad = (V + kFsTile - 1) / kFsTile * kFsTile;
+  const at::Device dev = weight.device();
+  TORCH_CHECK(dloss.device() == dev && dloss.scalar_type() == at::kFloat && (reduction == 0 ? dloss.dim() == 1 && dloss.size(0) == P : dloss.numel() == 1),
+              "full_softmax_bwd: the upstream gradient is fp32, [P] without a reduction and one value with it");
+  TORCH_CHECK(P >= 0 && P < kFsMaxRows && D >= 1 && D <= Dp && Dp - D < 8 && reduction >= 0 && reduction <= 2);
+  TORCH_CHECK(hc.device() == dev && hc.scalar_type() == at::kBFloat16 && hc.is_contiguous() && hc.dim() == 2 && hc.size(0) == Ppad && hc.size(1) == Dp);
+  TORCH_CHECK(meta.device() == dev && meta.scalar_type() == at::kInt && meta.is_contiguous() && meta.numel() == 4 + Ppad + P);
+  TORCH_CHECK(stat.device() == dev && stat.scalar_type() == at::kFloat && stat.is_contiguous() && stat.numel() == 2 * Ppad + (has_bias ? Vpad : 0));
+  TORCH_CHECK(!want_h || (unit.device() == dev && unit.scalar_type() == at::kFloat && unit.is_contiguous() && unit.numel() == Ppad * Dp));
+  TORCH_CHECK(!want_b || has_bias);
+  c10::cuda::CUDAGuard guard(dev);
+  auto stream = at::cuda::getCurrentCUDAStream();
+  const auto f32 = hc.options().dtype(at::kFloat);
+  at::Tensor dh = at::empty({want_h ? P : 0, D}, dh_fp32 ? f32 : hc.options());
+  const bool main = want_w || want_b;
+  at::Tensor dw = at::empty({main ? V : 0, Dp}, dw_fp32 ? f32 : hc.options());  // the kernel that sums db computes dW on the way
+  at::Tensor db = at::empty({want_b ? V : 0}, f32);
+  if (P == 0) {
+    dw.zero_();
+    db.zero_();
+    return {dh, dw, db};
+  }
+  const int grid = fs_grid(dev);
+  const int* n_valid = meta.data_ptr<int>();
+  const int* target = n_valid + 4;
+  const int* slot = target + Ppad;
+  const float* lse2 = stat.data_ptr<float>();
+  const bool per_row = reduction == 0, mean = reduction == 1;
+  at::Tensor gcol = per_row && main ? at::empty({Ppad}, f32) : at::Tensor();
+  if (want_h || gcol.defined()) {
+    const int64_t work = P * (Dp / 8);
+    const unsigned blocks = unsigned((work + 255) / 256);
+    const int64_t stride = per_row ? dloss.stride(0) : 0;
+    float* gc = gcol.defined() ? gcol.data_ptr<float>() : nullptr;
+    const float* u = want_h ? unit.data_ptr<float>() : nullptr;
+    if (dh_fp32)
+      full_softmax_dh_kernel<float><<<blocks, 256, 0, stream>>>(int(P), int(D), int(Dp), n_valid, slot, u, dloss.data_ptr<float>(), stride, per_row, mean,
+                                                                want_h ? dh.data_ptr<float>() : nullptr, gc);
+    else
+      full_softmax_dh_kernel<__nv_bfloat16><<<blocks, 256, 0, stream>>>(int(P), int(D), int(Dp), n_valid, slot, u, dloss.data_ptr<float>(), stride, per_row, mean,
+                                                                        want_h ? reinterpret_cast<__nv_bfloat16*>(dh.data_ptr()) : nullptr, gc);
+    TRB_CUDA_CHECK(cudaGetLastError());
+  }
+  if (!main) return {dh, dw, db};
+  const int pieces = int((Dp + kFsAcc - 1) / kFsAcc);
+  const int64_t prows = fs_partial_rows(V, P, grid);
+  const bool may_split = int64_t(kFsItemsPerSm) * grid / (Vpad / kFsTile) > 1 && Ppad > kFsTile;  // mirrors fs_schedule
+  at::Tensor part_acc = may_split ? at::empty({prows, Dp}, f32) : at::Tensor();
+  at::Tensor part_l = want_b || has_bias ? at::empty({2 * prows}, f32) : at::Tensor();
+  FsParams p{};
+  fs_shape(p, V, Dp, true);
+  p.n_valid = n_valid;
+  p.grid = grid;
+  p.target = target;
+  p.bias = has_bias ? lse2 + 2 * Ppad : nullptr;
+  p.part_acc = may_split ? part_acc.data_ptr<float>() : nullptr;
+  p.part_l = part_l.defined() ? part_l.data_ptr<float>() : nullptr;
+  p.lse2 = lse2;
+  p.wex = lse2 + Ppad;
+  p.gcol = gcol.defined() ? gcol.data_ptr<float>() : nullptr;
+  p.dloss = dloss.data_ptr<float>();
+  p.mean = mean;
+  p.dw = dw.data_ptr();
+  p.dw_fp32 = dw_fp32;
+  const CUtensorMap tx = make_tmap(weight.data_ptr(), V, Dp, weight.stride(0), 64, kFsTile);
+  const CUtensorMap ty = make_tmap(hc.data_ptr(), Ppad, Dp, Dp, 64, kFsTile);
+  if (has_bias) per_row ? fs_launch<FS_BWD, true, true>(tx, ty, p) : fs_launch<FS_BWD, true, false>(tx, ty, p);
+  else per_row ? fs_launch<FS_BWD, false, true>(tx, ty, p) : fs_launch<FS_BWD, false, false>(tx, ty, p);
+  if (may_split) {
+    const unsigned blocks = unsigned(std::min<int64_t>((V * Dp / 4 + 255) / 256, 16 * grid));
+    if (dw_fp32)
+      full_softmax_dw_kernel<float><<<blocks, 256, 0, stream>>>(n_valid, int(V), int(Dp), grid, pieces, p.part_acc, p.dloss, per_row, mean, dw.data_ptr<float>());
+    else
+      full_softmax_dw_kernel<__nv_bfloat16><<<blocks, 256, 0, stream>>>(n_valid, int(V), int(Dp), grid, pieces, p.part_acc, p.dloss, per_row, mean,
+                                                                        reinterpret_cast<__nv_bfloat16*>(dw.data_ptr()));
+    TRB_CUDA_CHECK(cudaGetLastError());
+  }
+  if (want_b) {
+    full_softmax_db_kernel<<<unsigned((V + 255) / 256), 256, 0, stream>>>(n_valid, int(V), grid, pieces, p.part_l, p.dloss, per_row, mean, db.data_ptr<float>());
+    TRB_CUDA_CHECK(cudaGetLastError());
+  }
+  return {dh, dw, db};
+}
+
+// non-zero after a launch gave up waiting (1..9) or met a target outside [0, V) (16); reading it synchronises and resets it
+int64_t full_softmax_status() {
+  int v = 0;
+  const int zero = 0;
+  TRB_CUDA_CHECK(cudaDeviceSynchronize());
+  TRB_CUDA_CHECK(cudaMemcpyFromSymbol(&v, g_fs_error, sizeof(int)));
+  if (v != 0) TRB_CUDA_CHECK(cudaMemcpyToSymbol(g_fs_error, &zero, sizeof(int)));
+  return v;
+}
+
+}  // namespace trb
+
+TORCH_LIBRARY_FRAGMENT(trb200, m) {
+  m.def("full_softmax_fwd(Tensor h, Tensor weight, Tensor targets, Tensor? bias, int ignore_index, int reduction, int grad) -> (Tensor, Tensor, Tensor, Tensor, Tensor)");
+  m.def("full_softmax_bwd(Tensor dloss, Tensor weight, Tensor hc, Tensor meta, Tensor stat, Tensor unit, int P, int D, bool has_bias, int reduction, bool want_h, bool want_w, "
+        "bool want_b, bool dh_fp32, bool dw_fp32) -> (Tensor, Tensor, Tensor)");
+  m.def("full_softmax_status() -> int");
+}
+
+TORCH_LIBRARY_IMPL(trb200, CUDA, m) {
+  m.impl("full_softmax_fwd", &trb::full_softmax_fwd);
+  m.impl("full_softmax_bwd", &trb::full_softmax_bwd);
+}
+
+TORCH_LIBRARY_IMPL(trb200, CompositeExplicitAutograd, m) { m.impl("full_softmax_status", &trb::full_softmax_status); }

@@ -6,7 +6,8 @@ elsewhere plain torch, which is also the oracle of the kernel tests).
 ``gelu_dropout(z, p)`` is ``dropout(gelu(z))``.  Dropout masks are recomputed from a per-call seed in the backward instead of being
 stored.  ``packed_attention(qkv, offsets, heads, max_len, p)`` is self-attention inside every sequence of packed tokens
 (``varlen_attention.cu``).  ``sampled_softmax_loss(h, positive, negatives)`` is the cross entropy of a sampled softmax with its
-gradient produced in the same pass over the scores (``sampled_softmax_kernels.cu``).
+gradient produced in the same pass over the scores (``sampled_softmax_kernels.cu``).  ``full_softmax_loss(h, weight, targets, bias)``
+is the cross entropy over all rows of ``weight``, with its gradient, without keeping the scores (``full_softmax_kernels.cu``).
 """
 from __future__ import annotations
 
@@ -208,3 +209,165 @@ def sampled_softmax_loss(h: torch.Tensor, positive: torch.Tensor, negatives: tor
         return _SampledSoftmaxLoss.apply(h, positive, negatives)
     scores = torch.cat([(h * positive.to(h.dtype)).sum(-1, keepdim=True), h @ negatives.to(h.dtype).t()], dim=1).float()
     return torch.nn.functional.cross_entropy(scores, torch.zeros(scores.shape[0], dtype=torch.long, device=scores.device))
+
+
+# --------------------------------------------------------------------------------------
+# softmax over the whole catalogue
+# --------------------------------------------------------------------------------------
+FULL_SOFTMAX_MAX_DIM = 1024  # widest row of the tensor-core kernel
+_REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
+
+
+def full_softmax_error(device: torch.device) -> int:
+    """Non-zero after a ``full_softmax_loss`` launch on ``device`` met a target outside ``[0, V)`` that is not ``ignore_index`` (16: the
+    loss of that row is NaN, its gradient zero) or gave up waiting for its own copies (1..9).  Reading it synchronises and resets it."""
+    device = torch.device(device)
+    if device.type != "cuda" or not _ext.has_cuda_ext():
+        return 0
+    with torch.cuda.device(device):
+        return int(torch.ops.trb200.full_softmax_status())
+
+
+def _weight_rows(weight: torch.Tensor) -> torch.Tensor:
+    """The weight as the kernel reads it: bf16 rows on 16-byte boundaries, zero columns up to a multiple of 8.  fp32 parameters go
+    through the cache that the dense layers use, so they are rounded once per optimizer step."""
+    from torchrec_b200.ops import dense_ops
+
+    if weight.dtype == torch.bfloat16:
+        w = weight.detach()
+    elif isinstance(weight, torch.nn.Parameter):
+        w = dense_ops.bf16_cache.get(weight)
+    else:
+        w = weight.detach().to(torch.bfloat16)
+    if w.shape[1] % 8:
+        return torch.nn.functional.pad(w, (0, -w.shape[1] % 8))
+    if w.stride(1) != 1 or w.stride(0) % 8 or w.stride(0) < w.shape[1] or w.data_ptr() % 16:
+        w = w.clone(memory_format=torch.contiguous_format)
+    return w
+
+
+class _FullSoftmaxLoss(torch.autograd.Function):
+    """The tensor-core path.  With a gradient of ``h`` wanted the forward already leaves it, up to the upstream factor, in fp32."""
+
+    @staticmethod
+    def forward(ctx, h, weight, bias, targets, ignore_index: int, reduction: int, grad: int):
+        w16 = _weight_rows(weight)
+        loss, hc, meta, stat, unit = torch.ops.trb200.full_softmax_fwd(h, w16, targets, bias, ignore_index, reduction, grad)
+        if grad:
+            # the caller's weight is saved too where the kernel read a copy, so that a change in place is noticed
+            ctx.save_for_backward(hc, meta, stat, unit, weight, *(() if w16.data_ptr() == weight.data_ptr() else (w16,)))
+            ctx.cfg = (tuple(h.shape), h.dtype, bias is not None, reduction)
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        hc, meta, stat, unit, weight, *copy = ctx.saved_tensors
+        (P, D), h_dtype, has_bias, reduction = ctx.cfg
+        w16 = copy[0] if copy else weight
+        want_h, want_w, want_b = ctx.needs_input_grad[:3]
+        dh, dw, db = torch.ops.trb200.full_softmax_bwd(g, w16, hc, meta, stat, unit, P, D, has_bias, reduction, want_h, want_w, want_b and has_bias,
+                                                       h_dtype == torch.float32, weight.dtype == torch.float32)
+        if want_w and dw.shape[1] != D:
+            dw = dw[:, :D].contiguous()
+        return dh if want_h else None, dw if want_w else None, db if want_b and has_bias else None, None, None, None, None
+
+
+class _FullSoftmaxPieces(torch.autograd.Function):
+    """The same loss in plain torch, a piece of the rows at a time (never the whole ``[P, V]`` scores), recomputed in the backward:
+    CPU tensors, types and widths the kernel does not take, and the oracle of the small tests."""
+
+    PIECE = 1 << 26  # scores held at a time
+
+    @staticmethod
+    def _scores(h, weight, bias, keep, lo, hi, acc):
+        x = torch.where(keep[lo:hi, None], h[lo:hi].to(acc), 0)
+        z = x @ weight.to(acc).t()
+        return x, z if bias is None else z + bias.to(acc)
+
+    @staticmethod
+    def forward(ctx, h, weight, bias, targets, ignore_index: int, reduction: int):
+        P, V = h.shape[0], weight.shape[0]
+        acc = torch.float64 if h.dtype == torch.float64 else torch.float32
+        keep = targets != ignore_index
+        bad = keep & ((targets < 0) | (targets >= V))
+        if not targets.is_cuda and bool(bad.any()):
+            raise IndexError(f"full_softmax_loss: target {int(targets[bad][0])} is out of bounds for {V} classes")
+        keep = keep & ~bad
+        t = torch.where(keep, targets, 0)
+        step = max(1, _FullSoftmaxPieces.PIECE // V)
+        lse, rows = h.new_zeros(P, dtype=acc), h.new_zeros(P, dtype=acc)
+        for lo in range(0, P, step):
+            hi = min(P, lo + step)
+            _, z = _FullSoftmaxPieces._scores(h, weight, bias, keep, lo, hi, acc)
+            lse[lo:hi] = torch.logsumexp(z, 1)
+            rows[lo:hi] = lse[lo:hi] - z.gather(1, t[lo:hi, None]).squeeze(1)
+        rows = torch.where(keep, rows, 0).masked_fill(bad, float("nan"))
+        count = keep.sum().clamp(min=1)
+        ctx.save_for_backward(h, weight, bias, t, keep, lse, count)
+        ctx.cfg = (reduction, acc)
+        return rows if reduction == 0 else rows.sum() if reduction == 2 else rows.sum() / count
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        h, weight, bias, t, keep, lse, count = ctx.saved_tensors
+        reduction, acc = ctx.cfg
+        P, V = h.shape[0], weight.shape[0]
+        scale = torch.where(keep, (g / count if reduction == 1 else g).to(acc), 0)
+        step = max(1, _FullSoftmaxPieces.PIECE // V)
+        w = weight.to(acc)
+        dh = torch.zeros_like(h)
+        dw = weight.new_zeros(weight.shape, dtype=acc)
+        db = None if bias is None else bias.new_zeros(bias.shape, dtype=acc)
+        for lo in range(0, P, step):
+            hi = min(P, lo + step)
+            x, z = _FullSoftmaxPieces._scores(h, weight, bias, keep, lo, hi, acc)
+            p = torch.exp(z - lse[lo:hi, None])
+            p.scatter_add_(1, t[lo:hi, None], p.new_full((hi - lo, 1), -1.0))
+            p = torch.where(keep[lo:hi, None], p * scale[lo:hi, None], 0)
+            dh[lo:hi] = (p @ w).to(h.dtype)
+            dw += p.t() @ x
+            if db is not None:
+                db += p.sum(0)
+        return dh, dw.to(weight.dtype), None if db is None else db.to(bias.dtype), None, None, None
+
+
+def full_softmax_loss(h: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, bias: Optional[torch.Tensor] = None, ignore_index: int = -100,
+                      reduction: str = "mean") -> torch.Tensor:
+    """Cross entropy of ``h [P, D]`` against all ``V`` rows of ``weight``: ``cross_entropy(h @ weight.T + bias, targets)`` in fp32, with
+    gradients of ``h``, ``weight`` and ``bias``, without ever holding the ``[P, V]`` scores.
+
+    ``targets [P]`` are class indices; a row whose target is ``ignore_index`` counts nowhere, whatever its ``h`` holds.  ``bias [V]`` may
+    hold ``-inf`` for classes that are out of the race.  ``reduction`` is ``"mean"`` (over the rows that are not ignored; 0 when there is
+    none), ``"sum"`` or ``"none"`` (``[P]``, 0 at ignored rows).
+
+    On CUDA bf16 ``h`` (and fp32 ``h`` while the dense compute type is bf16, ``dense_ops.set_dense_compute_dtype``) with ``D <= 1024`` runs
+    on the tensor cores with bf16 operands and fp32 sums; an fp32 ``weight`` is rounded to bf16 for the products and gets an fp32
+    gradient.  Everything else is computed in fp32 (fp64 for fp64 ``h``), a piece of the rows at a time.  A target outside ``[0, V)``
+    raises on the CPU; on CUDA it makes the row's loss NaN and its gradient zero, and ``full_softmax_error`` reports it."""
+    if h.dim() != 2 or weight.dim() != 2 or h.shape[1] != weight.shape[1] or weight.shape[0] == 0 or h.shape[1] == 0:
+        raise ValueError(f"full_softmax_loss: h [P, D] and weight [V, D] with V, D > 0, got {tuple(h.shape)} and {tuple(weight.shape)}")
+    if targets.shape != h.shape[:1] or targets.dtype not in (torch.int64, torch.int32):
+        raise ValueError(f"full_softmax_loss: targets is an int32 or int64 [P], got {targets.dtype} {tuple(targets.shape)}")
+    if bias is not None and bias.shape != weight.shape[:1]:
+        raise ValueError(f"full_softmax_loss: bias is [V], got {tuple(bias.shape)} for {weight.shape[0]} classes")
+    if reduction not in _REDUCTIONS:
+        raise ValueError(f"full_softmax_loss: reduction is one of {sorted(_REDUCTIONS)}, got {reduction!r}")
+    for name, t in (("h", h), ("weight", weight), ("bias", bias)):
+        if t is not None and not t.is_floating_point():
+            raise ValueError(f"full_softmax_loss: {name} is a floating-point tensor, got {t.dtype}")
+    for name, t in (("weight", weight), ("targets", targets), ("bias", bias)):
+        if t is not None and t.device != h.device:
+            raise ValueError(f"full_softmax_loss: {name} is on {t.device}, h on {h.device}")
+    from torchrec_b200.ops import dense_ops
+
+    targets = targets.to(torch.int64)
+    if _ext.use_cuda_kernel(h, "full_softmax_loss") and h.shape[1] <= FULL_SOFTMAX_MAX_DIM and weight.dtype in (torch.bfloat16, torch.float32) and (
+            h.dtype == torch.bfloat16 or (h.dtype == torch.float32 and dense_ops.fused_dense_enabled(h))):
+        bias = None if bias is None else bias.float().contiguous()
+        grad = 0
+        if torch.is_grad_enabled():
+            grad = 2 if h.requires_grad else int(weight.requires_grad or (bias is not None and bias.requires_grad))
+        return _FullSoftmaxLoss.apply(h, weight, bias, targets, int(ignore_index), _REDUCTIONS[reduction], grad)
+    return _FullSoftmaxPieces.apply(h, weight, bias, targets, int(ignore_index), _REDUCTIONS[reduction])

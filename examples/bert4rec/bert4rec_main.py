@@ -1,6 +1,7 @@
 """Masked-item training of BERT4Rec on synthetic sessions with a sharded item table.
 
     python examples/bert4rec/bert4rec_main.py --num_iterations 5
+    python examples/bert4rec/bert4rec_main.py --full_softmax --rotary
     torchrun --standalone --local-addr 127.0.0.1 --nproc-per-node 8 examples/bert4rec/bert4rec_main.py --sharding column_wise
 
 (cf. ``examples/bert4rec/bert4rec_main.py`` of the reference.)"""
@@ -53,6 +54,8 @@ def main() -> None:
     p.add_argument("--num_negatives", type=int, default=512)
     p.add_argument("--num_iterations", type=int, default=10)
     p.add_argument("--lr", type=float, default=1e-3)
+    p.add_argument("--full_softmax", action="store_true", help="cross entropy over the whole vocabulary instead of sampled negatives")
+    p.add_argument("--rotary", action="store_true", help="normalised, position-rotated queries and keys instead of learned position embeddings")
     p.add_argument("--sharding", default="row_wise", choices=["table_wise", "row_wise", "column_wise", "data_parallel"])
     a = p.parse_args()
     rank, world = int(os.environ.get("RANK", 0)), int(os.environ.get("WORLD_SIZE", 1))
@@ -67,7 +70,7 @@ def main() -> None:
         os.environ.setdefault("MASTER_PORT", "29551")
         dist.init_process_group(backend, rank=rank, world_size=world)
     torch.manual_seed(0)
-    model = BERT4Rec(a.vocab_size, a.max_len, a.emb_dim, a.nhead, a.num_layers).to(device)
+    model = BERT4Rec(a.vocab_size, a.max_len, a.emb_dim, a.nhead, a.num_layers, rotary=a.rotary).to(device)
     apply_optimizer_in_backward(torch.optim.Adam, model.history.ec.parameters(), {"lr": a.lr})
     gen_fn = {"table_wise": lambda: sp.table_wise(rank=0), "row_wise": sp.row_wise, "data_parallel": sp.data_parallel,
               "column_wise": lambda: sp.column_wise(ranks=list(range(min(world, max(a.emb_dim // 32, 1)))))}[a.sharding]
@@ -81,13 +84,16 @@ def main() -> None:
         kjt, pos, targets = synthetic_batch(a.batch_size, a.max_len, a.vocab_size, 0.15, gen, device)
         negatives = torch.randint(1, a.vocab_size - 1, (a.num_negatives,), generator=gen).to(device)
         opt.zero_grad()
-        logits = dmp.module.sampled_logits(kjt, pos, targets, negatives) if world == 1 else dmp(kjt).reshape(-1, a.vocab_size).index_select(0, pos)
-        labels = torch.zeros(logits.shape[0], dtype=torch.long, device=device) if world == 1 else targets
-        loss = torch.nn.functional.cross_entropy(logits.float(), labels)
+        if a.full_softmax:
+            loss = dmp(kjt, pos, targets)
+        else:
+            logits = dmp.module.sampled_logits(kjt, pos, targets, negatives) if world == 1 else dmp(kjt).reshape(-1, a.vocab_size).index_select(0, pos)
+            labels = torch.zeros(logits.shape[0], dtype=torch.long, device=device) if world == 1 else targets
+            loss = torch.nn.functional.cross_entropy(logits.float(), labels)
         loss.backward()
         opt.step()
         if rank == 0:
-            print(f"iter {it + 1}: masked-item loss {float(loss):.4f} ({logits.shape[0]} masked positions)", flush=True)
+            print(f"iter {it + 1}: masked-item loss {float(loss):.4f} ({pos.numel()} masked positions)", flush=True)
 
 
 if __name__ == "__main__":

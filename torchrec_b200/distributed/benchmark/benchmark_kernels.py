@@ -267,8 +267,8 @@ def bench_engine(B: int, n: int, warm: int) -> None:
 
 
 def bench_transformer(B: int, n: int, warm: int) -> None:
-    """Packed attention (forward, backward), the fused layer-norm / GELU kernels and the sampled-softmax cross entropy on BERT4Rec
-    shapes: ``B`` sequences with lengths uniform in [20, 200], 4 heads of 64, hidden 256, feed-forward 1024, 8192 negatives."""
+    """Packed attention (forward, backward), the fused layer-norm / GELU kernels, the sampled-softmax cross entropy, the query / key
+    norm with rotation and the softmax loss over a whole catalogue on BERT4Rec shapes: ``B`` sequences with lengths uniform in [20, 200], 4 heads of 64, hidden 256, feed-forward 1024, 8192 negatives."""
     from torchrec_b200.ops import transformer_ops as tops
 
     ops = torch.ops.trb200
@@ -306,7 +306,21 @@ def bench_transformer(B: int, n: int, warm: int) -> None:
     pos = torch.randn(P, device="cuda")
     t = timeit(lambda: ops.sampled_ce_fwd_bwd(pos, scores, 1.0 / P), n, warm)
     print(f"sampled-softmax cross entropy + gradient [{P}, {N}]: {t:.3f} ms, {2 * scores.numel() * 2 / t / 1e6:.0f} GB/s", flush=True)
-    assert tops.attention_error(qkv.device) == 0 and int(err.item()) == 0
+    pos, inv_freq, dout = torch.randint(0, 200, (T,), device="cuda"), tops.rotary_inv_freq(64, device="cuda"), torch.randn_like(qkv)
+    scale = torch.ones(64, device="cuda")
+    t = timeit(lambda: ops.qk_norm_rotary_fwd(qkv, pos[None], inv_freq, scale, scale, [32], H, H, 1e-6, True, False), n, warm)
+    print(f"query / key norm + rotation fwd [{T}, {3 * D}]: {t:.3f} ms, {2 * qkv.numel() * 2 / t / 1e6:.0f} GB/s", flush=True)
+    t = timeit(lambda: ops.qk_norm_rotary_bwd(dout, qkv, pos[None], inv_freq, scale, scale, [32], H, H, 1e-6, True, False, True), n, warm)
+    print(f"query / key norm + rotation bwd [{T}, {3 * D}]: {t:.3f} ms, {(2 + 2 / 3) * qkv.numel() * 2 / t / 1e6:.0f} GB/s", flush=True)
+    P, V = min(P, 16384), 131071
+    h, weight = torch.randn(P, D, device="cuda").bfloat16().requires_grad_(True), (torch.randn(V, D, device="cuda") / D**0.5).bfloat16().requires_grad_(True)
+    targets = torch.randint(0, V, (P,), device="cuda")
+    with torch.no_grad():
+        t = timeit(lambda: tops.full_softmax_loss(h, weight, targets), n, warm)
+    print(f"softmax loss over {V} classes [{P}, {D}], no gradient: {t:.3f} ms, {2.0 * P * V * D / t / 1e9:.0f} TFLOP/s (1 product)", flush=True)
+    t = timeit(lambda: torch.autograd.grad(tops.full_softmax_loss(h, weight, targets), (h, weight)), n, warm)
+    print(f"softmax loss over {V} classes [{P}, {D}], with gradients: {t:.3f} ms, {8.0 * P * V * D / t / 1e9:.0f} TFLOP/s (4 products)", flush=True)
+    assert tops.attention_error(qkv.device) == 0 and int(err.item()) == 0 and tops.full_softmax_error(qkv.device) == 0
 
 
 def main() -> None:

@@ -7,6 +7,7 @@ padding position is ever computed.
 * projections and feed-forward layers are the tcgen05 GEMMs with bias epilogues (``ops.dense_ops.linear_act``);
 * ``dropout + residual add + layer norm`` is one kernel, ``gelu + dropout`` another (``ops.transformer_ops``), with masks recomputed in
   the backward instead of stored;
+* optionally queries and keys are normalised per head and turned by their position in one pass (``QKNormRotary``);
 * attention runs on the packed tokens too: one CTA per (sequence, head) with the sequence's K and V in shared memory
   (``ops.transformer_ops.packed_attention``, head dimension 64, sequences up to 768 tokens).  Other shapes pad q, k, v for one
   library attention call with the padded keys masked (``ATTENTION_MODE = "padded"``; ``"nested"`` selects the library's
@@ -17,13 +18,43 @@ BERT4Rec runs padded ``[B, L, D]`` tensors through library modules (``examples/b
 """
 from __future__ import annotations
 
-from typing import Optional
+from typing import Optional, Sequence
 
 import torch
 from torch import nn
 
 from torchrec_b200.ops import dense_ops
-from torchrec_b200.ops.transformer_ops import gelu_dropout, packed_attention, packed_attention_supported, residual_layer_norm
+from torchrec_b200.ops.transformer_ops import gelu_dropout, packed_attention, packed_attention_supported, qk_norm_rotary, residual_layer_norm, rotary_inv_freq
+
+
+class QKNormRotary(nn.Module):
+    """Root-mean-square norm of every query and key head with learned scales, and their rotation by the token's position, on the packed
+    ``qkv`` of one attention layer (``ops.transformer_ops.qk_norm_rotary``).  ``sections`` deals the frequencies to several position axes."""
+
+    def __init__(self, head_dim: int, rotary_dim: Optional[int] = None, base: float = 10000.0, sections: Optional[Sequence[int]] = None, interleaved: bool = False,
+                 eps: float = 1e-6, device: Optional[torch.device] = None) -> None:
+        super().__init__()
+        self.rotary_dim, self.base, self.interleaved, self.eps = rotary_dim or head_dim // 2 * 2, base, interleaved, eps
+        self.sections = None if sections is None else [int(n) for n in sections]
+        self.q_weight = nn.Parameter(torch.ones(head_dim, device=device))
+        self.k_weight = nn.Parameter(torch.ones(head_dim, device=device))
+        self.register_buffer("inv_freq", rotary_inv_freq(self.rotary_dim, base, device), persistent=False)
+
+    def _apply(self, fn, recurse: bool = True):
+        super()._apply(fn, recurse)
+        # a cast of the module must not round the frequencies, and a move off the meta device has to fill them
+        self.inv_freq = rotary_inv_freq(self.rotary_dim, self.base, self.q_weight.device)
+        return self
+
+    def forward(self, qkv: torch.Tensor, positions: torch.Tensor, num_heads: int, num_kv_heads: Optional[int] = None) -> torch.Tensor:
+        return qk_norm_rotary(qkv, positions, self.inv_freq, num_heads, num_kv_heads, self.q_weight, self.k_weight, self.eps, self.sections, self.interleaved)
+
+
+def packed_token_positions(offsets: torch.Tensor, num_tokens: int) -> torch.Tensor:
+    """Place of every packed token in its own sequence, ``[num_tokens]`` (no host synchronisation)."""
+    offsets = offsets.to(torch.int64)
+    first = torch.repeat_interleave(offsets[:-1], offsets[1:] - offsets[:-1], output_size=num_tokens)
+    return torch.arange(num_tokens, device=offsets.device) - first
 
 
 def supports(encoder: nn.TransformerEncoder) -> bool:
@@ -92,9 +123,10 @@ def varlen_attention(qkv: torch.Tensor, offsets: torch.Tensor, num_heads: int, m
 
 
 def jagged_encoder_forward(encoder: nn.TransformerEncoder, x: torch.Tensor, offsets: torch.Tensor, max_len: int,
-                           training: Optional[bool] = None) -> torch.Tensor:
+                           training: Optional[bool] = None, rotary: Optional[Sequence[QKNormRotary]] = None, positions: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``x [T, D]`` packed tokens, ``offsets [B + 1]`` sequence bounds; returns the encoded tokens ``[T, D]`` in ``x``'s dtype
-    (bf16 inside when the fused dense path is on)."""
+    (bf16 inside when the fused dense path is on).  With ``rotary``, one module per layer, queries and keys are normalised per head and
+    turned by ``positions`` (``[T]`` or ``[axes, T]``; by default the place in the sequence) in front of the attention."""
     training = encoder.training if training is None else training
     fused = dense_ops.fused_dense_enabled(x)
     T = x.shape[0]
@@ -103,15 +135,24 @@ def jagged_encoder_forward(encoder: nn.TransformerEncoder, x: torch.Tensor, offs
     if pad:  # the weight-gradient GEMMs want a token count that is a multiple of 8: a short dummy sequence at the end
         s = torch.cat([s, s.new_zeros(pad, s.shape[1])])
         offsets = torch.cat([offsets, offsets.new_tensor([T + pad])])
+    if rotary is not None:
+        if len(rotary) != len(encoder.layers):
+            raise ValueError(f"{len(rotary)} rotary modules for {len(encoder.layers)} layers")
+        if positions is None:
+            positions = packed_token_positions(offsets, T + pad)
+        elif pad:
+            positions = torch.nn.functional.pad(positions, (0, pad))
     s = s.contiguous()
     pending: Optional[torch.Tensor] = None  # output of the previous sub-block, not yet added to the stream
     pending_p = 0.0
     with torch.autocast(device_type=x.device.type, enabled=False):
-        for layer in encoder.layers:
+        for i, layer in enumerate(encoder.layers):
             attn = layer.self_attn
             # (dropout + add of the previous feed-forward output) + norm1, in one pass
             s, y = residual_layer_norm(pending, s, layer.norm1.weight, layer.norm1.bias, pending_p, training, layer.norm1.eps)
             qkv = dense_ops.linear_act(y, attn.in_proj_weight, attn.in_proj_bias)
+            if rotary is not None:
+                qkv = rotary[i](qkv, positions, attn.num_heads)
             ctx = varlen_attention(qkv, offsets, attn.num_heads, max_len, attn.dropout if training else 0.0)
             o = dense_ops.linear_act(ctx, attn.out_proj.weight, attn.out_proj.bias)
             s, y = residual_layer_norm(o, s, layer.norm2.weight, layer.norm2.bias, layer.dropout1.p, training, layer.norm2.eps)

@@ -8,11 +8,13 @@ stored.  ``packed_attention(qkv, offsets, heads, max_len, p)`` is self-attention
 (``varlen_attention.cu``).  ``sampled_softmax_loss(h, positive, negatives)`` is the cross entropy of a sampled softmax with its
 gradient produced in the same pass over the scores (``sampled_softmax_kernels.cu``).  ``full_softmax_loss(h, weight, targets, bias)``
 is the cross entropy over all rows of ``weight``, with its gradient, without keeping the scores (``full_softmax_kernels.cu``).
+``qk_norm_rotary(qkv, positions, inv_freq, heads)`` normalises the queries and keys of every head and turns them by their token's
+position, in one pass over the packed tokens in front of the attention (``rotary_kernels.cu``).
 """
 from __future__ import annotations
 
 import itertools
-from typing import Optional, Tuple
+from typing import Optional, Sequence, Tuple
 
 import torch
 
@@ -156,6 +158,109 @@ def packed_attention(qkv: torch.Tensor, offsets: torch.Tensor, num_heads: int, m
     bf16); ``offsets [B + 1]`` bounds the sequences, none longer than ``max_len``.  Returns ``[T, D]``; dropout with probability ``p``
     acts on the attention probabilities.  The caller checks ``packed_attention_supported`` first."""
     return _PackedAttention.apply(qkv.contiguous(), offsets.to(torch.int64).contiguous(), int(num_heads), int(max_len), float(p))
+
+
+# --------------------------------------------------------------------------------------
+# norm and rotation of queries and keys
+# --------------------------------------------------------------------------------------
+def rotary_inv_freq(rotary_dim: int, base: float = 10000.0, device: Optional[torch.device] = None) -> torch.Tensor:
+    """The usual frequencies ``base ** (-2 j / rotary_dim)``, ``j < rotary_dim / 2``, in fp64."""
+    if rotary_dim < 2 or rotary_dim % 2 or not base > 0:
+        raise ValueError(f"rotary_inv_freq: a positive even dimension and a positive base, got {rotary_dim} and {base}")
+    return base ** (torch.arange(rotary_dim // 2, dtype=torch.float64, device=device) * (-2.0 / rotary_dim))
+
+
+def _rows16(t: torch.Tensor) -> torch.Tensor:
+    """``t [T, C]`` with contiguous rows that start on 16-byte boundaries (``t`` itself where it has them)."""
+    if t.stride(1) == 1 and t.data_ptr() % 16 == 0 and (t.stride(0) * t.element_size()) % 16 == 0 and (t.shape[0] <= 1 or t.stride(0) >= t.shape[1]):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+class _QKNormRotary(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, qkv, positions, inv_freq, q_weight, k_weight, cfg):
+        qkv = _rows16(qkv)
+        sections, heads, kv_heads, eps, norm, interleaved = cfg
+        ctx.save_for_backward(qkv, positions, inv_freq, q_weight, k_weight)
+        ctx.cfg = cfg
+        return torch.ops.trb200.qk_norm_rotary_fwd(qkv, positions, inv_freq, q_weight, k_weight, sections, heads, kv_heads, eps, norm, interleaved)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        qkv, positions, inv_freq, q_weight, k_weight = ctx.saved_tensors
+        sections, heads, kv_heads, eps, norm, interleaved = ctx.cfg
+        want_q, want_k = ctx.needs_input_grad[3], ctx.needs_input_grad[4]
+        dqkv, dw = torch.ops.trb200.qk_norm_rotary_bwd(_rows16(dy), qkv, positions, inv_freq, q_weight, k_weight, sections, heads, kv_heads, eps, norm, interleaved,
+                                                       want_q or want_k)
+        return dqkv if ctx.needs_input_grad[0] else None, None, None, dw[0] if want_q else None, dw[1] if want_k else None, None
+
+
+def _qk_norm_rotary_plain(qkv, positions, inv_freq, q_weight, k_weight, cfg):
+    """Oracle / fallback in plain torch: fp32 (fp64 for fp64 ``qkv``) with fp64 angles, one rounding at the end."""
+    sections, heads, kv_heads, eps, norm, interleaved = cfg
+    T, half = qkv.shape[0], inv_freq.shape[0]
+    dim = qkv.shape[1] // (heads + 2 * kv_heads)
+    x = qkv.to(torch.float64 if qkv.dtype == torch.float64 else torch.float32).reshape(T, heads + 2 * kv_heads, dim)
+    place = [a for a, n in enumerate(sections) for _ in range(n)]
+    angle = (positions.double()[place] * inv_freq.unsqueeze(1)).t().unsqueeze(1)  # [T, 1, R / 2]
+    cos, sin = angle.cos().to(x.dtype), angle.sin().to(x.dtype)
+    y = x[:, :heads + kv_heads]
+    if norm:
+        y = y * torch.rsqrt(y.square().mean(-1, keepdim=True) + eps)
+    parts = [p if w is None else p * w.to(p.dtype) for p, w in ((y[:, :heads], q_weight), (y[:, heads:], k_weight))]
+    y = torch.cat(parts, 1)
+    rot, rest = y[..., :2 * half], y[..., 2 * half:]
+    a, b = (rot[..., 0::2], rot[..., 1::2]) if interleaved else (rot[..., :half], rot[..., half:])
+    u, v = a * cos - b * sin, a * sin + b * cos
+    rot = torch.stack([u, v], -1).flatten(-2) if interleaved else torch.cat([u, v], -1)
+    return torch.cat([torch.cat([rot, rest], -1), x[:, heads + kv_heads:]], 1).reshape(qkv.shape).to(qkv.dtype)
+
+
+def qk_norm_rotary(qkv: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, num_heads: int, num_kv_heads: Optional[int] = None,
+                   q_weight: Optional[torch.Tensor] = None, k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6,
+                   sections: Optional[Sequence[int]] = None, interleaved: bool = False, norm: bool = True) -> torch.Tensor:
+    """Queries and keys of the packed ``qkv [T, (num_heads + 2 * num_kv_heads) * head_dim]`` (``q | k | v`` along the columns) with every head
+    divided by its root mean square (``norm``), scaled by ``q_weight`` / ``k_weight [head_dim]`` and turned by its token's position; ``v``
+    unchanged.  Returns a new tensor of the same shape and type, ready for :func:`packed_attention`.
+
+    The first ``2 * len(inv_freq)`` values of a head are turned, pair ``j`` by ``positions[t] * inv_freq[j]`` (:func:`rotary_inv_freq`; the
+    angle is formed in fp64): value ``j`` with value ``j + len(inv_freq)``, or neighbours ``2 j, 2 j + 1`` with ``interleaved``.  With several
+    axes ``positions`` is ``[axes, T]`` and ``sections`` says how many of the frequencies, in order, take their position from each axis.
+    Positions are int32 or int64, below ``2 ** 53`` in magnitude.
+
+    Gradients reach ``qkv`` and the weights.  CUDA tensors in bf16, fp16 or fp32 with a head dimension that is a multiple of 8 up to 256
+    run in one kernel; others in plain torch."""
+    kv_heads = num_heads if num_kv_heads is None else num_kv_heads
+    if num_heads < 1 or kv_heads < 1 or qkv.dim() != 2 or qkv.shape[1] == 0 or qkv.shape[1] % (num_heads + 2 * kv_heads):
+        raise ValueError(f"qk_norm_rotary: qkv is [T, (heads + 2 kv_heads) * head_dim], got {tuple(qkv.shape)} for {num_heads} and {kv_heads} heads")
+    T, dim = qkv.shape[0], qkv.shape[1] // (num_heads + 2 * kv_heads)
+    if not qkv.is_floating_point():
+        raise ValueError(f"qk_norm_rotary: qkv is a floating-point tensor, got {qkv.dtype}")
+    if inv_freq.dim() != 1 or not inv_freq.is_floating_point() or not 1 <= inv_freq.shape[0] <= dim // 2:
+        raise ValueError(f"qk_norm_rotary: inv_freq holds 1 to head_dim / 2 = {dim // 2} frequencies, got {inv_freq.dtype} {tuple(inv_freq.shape)}")
+    sections = [inv_freq.shape[0]] if sections is None else [int(n) for n in sections]
+    if positions.dtype not in (torch.int64, torch.int32) or tuple(positions.shape) not in ({(T,), (1, T)} if len(sections) == 1 else {(len(sections), T)}):
+        raise ValueError(f"qk_norm_rotary: positions is an int32 or int64 [T] or [axes, T], got {positions.dtype} {tuple(positions.shape)} for {T} tokens and "
+                         f"{len(sections)} axes")
+    if not 1 <= len(sections) <= 8 or min(sections) < 0 or sum(sections) != inv_freq.shape[0]:
+        raise ValueError(f"qk_norm_rotary: up to 8 sections that add up to the {inv_freq.shape[0]} frequencies, got {sections}")
+    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if w is not None and (w.shape != (dim,) or not w.is_floating_point()):
+            raise ValueError(f"qk_norm_rotary: {name} is [head_dim] = [{dim}], got {w.dtype} {tuple(w.shape)}")
+    for name, t in (("positions", positions), ("inv_freq", inv_freq), ("q_weight", q_weight), ("k_weight", k_weight)):
+        if t is not None and t.device != qkv.device:
+            raise ValueError(f"qk_norm_rotary: {name} is on {t.device}, qkv on {qkv.device}")
+    if eps < 0:
+        raise ValueError(f"qk_norm_rotary: eps is not negative, got {eps}")
+    positions = positions.reshape(len(sections), T)
+    inv_freq = inv_freq.detach().to(torch.float64).contiguous()
+    cfg = (sections, int(num_heads), int(kv_heads), float(eps), bool(norm), bool(interleaved))
+    if _ext.use_cuda_kernel(qkv, "qk_norm_rotary") and qkv.dtype in (torch.bfloat16, torch.float16, torch.float32) and dim % 8 == 0 and dim <= 256 and max(num_heads, kv_heads) <= 4096:
+        q_weight, k_weight = (w if w is None else w.float().contiguous() for w in (q_weight, k_weight))
+        return _QKNormRotary.apply(qkv, positions, inv_freq, q_weight, k_weight, cfg)
+    return _qk_norm_rotary_plain(qkv, positions, inv_freq, q_weight, k_weight, cfg)
 
 
 # --------------------------------------------------------------------------------------

@@ -125,6 +125,25 @@ def test_maximum_that_keeps_rising():
     _check(-h, w, t, b, reduction="sum")
 
 
+@pytest.mark.parametrize("D", [64, 256])
+def test_maximum_that_rises_by_hundreds(D):
+    """Maxima that grow by far more than what one reference can hold, tile after tile, in some rows only, and in one tile of many."""
+    g = torch.Generator().manual_seed(D)
+    V, P = 2600, 150
+    level = (torch.arange(V) // 128).float() * 30  # a tile's scores are 30 above those of the tile before
+    level[1000:1010] = 900
+    h = torch.zeros(P, D)
+    h[:, 0] = torch.linspace(0, 1, P)
+    h[:, 1:] = torch.randn(P, D - 1, generator=g) / 8
+    w = torch.randn(V, D, generator=g)
+    w[:, 0] = level
+    t = torch.randint(0, V, (P,), generator=g)
+    h, w, t = h.bfloat16().cuda(), w.bfloat16().cuda(), t.cuda()
+    _check(h, w, t, None, "none")
+    _check(h, w.flip(0), t, None, "sum")
+    _check(h, w, t, torch.randn(V, generator=g).cuda(), "mean")
+
+
 def test_confident_rows_keep_their_accuracy():
     """Rows whose target has almost all of the probability: 1 - p_t must not be the difference of two rounded numbers."""
     h, w, t, b = _inputs(300, 900, 128, False, seed=6)

@@ -16,8 +16,7 @@
 // Both products want the streamed tile, once K-major (S) and once MN-major (ACC); one copy in shared memory serves both up to
 // D = 256, where ACC takes the 256 TMEM columns that two S tiles leave.  Wider rows are cut into pieces of 256 columns that
 // recompute S (and load the tile twice).
-// The maximum is raised lazily: ACC and the sum are rescaled only when a row's maximum grew by more than 2^8 (the rounded terms stay
-// below 2^8, which bf16 holds with its usual relative error).
+// The maximum is raised lazily: ACC and the sums are rescaled only when a row's maximum grew by more than 2^40.
 // Ignored rows are left out at the start (their h is never multiplied, so NaN or infinity in padding does not spread) and cost nothing.
 // All sums run in a fixed order: pieces of the streamed axis go to a workspace and are joined by a second kernel.
 // Every wait is bounded (tcgen05.cuh); a block that gives up raises an error word and returns.
@@ -47,7 +46,9 @@ constexpr int kFsSmem = kFsSlots * kFsSlotBytes + kFsExtra;
 constexpr int kFsItemsPerSm = 4;                    // bounds the workspace of partial results
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
-constexpr float kRaise = 8.f;                       // base-2 growth of the maximum that forces a rescale
+// Base-2 growth of a row's maximum that forces a rescale.  The terms have bf16's and fp32's exponents: 2^40 over 2^31 columns is far
+// from overflow, and what is flushed lies 2^86 below the largest term.
+constexpr float kRaise = 40.f;
 
 enum FsMode : int { FS_LSE = 0, FS_FWD = 1, FS_BWD = 2 };
 enum FsErr : int { FS_ERR_EMPTY = 1, FS_ERR_FULL = 2, FS_ERR_X = 3, FS_ERR_S = 4, FS_ERR_P = 5, FS_ERR_ACC = 6, FS_ERR_COL = 7, FS_ERR_XCH = 8, FS_ERR_SMEM = 9, FS_ERR_TARGET = 16 };
@@ -141,22 +142,44 @@ __host__ __device__ constexpr uint32_t fs_idesc(int n, bool b_mn) {
 struct FsBars {
   uint64_t full[kFsMaxUnits], empty[kFsMaxUnits];
   uint64_t x_full, x_empty;
-  uint64_t s_full[2], p_full[2];
+  uint64_t s_full[4], p_full[4];
   uint64_t acc_done[2], o_empty;  // acc_done by the tile's parity: a waiter may be one tile behind the last commit
   uint64_t c_full[2], c_empty[2];
-  uint64_t xch[4], drain;
+  uint64_t m_done[4], drain;
   uint32_t tmem_base;
   int abort_flag;
 };
 static_assert(sizeof(FsBars) + 2048 <= kFsExtra, "the shared memory behind the slots is too small");
 
+// The part of a wait that loops is kept out of line: the roles' loops have to stay within the instruction caches.
+__device__ __noinline__ bool fs_wait_long(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int code) {
+  return mbar_wait(bar, parity, abort_flag, &g_fs_error, code);
+}
+__device__ __forceinline__ bool fs_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int code) {
+  return mbar_try_wait(bar, parity) || fs_wait_long(bar, parity, abort_flag, code);
+}
+
+// position in the ring of streamed blocks
+struct FsRing {
+  uint32_t units, stage = 0, phase = 0;
+  __device__ explicit FsRing(uint32_t n) : units(n) {}
+  __device__ void next() {
+    if (++stage == units) {
+      stage = 0;
+      phase ^= 1;
+    }
+  }
+};
+
 template <int MODE, bool BIAS, bool ROWG>
 __global__ void __launch_bounds__(kFsThreads, 1)
 full_softmax_kernel(const __grid_constant__ CUtensorMap tmapX, const __grid_constant__ CUtensorMap tmapY, const FsParams p) {
   constexpr bool kAcc = MODE != FS_LSE;
-  constexpr uint32_t kTmemCols = kAcc ? 512 : 256;
+  constexpr uint32_t kTmemCols = 512;
+  constexpr int kBufs = kAcc ? 2 : 4;       // score tiles in TMEM; the accumulator takes the other half
+  constexpr int kBufShift = kAcc ? 1 : 2;
   extern __shared__ __align__(1024) uint8_t fs_smem[];
-  float* cols = reinterpret_cast<float*>(fs_smem + kFsSlots * kFsSlotBytes);  // 512 floats: FWD maxima [2][8][32]; BWD lse2 [2][128], g [2][128]
+  float* cols = reinterpret_cast<float*>(fs_smem + kFsSlots * kFsSlotBytes);  // FWD: the rows' maxima [128]; BWD: lse2 [2][128], g [2][128]
   FsBars* B = reinterpret_cast<FsBars*>(cols + 512);
   volatile int* abort_flag = &B->abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -166,7 +189,7 @@ full_softmax_kernel(const __grid_constant__ CUtensorMap tmapX, const __grid_cons
   const int spu = p.kb == 1 ? 1 : 2;                       // slots of a unit of the ring
   const int upt = (p.kb + spu - 1) / spu;                  // units of a streamed tile
   const int x_slots = p.x_resident ? p.kb : 0;
-  const int units = min((kFsSlots - x_slots) / spu, kFsMaxUnits);
+  const uint32_t units = min((kFsSlots - x_slots) / spu, kFsMaxUnits);
   uint8_t* ring = fs_smem + x_slots * kFsSlotBytes;
 
   if (threadIdx.x == 0) {
@@ -176,15 +199,17 @@ full_softmax_kernel(const __grid_constant__ CUtensorMap tmapX, const __grid_cons
     }
     mbar_init(&B->x_full, 1);
     mbar_init(&B->x_empty, 1);
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < 4; ++i) {
       mbar_init(&B->s_full[i], 1);
-      mbar_init(&B->p_full[i], 8);
+      mbar_init(&B->p_full[i], 4);
+      mbar_init(&B->m_done[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
       mbar_init(&B->acc_done[i], 1);
       mbar_init(&B->c_full[i], 1);
-      mbar_init(&B->c_empty[i], 8);
+      mbar_init(&B->c_empty[i], 4);
     }
     mbar_init(&B->o_empty, 8);
-    for (int i = 0; i < 4; ++i) mbar_init(&B->xch[i], 2);
     mbar_init(&B->drain, 1);
     *abort_flag = 0;
     // the swizzled descriptors want slots on 1024-byte boundaries
@@ -211,21 +236,24 @@ full_softmax_kernel(const __grid_constant__ CUtensorMap tmapX, const __grid_cons
   if (warp == 0) {
     // ---------------- TMA producer ----------------
     if (lane == 0) {
-      uint32_t uc = 0, item = 0, tc = 0;
+      FsRing r(units);
+      uint32_t item = 0, tc = 0, loads = 0;
       auto load_unit = [&](const CUtensorMap* map, int u, int row) {
-        const uint32_t s = uc % units, ph = (uc / units) & 1;
-        if (!mbar_wait(&B->empty[s], ph ^ 1, abort_flag, &g_fs_error, FS_ERR_EMPTY)) return false;
+        if (!fs_wait(&B->empty[r.stage], r.phase ^ 1, abort_flag, FS_ERR_EMPTY)) return false;
         const int n = min(spu, p.kb - u * spu);
-        mbar_expect_tx(&B->full[s], n * kFsSlotBytes);
-        for (int k = 0; k < n; ++k) tma_load_2d(ring + (s * spu + k) * kFsSlotBytes, map, &B->full[s], (u * spu + k) * 64, row);
-        ++uc;
+        uint8_t* dst = ring + r.stage * spu * kFsSlotBytes;
+        mbar_expect_tx(&B->full[r.stage], n * kFsSlotBytes);
+        tma_load_2d(dst, map, &B->full[r.stage], u * spu * 64, row);
+        if (n > 1) tma_load_2d(dst + kFsSlotBytes, map, &B->full[r.stage], u * spu * 64 + 64, row);
+        r.next();
+        ++loads;
         return true;
       };
       for (int w = blockIdx.x; w < sc.items && ok; w += gridDim.x, ++item) {
         const int split = w / base, rem = w - split * base, x = rem % sc.tx, piece = rem / sc.tx;
         const int t0 = split * sc.per, nt = min(sc.ty, t0 + sc.per) - t0;
         if (p.x_resident && nt > 0) {
-          if (item > 0 && !mbar_wait(&B->x_empty, (item - 1) & 1, abort_flag, &g_fs_error, FS_ERR_X)) { ok = false; break; }
+          if (item > 0 && !fs_wait(&B->x_empty, (item - 1) & 1, abort_flag, FS_ERR_X)) { ok = false; break; }
           mbar_expect_tx(&B->x_full, p.kb * kFsSlotBytes);
           for (int k = 0; k < p.kb; ++k) tma_load_2d(fs_smem + k * kFsSlotBytes, &tmapX, &B->x_full, k * 64, x * kFsTile);
         }
@@ -234,7 +262,7 @@ full_softmax_kernel(const __grid_constant__ CUtensorMap tmapX, const __grid_cons
           if (t < nt) {
             if constexpr (MODE == FS_BWD) {
               const int b = tc & 1;
-              if (!mbar_wait(&B->c_empty[b], ((tc >> 1) & 1) ^ 1, abort_flag, &g_fs_error, FS_ERR_COL)) { ok = false; break; }
+              if (!fs_wait(&B->c_empty[b], ((tc >> 1) & 1) ^ 1, abort_flag, FS_ERR_COL)) { ok = false; break; }
               mbar_expect_tx(&B->c_full[b], ROWG ? 1024 : 512);
               fs_bulk_load(cols + b * 128, p.lse2 + int64_t(t0 + t) * kFsTile, 512, &B->c_full[b]);
               if constexpr (ROWG) fs_bulk_load(cols + 256 + b * 128, p.gcol + int64_t(t0 + t) * kFsTile, 512, &B->c_full[b]);
@@ -252,7 +280,7 @@ full_softmax_kernel(const __grid_constant__ CUtensorMap tmapX, const __grid_cons
       if (!ok) {
         // copies may still be on their way into shared memory: give them a bounded time to land before the block may exit
         const long long begin = clock64();
-        for (uint32_t j = uc > uint32_t(units) ? uc - units : 0; j < uc; ++j)
+        for (uint32_t j = loads > units ? loads - units : 0; j < loads; ++j)
           while (!mbar_try_wait(&B->full[j % units], (j / units) & 1) && clock64() - begin < kWaitCycles) {
           }
         if (p.x_resident && item < uint32_t(sc.items))
@@ -266,42 +294,54 @@ full_softmax_kernel(const __grid_constant__ CUtensorMap tmapX, const __grid_cons
     }
   } else if (warp == 1) {
     // ---------------- MMA issuer ----------------
-    // S(t + 1) is issued before ACC(t), so the tensor cores work while the softmax warps turn S(t) into E(t).
+    // S(t + 1) is issued before ACC(t), so the tensor cores work while the softmax warps turn S(t) into E(t).  Descriptors advance by
+    // additions (addresses in units of 16 bytes): one thread issues an instruction every 32 to 64 cycles.
     if (lane == 0) {
-      uint32_t uc = 0, item = 0, tc = 0;  // tc: tile whose S is issued next
+      FsRing r(units);
+      uint32_t item = 0, tc = 0;  // tc: tile whose S is issued next
       constexpr uint32_t idesc_s = fs_idesc(kFsTile, false);
+      constexpr uint32_t kSlot16 = kFsSlotBytes / 16;
+      const uint64_t desc_k = make_smem_desc(0, 16, 1024), desc_mn = make_smem_desc(0, kFsSlotBytes, 1024);
+      const uint32_t x16 = smem_u32(fs_smem) >> 4, ring16 = smem_u32(ring) >> 4, unit16 = spu * kSlot16;
       for (int w = blockIdx.x; w < sc.items && ok; w += gridDim.x, ++item) {
         const int split = w / base, rem = w - split * base, piece = rem / sc.tx;
         const int t0 = split * sc.per, nt = min(sc.ty, t0 + sc.per) - t0;
-        if (p.x_resident && nt > 0 && !mbar_wait(&B->x_full, item & 1, abort_flag, &g_fs_error, FS_ERR_X)) { ok = false; break; }
+        if (p.x_resident && nt > 0 && !fs_wait(&B->x_full, item & 1, abort_flag, FS_ERR_X)) { ok = false; break; }
         const int pu0 = piece * (kFsAcc / 128), pu1 = min(upt, pu0 + kFsAcc / 128);
-        uint32_t held[2] = {0, 0};  // first unit of a held tile
+        uint32_t held[2] = {0, 0};  // first stage of a held tile
         for (int t = 0; t <= nt && ok; ++t) {
           if (t < nt) {
-            const int b = tc & 1;
+            const uint32_t b = tc & (kBufs - 1), use = tc >> kBufShift;
             // the buffer's previous tile: with ACC its E was consumed by an MMA issued before this one; without, its readers must be done
-            if (!kAcc && tc >= 2 && !mbar_wait(&B->p_full[b], ((tc >> 1) - 1) & 1, abort_flag, &g_fs_error, FS_ERR_P)) { ok = false; break; }
+            if (!kAcc && use > 0 && !fs_wait(&B->p_full[b], (use - 1) & 1, abort_flag, FS_ERR_P)) { ok = false; break; }
             tcgen05_fence_after();
             const uint32_t d = tmem + b * kFsTile;
-            held[t & 1] = uc;
-            for (int u = 0; u < upt && ok; ++u) {
-              const uint32_t xs = uc % units;
+            held[t & 1] = r.stage;
+            for (int u = 0; u < upt; ++u) {
+              uint64_t dx = desc_k + x16 + u * unit16;
+              const uint32_t xs = r.stage;
               if (!p.x_resident) {
-                if (!mbar_wait(&B->full[xs], (uc / units) & 1, abort_flag, &g_fs_error, FS_ERR_FULL)) { ok = false; break; }
-                ++uc;
+                if (!fs_wait(&B->full[xs], r.phase, abort_flag, FS_ERR_FULL)) { ok = false; break; }
+                dx = desc_k + ring16 + xs * unit16;
+                r.next();
               }
-              const uint32_t ys = uc % units;
-              if (!mbar_wait(&B->full[ys], (uc / units) & 1, abort_flag, &g_fs_error, FS_ERR_FULL)) { ok = false; break; }
-              ++uc;
+              const uint32_t ys = r.stage;
+              if (!fs_wait(&B->full[ys], r.phase, abort_flag, FS_ERR_FULL)) { ok = false; break; }
+              r.next();
               tcgen05_fence_after();
-              const int n = min(spu, p.kb - u * spu);
-              for (int k = 0; k < n; ++k) {
-                const int col0 = (u * spu + k) * 64;
-                const uint32_t ax = smem_u32(p.x_resident ? fs_smem + (u * spu + k) * kFsSlotBytes : ring + (xs * spu + k) * kFsSlotBytes);
-                const uint32_t by = smem_u32(ring + (ys * spu + k) * kFsSlotBytes);
-                const int steps = min(4, (p.D - col0 + 15) / 16);
-                for (int i = 0; i < steps; ++i)
-                  umma_bf16(d, make_smem_desc(ax + i * 32, 16, 1024), make_smem_desc(by + i * 32, 16, 1024), idesc_s, (col0 > 0 || i > 0) ? 1u : 0u);
+              const uint64_t dy = desc_k + ring16 + ys * unit16;
+              const int steps = min(4 * spu, (p.D - u * spu * 64 + 15) / 16);  // 16 columns each
+              if (steps == 8) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                  const uint32_t off = (i >> 2) * kSlot16 + (i & 3) * 2;
+                  umma_bf16(d, dx + off, dy + off, idesc_s, (i > 0 || u > 0) ? 1u : 0u);
+                }
+              } else {
+                for (int i = 0; i < steps; ++i) {
+                  const uint32_t off = (i >> 2) * kSlot16 + (i & 3) * 2;
+                  umma_bf16(d, dx + off, dy + off, idesc_s, (i > 0 || u > 0) ? 1u : 0u);
+                }
               }
               if (!p.x_resident) tcgen05_commit(&B->empty[xs]);
               if (!p.hold) tcgen05_commit(&B->empty[ys]);
@@ -313,28 +353,27 @@ full_softmax_kernel(const __grid_constant__ CUtensorMap tmapX, const __grid_cons
           }
           if (kAcc && t > 0) {
             const uint32_t tt = (t < nt) ? tc - 2 : tc - 1;  // tile whose E is multiplied now
-            if (t == 1 && item > 0 && !mbar_wait(&B->o_empty, (item - 1) & 1, abort_flag, &g_fs_error, FS_ERR_ACC)) { ok = false; break; }
-            if (!mbar_wait(&B->p_full[tt & 1], (tt >> 1) & 1, abort_flag, &g_fs_error, FS_ERR_P)) { ok = false; break; }
+            if (t == 1 && item > 0 && !fs_wait(&B->o_empty, (item - 1) & 1, abort_flag, FS_ERR_ACC)) { ok = false; break; }
+            if (!fs_wait(&B->p_full[tt & 1], (tt >> 1) & 1, abort_flag, FS_ERR_P)) { ok = false; break; }
             tcgen05_fence_after();
             const uint32_t e = tmem + (tt & 1) * kFsTile;
-            for (int u = pu0; u < pu1 && ok; ++u) {
-              uint32_t s;
+            uint32_t hs = held[(t - 1) & 1];
+            for (int u = pu0; u < pu1; ++u) {
+              uint32_t ys = hs;
               if (p.hold) {
-                s = (held[(t - 1) & 1] + u) % units;
+                if (++hs == units) hs = 0;
               } else {
-                s = uc % units;
-                if (!mbar_wait(&B->full[s], (uc / units) & 1, abort_flag, &g_fs_error, FS_ERR_FULL)) { ok = false; break; }
-                ++uc;
+                ys = r.stage;
+                if (!fs_wait(&B->full[ys], r.phase, abort_flag, FS_ERR_FULL)) { ok = false; break; }
+                r.next();
                 tcgen05_fence_after();
               }
               const int n = min(64 * spu, (p.D - u * 64 * spu + 15) / 16 * 16);
-              const uint32_t idesc = fs_idesc(n, true);
-              const uint32_t by = smem_u32(ring + s * spu * kFsSlotBytes);
+              const uint32_t idesc = fs_idesc(n, true), d = tmem + 256 + (u - pu0) * 128;
+              const uint64_t dy = desc_mn + ring16 + ys * unit16;
 #pragma unroll
-              for (int i = 0; i < 8; ++i)
-                umma_bf16_ts(tmem + 256 + (u - pu0) * 128, e + (i < 4 ? i * 8 : 64 + (i - 4) * 8), make_smem_desc(by + i * 2048, kFsSlotBytes, 1024), idesc,
-                             (t > 1 || i > 0) ? 1u : 0u);
-              tcgen05_commit(&B->empty[s]);
+              for (int i = 0; i < 8; ++i) umma_bf16_ts(d, e + i * 8, dy + i * 128, idesc, (i > 0 || t > 1) ? 1u : 0u);
+              tcgen05_commit(&B->empty[ys]);
             }
             if (ok) tcgen05_commit(&B->acc_done[tt & 1]);
           }
@@ -349,12 +388,14 @@ full_softmax_kernel(const __grid_constant__ CUtensorMap tmapX, const __grid_cons
     }
   } else {
     // ---------------- softmax warps (2..9) ----------------
-    // Two warps share the 32 rows of a TMEM lane quarter (warp % 4) and take 64 columns each; a thread owns one row.
-    const int q = warp & 3, half = (warp - 2) >> 2, ew = warp - 2;
+    // Two groups of four warps take the tiles in turn (group = parity of the tile), so that one group's exponentials fill the other's
+    // waits; a thread owns a row of the tile (TMEM lane quarter = warp % 4) and walks its 128 columns in pieces of 32.  The loop over
+    // the pieces is not unrolled: with the tile unrolled the warps waited for instructions a third of the time.
+    const int q = warp & 3, half = (warp - 2) >> 2;
     const uint32_t lanes = uint32_t(q * 32) << 16;
     uint32_t item = 0, tc = 0;
     auto wait_all = [&](uint64_t* bar, uint32_t parity, int code) {
-      return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, &g_fs_error, code)) != 0;
+      return __all_sync(0xffffffffu, fs_wait(bar, parity, abort_flag, code)) != 0;
     };
     for (int w = blockIdx.x; w < sc.items && ok; w += gridDim.x, ++item) {
       const int split = w / base, rem = w - split * base, x = rem % sc.tx, piece = rem / sc.tx;
@@ -368,164 +409,219 @@ full_softmax_kernel(const __grid_constant__ CUtensorMap tmapX, const __grid_cons
       } else {
         tgt = p.target[row];
       }
-      float m2 = -INFINITY, l = 0.f;
-      for (int t = 0; t < nt && ok; ++t, ++tc) {
-        const int b = tc & 1;
-        const int col0 = (t0 + t) * kFsTile + half * 64;  // first of this warp's 64 columns
-        int tc0 = -1, tc1 = -1;
-        if constexpr (MODE == FS_BWD) {  // targets of the 64 rows of h, two per lane
-          tc0 = p.target[col0 + lane];
-          tc1 = p.target[col0 + 32 + lane];
-        }
-        if (!wait_all(&B->s_full[b], (tc >> 1) & 1, FS_ERR_S)) { ok = false; break; }
+      float m2 = -INFINITY, l = 0.f;  // m2: reference of the exponentials, a whole number, so that rescaling is exact
+      const uint32_t tc0 = tc, tc1 = tc + nt;
+      for (tc += (tc ^ half) & 1; tc < tc1 && ok; tc += 2) {
+        const int t = int(tc - tc0);
+        const uint32_t b = tc & (kBufs - 1), ph = (tc >> kBufShift) & 1;
+        const int col0 = (t0 + t) * kFsTile;
+        if (!wait_all(&B->s_full[b], ph, FS_ERR_S)) { ok = false; break; }
         tcgen05_fence_after();
-        const uint32_t ts = tmem + lanes + b * kFsTile + half * 64;
-        uint32_t r0[32], r1[32];
-        tmem_ld_32x32_issue(ts, r0);
-        tmem_ld_32x32_issue(ts + 32, r1);
-        tmem_ld_wait(r0);
-        tmem_ld_wait(r1);
-        if constexpr (!kAcc) {
-          tcgen05_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&B->p_full[b]);
-        }
-        float z[64];
-#pragma unroll
-        for (int j = 0; j < 32; ++j) {
-          z[j] = __uint_as_float(r0[j]);
-          z[32 + j] = __uint_as_float(r1[j]);
-        }
-        if constexpr (MODE != FS_BWD) {
-          if constexpr (BIAS) {
-            const float4* bp = reinterpret_cast<const float4*>(p.bias + col0);
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              const float4 v = __ldg(bp + j);
-              z[4 * j] += v.x;
-              z[4 * j + 1] += v.y;
-              z[4 * j + 2] += v.z;
-              z[4 * j + 3] += v.w;
-            }
-          } else if (col0 + 64 > p.V) {
-#pragma unroll
-            for (int j = 0; j < 64; ++j)
-              if (col0 + j >= p.V) z[j] = -INFINITY;
-          }
-          const int rel = tgt - col0;
-          const bool hit = rel >= 0 && rel < 64 && tgt >= 0;
-          if (__any_sync(0xffffffffu, hit)) {
-#pragma unroll
-            for (int j = 0; j < 64; ++j)
-              if (hit && j == rel) {
-                if (piece == 0) p.zt[row] = z[j] * kLog2e;
-                z[j] = -INFINITY;
-              }
-          }
-          float mx[4] = {z[0], z[1], z[2], z[3]};
-#pragma unroll
-          for (int j = 4; j < 64; ++j) mx[j & 3] = fmaxf(mx[j & 3], z[j]);
-          float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * kLog2e;
-          if constexpr (MODE == FS_FWD) {
-            // both halves of a row scale by the same maximum
-            cols[(b * 8 + ew) * 32 + lane] = mt;
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&B->xch[q]);
-            if (!wait_all(&B->xch[q], tc & 1, FS_ERR_XCH)) { ok = false; break; }
-            mt = fmaxf(mt, cols[(b * 8 + (ew ^ 4)) * 32 + lane]);
-            const bool raise = mt > m2 + kRaise || (t == 0);
-            if (__any_sync(0xffffffffu, raise)) {
-              const float mn = raise ? fmaxf(mt, m2) : m2;
-              const float f = (m2 == mn) ? 1.f : fs_ex2(m2 - mn);
-              l *= f;
-              m2 = mn;
-              if (t > 0) {
-                // rescale this warp's share of the accumulator: every ACC up to the previous tile has to be complete
-                if (!wait_all(&B->acc_done[(tc - 1) & 1], ((tc - 1) >> 1) & 1, FS_ERR_ACC)) { ok = false; break; }
-                tcgen05_fence_after();
-                const int groups = (min(kFsAcc, p.D - piece * kFsAcc) + 31) / 32;
-                for (int g = half; g < groups; g += 2) {
-                  const uint32_t to = tmem + lanes + 256 + g * 32;
-                  uint32_t a[32];
-                  tmem_ld_32x32_issue(to, a);
-                  tmem_ld_wait(a);
-#pragma unroll
-                  for (int j = 0; j < 32; ++j) a[j] = __float_as_uint(__uint_as_float(a[j]) * f);
-                  tmem_st_32x32(to, a);
-                }
-                tmem_st_wait();
-              }
-            }
-          } else {
-            const float mn = fmaxf(m2, mt);
-            if (mn > m2) l *= fs_ex2(m2 - mn);
-            m2 = mn;
-          }
-          const float ms = m2 == -INFINITY ? 0.f : m2;
-          float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int j = 0; j < 64; ++j) {
-            z[j] = fs_ex2(fmaf(z[j], kLog2e, -ms));
-            sum[j & 3] += z[j];
-          }
-          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-        } else {
-          if (!wait_all(&B->c_full[b], (tc >> 1) & 1, FS_ERR_COL)) { ok = false; break; }
-          const float4* lp = reinterpret_cast<const float4*>(cols + b * 128 + half * 64);
-#pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            const float4 v = lp[j];
-            z[4 * j] = fs_ex2(fmaf(z[4 * j], kLog2e, bias_row) - v.x);
-            z[4 * j + 1] = fs_ex2(fmaf(z[4 * j + 1], kLog2e, bias_row) - v.y);
-            z[4 * j + 2] = fs_ex2(fmaf(z[4 * j + 2], kLog2e, bias_row) - v.z);
-            z[4 * j + 3] = fs_ex2(fmaf(z[4 * j + 3], kLog2e, bias_row) - v.w);
-          }
-          // entries (item, row of h) with the row's target: p - 1 = -(1 - p_t)
+        const uint32_t ts = tmem + lanes + b * kFsTile;
+        uint32_t r[32];
+        tmem_ld_32x32_issue(ts, r);
+        if constexpr (MODE == FS_BWD) {
           const int v0 = x * kFsTile + q * 32;
-          uint32_t h0 = __ballot_sync(0xffffffffu, tc0 >= v0 && tc0 < v0 + 32), h1 = __ballot_sync(0xffffffffu, tc1 >= v0 && tc1 < v0 + 32);
-          if (h0 | h1) {
+          int tg = __ldg(p.target + col0 + lane);  // targets of 32 rows of h, one per lane
+          if (!wait_all(&B->c_full[b], ph, FS_ERR_COL)) { ok = false; break; }
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) {
+            float z[32];
+            tmem_ld_wait(r);
+            const float4* lp = reinterpret_cast<const float4*>(cols + b * 128 + c * 32);
 #pragma unroll
-            for (int j = 0; j < 64; ++j) {
-              if (((j < 32 ? h0 : h1) >> (j & 31)) & 1u) {
-                const int owner = __shfl_sync(0xffffffffu, j < 32 ? tc0 : tc1, j & 31) - v0;
-                if (lane == owner) z[j] = -__ldg(p.wex + col0 + j);
+            for (int j = 0; j < 8; ++j) {
+              const float4 v = lp[j];
+              const float s4[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                const float s = __uint_as_float(r[4 * j + k]);
+                z[4 * j + k] = BIAS ? fmaf(s, kLog2e, bias_row) - s4[k] : fmaf(s, kLog2e, -s4[k]);
               }
             }
-          }
-          if constexpr (ROWG) {
-            const float4* gp = reinterpret_cast<const float4*>(cols + 256 + b * 128 + half * 64);
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              const float4 v = gp[j];
-              z[4 * j] *= v.x;
-              z[4 * j + 1] *= v.y;
-              z[4 * j + 2] *= v.z;
-              z[4 * j + 3] *= v.w;
+            // entries (item, row of h) with the row's target: p - 1 = -(1 - p_t)
+            uint32_t hits = __ballot_sync(0xffffffffu, tg >= v0 && tg < v0 + 32);
+            const int tg_now = tg;
+            if (c < 3) {
+              tmem_ld_32x32_issue(ts + (c + 1) * 32, r);
+              tg = __ldg(p.target + col0 + (c + 1) * 32 + lane);
             }
-          }
-          if constexpr (BIAS) {
-            float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int j = 0; j < 64; ++j) sum[j & 3] += z[j];
-            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            for (int j = 0; j < 32; ++j) z[j] = fs_ex2(z[j]);
+            while (hits) {
+              const int j = __ffs(hits) - 1;
+              hits &= hits - 1;
+              if (__shfl_sync(0xffffffffu, tg_now, j) == v0 + lane) {
+                const float v = -__ldg(p.wex + col0 + c * 32 + j);
+#pragma unroll
+                for (int k = 0; k < 32; ++k) z[k] = k == j ? v : z[k];
+              }
+              __syncwarp();
+            }
+            if constexpr (ROWG) {
+              const float4* gp = reinterpret_cast<const float4*>(cols + 256 + b * 128 + c * 32);
+#pragma unroll
+              for (int j = 0; j < 8; ++j) {
+                const float4 v = gp[j];
+                z[4 * j] *= v.x;
+                z[4 * j + 1] *= v.y;
+                z[4 * j + 2] *= v.z;
+                z[4 * j + 3] *= v.w;
+              }
+            }
+            if constexpr (BIAS) {
+              float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+              for (int j = 0; j < 32; ++j) sum[j & 3] += z[j];
+              l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            }
+            // E of these columns over score columns that this thread has read already
+            uint32_t e[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) e[j] = fs_pack(z[2 * j], z[2 * j + 1]);
+            tmem_st_32x16(ts + c * 16, e);
           }
           __syncwarp();
           if (lane == 0) mbar_arrive(&B->c_empty[b]);
-        }
-        if constexpr (kAcc) {
-          // E in bf16 over the first half of the score columns that this warp read
-          uint32_t e[32];
+        } else {
+          const int rel = tgt - col0;  // the target's column in this tile
+          const bool any_hit = __any_sync(0xffffffffu, tgt >= 0 && rel >= 0 && rel < kFsTile);
+          // multiplies the terms of this tile that are stored already
+          auto rescale_terms = [&](int pieces, float f) {
+            tmem_st_wait();
+#pragma unroll 1
+            for (int k = 0; k < pieces; ++k) {
+              uint32_t a[16];
+              tmem_ld_32x16_issue(ts + k * 16, a);
+              tmem_ld_wait(a);
 #pragma unroll
-          for (int j = 0; j < 32; ++j) e[j] = fs_pack(z[2 * j], z[2 * j + 1]);
-          tmem_st_32x32(ts, e);
-          tmem_st_wait();
-          tcgen05_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&B->p_full[b]);
+              for (int j = 0; j < 16; ++j) a[j] = fs_pack(__uint_as_float(a[j] << 16) * f, __uint_as_float(a[j] & 0xffff0000u) * f);
+              tmem_st_32x16(ts + k * 16, a);
+              tmem_st_wait();
+            }
+          };
+          if constexpr (MODE == FS_FWD) {
+            if (t == 1) {  // this group's first tile: the row's reference comes from the tile before
+              if (!wait_all(&B->m_done[q], (tc - 1) & 1, FS_ERR_XCH)) { ok = false; break; }
+              m2 = cols[q * 32 + lane];
+            }
+          }
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) {
+            float z[32];
+            tmem_ld_wait(r);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) z[j] = __uint_as_float(r[j]);
+            if constexpr (BIAS) {
+              const float4* bp = reinterpret_cast<const float4*>(p.bias + col0 + c * 32);
+#pragma unroll
+              for (int j = 0; j < 8; ++j) {
+                const float4 v = __ldg(bp + j);
+                z[4 * j] += v.x;
+                z[4 * j + 1] += v.y;
+                z[4 * j + 2] += v.z;
+                z[4 * j + 3] += v.w;
+              }
+            } else if (__builtin_expect(col0 + kFsTile > p.V, 0)) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j)
+                if (col0 + c * 32 + j >= p.V) z[j] = -INFINITY;
+            }
+            if (__builtin_expect(any_hit, 0)) {  // the target's own term stays out
+              float zt = 0.f;
+              const int at = rel - c * 32;
+#pragma unroll
+              for (int j = 0; j < 32; ++j) {
+                zt = j == at ? z[j] : zt;
+                z[j] = j == at ? -INFINITY : z[j];
+              }
+              if (piece == 0 && tgt >= 0 && at >= 0 && at < 32) p.zt[row] = zt * kLog2e;
+              __syncwarp();
+            }
+            float mx[4] = {z[0], z[1], z[2], z[3]};
+#pragma unroll
+            for (int j = 4; j < 32; ++j) mx[j & 3] = fmaxf(mx[j & 3], z[j]);
+            const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * kLog2e;
+            if (__builtin_expect(__any_sync(0xffffffffu, top > m2 + kRaise), 0)) {
+              const float mn = top > m2 + kRaise ? ceilf(top) : m2;
+              const float f = mn == m2 ? 1.f : fs_ex2(m2 - mn);
+              m2 = mn;
+              l *= f;
+              if constexpr (kAcc) rescale_terms(c, f);
+            }
+            const float ms = m2 == -INFINITY ? 0.f : m2;
+#pragma unroll
+            for (int j = 0; j < 32; ++j) z[j] = fmaf(z[j], kLog2e, -ms);
+            if (c < 3) tmem_ld_32x32_issue(ts + (c + 1) * 32, r);
+            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+              z[j] = fs_ex2(z[j]);
+              sum[j & 3] += z[j];
+            }
+            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            if constexpr (kAcc) {
+              // the terms in bf16 over score columns that this thread has read already
+              uint32_t e[16];
+#pragma unroll
+              for (int j = 0; j < 16; ++j) e[j] = fs_pack(z[2 * j], z[2 * j + 1]);
+              tmem_st_32x16(ts + c * 16, e);
+            }
+          }
+          if constexpr (MODE == FS_FWD) {
+            // The accumulator and both groups' sums refer to one maximum per row, kept in shared memory: a tile is published after the
+            // tile before it, by when that one's decision is known.
+            if (t == 0) {
+              cols[q * 32 + lane] = m2;
+            } else {
+              if (t > 1 && !wait_all(&B->m_done[q], (tc - 1) & 1, FS_ERR_XCH)) { ok = false; break; }
+              const float mr = cols[q * 32 + lane];
+              if (__builtin_expect(__any_sync(0xffffffffu, mr != m2), 0)) {
+                const float mn = fmaxf(mr, m2);
+                const float fe = mn == m2 ? 1.f : fs_ex2(m2 - mn);
+                l *= fe;
+                rescale_terms(4, fe);
+                if (__any_sync(0xffffffffu, mn != mr)) {
+                  // every ACC up to the previous tile has to be complete; this tile's has not been issued
+                  if (!wait_all(&B->acc_done[(tc - 1) & 1], ((tc - 1) >> 1) & 1, FS_ERR_ACC)) { ok = false; break; }
+                  tcgen05_fence_after();
+                  const float f = mr == mn ? 1.f : fs_ex2(mr - mn);
+                  const int groups = (min(kFsAcc, p.D - piece * kFsAcc) + 15) / 16;
+#pragma unroll 1
+                  for (int g = 0; g < groups; ++g) {
+                    const uint32_t to = tmem + lanes + 256 + g * 16;
+                    uint32_t a[16];
+                    tmem_ld_32x16_issue(to, a);
+                    tmem_ld_wait(a);
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) a[j] = __float_as_uint(__uint_as_float(a[j]) * f);
+                    tmem_st_32x16(to, a);
+                  }
+                  cols[q * 32 + lane] = mn;
+                }
+                m2 = mn;
+              }
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&B->m_done[q]);
+          }
         }
+        if constexpr (kAcc) tmem_st_wait();
+        tcgen05_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&B->p_full[b]);
       }
       if (!ok) break;
+      tc = tc1;
       // ---- end of the item ----
+      if constexpr (MODE == FS_FWD) {
+        if (nt > 0 && ((tc - 1) & 1) != uint32_t(half)) {  // the other group had the last tile
+          if (!wait_all(&B->m_done[q], (tc - 1) & 1, FS_ERR_XCH)) { ok = false; break; }
+          const float mr = cols[q * 32 + lane];
+          if (m2 != mr) l *= fs_ex2(m2 - mr);
+          m2 = mr;
+        }
+      }
       if (piece == 0 && (MODE != FS_BWD || BIAS)) {
         const int64_t at = (int64_t(split) * 2 + half) * prow + row;
         p.part_l[at] = l;
@@ -533,6 +629,9 @@ full_softmax_kernel(const __grid_constant__ CUtensorMap tmapX, const __grid_cons
       }
       if constexpr (kAcc) {
         if (nt > 0) {
+          // the tile before the last first: a parity wait may lag behind by one use of its barrier, and the group that did not have the
+          // last tile knows no more than that the scores of the tile before it are done
+          if (nt > 1 && !wait_all(&B->acc_done[tc & 1], ((tc - 2) >> 1) & 1, FS_ERR_ACC)) { ok = false; break; }
           if (!wait_all(&B->acc_done[(tc - 1) & 1], ((tc - 1) >> 1) & 1, FS_ERR_ACC)) { ok = false; break; }
           tcgen05_fence_after();
         }

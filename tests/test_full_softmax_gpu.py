@@ -293,3 +293,57 @@ def test_other_streams_and_captured_graphs():
         for _, out in graphs:
             assert all(torch.equal(x, y) for x, y in zip(out, expect))
     assert full_softmax_error(a[0].device) == 0
+
+
+def test_refusals_and_modes():
+    from torchrec_b200.ops.transformer_ops import full_softmax_loss
+
+    h, w, t, b = _inputs(20, 30, 16, True, seed=16)
+    with pytest.raises(ValueError, match="reduction"):
+        full_softmax_loss(h, w, t, reduction="max")
+    for bad in ((h, w[:, :8]), (h, w[:0])):
+        with pytest.raises(ValueError, match="h \\[P, D\\]"):
+            full_softmax_loss(*bad, t)
+    for bad in (t[:3], t.float(), t[:, None]):
+        with pytest.raises(ValueError, match="targets"):
+            full_softmax_loss(h, w, bad)
+    with pytest.raises(ValueError, match="bias"):
+        full_softmax_loss(h, w, t, b[:29])
+    for bad in ((h, w.cpu(), t), (h, w, t.cpu()), (h, w, t, b.cpu())):
+        with pytest.raises(ValueError, match=" is on "):
+            full_softmax_loss(*bad)
+    leaves = [x.clone().requires_grad_(True) for x in (h, w, b)]
+    loss = full_softmax_loss(leaves[0], leaves[1], t, leaves[2])
+    up = torch.ones((), device="cuda", requires_grad=True)
+    grads = torch.autograd.grad(loss, leaves, up, create_graph=True)
+    with pytest.raises(RuntimeError, match="differentiated again"):
+        grads[0].float().sum().backward()
+    loss = full_softmax_loss(leaves[0], leaves[1], t, leaves[2])
+    with torch.no_grad():
+        leaves[1].mul_(2)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    with torch.inference_mode():
+        assert not full_softmax_loss(h, w, t, b).requires_grad
+    # tensors of more than the kernel's width take the piecewise path
+    wide = [x.requires_grad_(True) for x in (torch.randn(5, 1040, device="cuda").bfloat16(), (torch.randn(9, 1040, device="cuda") / 30).bfloat16())]
+    target = torch.arange(5, device="cuda")
+    want = torch.nn.functional.cross_entropy(wide[0].double() @ wide[1].double().t(), target)
+    got = full_softmax_loss(*wide, target)
+    assert abs(float(got.detach()) - float(want.detach())) < 1e-5
+    for x, y in zip(torch.autograd.grad(got, wide), torch.autograd.grad(want, wide)):
+        torch.testing.assert_close(x.double(), y.double(), rtol=2.0**-7, atol=1e-6)  # a bf16 rounding on either side
+
+
+def test_bias_types_and_gradients_that_come_expanded():
+    from torchrec_b200.ops.transformer_ops import full_softmax_loss
+
+    h, w, t, b = _inputs(200, 300, 64, True, 0.2, seed=17)
+    b16 = b.bfloat16()
+    leaves = [x.clone().requires_grad_(True) for x in (h, w, b16)]
+    rows = full_softmax_loss(leaves[0], leaves[1], t, leaves[2], reduction="none")
+    rows.sum().backward()  # the upstream gradient is one value, expanded
+    want, tol = _oracle(h, w, t, b16.float(), torch.ones(200, device="cuda"), "none")
+    for name, leaf, x, lim in zip(("dh", "dw", "db"), leaves, want[1:], tol[1:]):
+        assert leaf.grad.dtype == torch.bfloat16
+        _within(name, leaf.grad, x, lim + (2.0**-8 * x.abs() if name == "db" else 0))

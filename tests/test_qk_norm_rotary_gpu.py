@@ -183,3 +183,41 @@ def test_runs_twice_alike_on_other_streams_and_in_graphs():
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, expect))
+
+
+def test_refusals_and_modes():
+    from torchrec_b200.ops.transformer_ops import qk_norm_rotary, rotary_inv_freq
+
+    qkv, pos, inv = torch.randn(5, 3 * 8, device="cuda"), torch.arange(5, device="cuda"), rotary_inv_freq(8, device="cuda")
+    for bad in (dict(num_heads=0), dict(num_heads=1, num_kv_heads=2), dict(num_heads=2)):  # the last: heads of 4
+        with pytest.raises(ValueError, match="qkv is|inv_freq"):
+            qk_norm_rotary(qkv, pos, inv, **bad)
+    for bad in (rotary_inv_freq(10, device="cuda"), inv[:0], inv[None], inv.int()):
+        with pytest.raises(ValueError, match="inv_freq"):
+            qk_norm_rotary(qkv, pos, bad, 1, sections=[4] if bad.dim() != 1 else None)
+    for bad in (pos[:4], pos.float(), torch.stack([pos, pos])):
+        with pytest.raises(ValueError, match="positions"):
+            qk_norm_rotary(qkv, bad, inv, 1)
+    for bad in ([3, 2], [5, -1], [1] * 9):
+        with pytest.raises(ValueError, match="sections|axes"):
+            qk_norm_rotary(qkv, torch.stack([pos] * len(bad)), inv, 1, sections=bad)
+    with pytest.raises(ValueError, match="k_weight"):
+        qk_norm_rotary(qkv, pos, inv, 1, k_weight=torch.ones(7, device="cuda"))
+    with pytest.raises(ValueError, match="eps"):
+        qk_norm_rotary(qkv, pos, inv, 1, eps=-1.0)
+    for bad in (dict(positions=pos.cpu()), dict(inv_freq=inv.cpu()), dict(q_weight=torch.ones(8))):
+        with pytest.raises(ValueError, match=" is on "):
+            qk_norm_rotary(**{**dict(qkv=qkv, positions=pos, inv_freq=inv, num_heads=1), **bad})
+    x = qkv.clone().requires_grad_(True)
+    up = torch.ones(5, 24, device="cuda", requires_grad=True)
+    (g,) = torch.autograd.grad(qk_norm_rotary(x, pos, inv, 1), x, up, create_graph=True)
+    with pytest.raises(RuntimeError, match="differentiated again"):
+        g.sum().backward()
+    with torch.inference_mode():
+        assert not qk_norm_rotary(qkv, pos, inv, 1).requires_grad
+    # one weight only, in another type; a head dimension that the kernel does not take
+    kw = torch.rand(8, device="cuda").bfloat16().requires_grad_(True)
+    qk_norm_rotary(x, pos, inv, 1, k_weight=kw).square().sum().backward()
+    assert kw.grad.dtype == torch.bfloat16 and bool((kw.grad != 0).any())
+    odd = torch.randn(5, 3 * 6, device="cuda")
+    torch.testing.assert_close(qk_norm_rotary(odd, pos, inv[:3], 1).cpu(), qk_norm_rotary(odd.cpu(), pos.cpu(), inv[:3].cpu(), 1), rtol=1e-5, atol=1e-5)

@@ -1,6 +1,6 @@
 """In-tree build of the native libraries.
 
-``build_all()`` compiles every ``.cu`` under ``csrc/cuda`` for sm_100a into
+``build_all()`` compiles every ``.cu`` (and host-only ``.cpp``) under ``csrc/cuda`` for sm_100a into
 ``torchrec_b200/_C_cuda.so`` and every ``.cpp`` under ``csrc/cpu`` into
 ``torchrec_b200/_C_cpu.so``.  Objects are cached under ``csrc/_obj`` keyed by a hash of the
 source, the headers next to it and the flags, so an unchanged file is never recompiled.
@@ -102,6 +102,10 @@ def build_cuda(verbose: bool = False, force: bool = False, ptxas_verbose: bool =
         return [nvcc] + flags + ["-c", src, "-o", obj]
 
     objs = _compile_objects(srcs, hdrs, cmd, " ".join(flags), verbose or ptxas_verbose, force)
+    # host-only sources next to the kernels (autograd nodes)
+    host_flags = ["-O2", "-std=c++17", "-fPIC", "-D_GLIBCXX_USE_CXX11_ABI=1", "-Wno-unused-result"] + [f"-I{p}" for p in inc]
+    objs += _compile_objects(sorted(glob.glob(os.path.join(HERE, "cuda", "*.cpp"))), hdrs, lambda src, obj: ["g++"] + host_flags + ["-c", src, "-o", obj],
+                             " ".join(host_flags), verbose, force)
     out = os.path.join(PKG, "_C_cuda.so")
     link_tag = _hash(objs, "link-cuda")
     stamp = os.path.join(OBJ, "cuda.link")

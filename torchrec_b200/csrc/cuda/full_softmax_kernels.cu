@@ -31,6 +31,7 @@
 
 #include "common.cuh"
 #include "tcgen05.cuh"
+#include "transformer_ops.h"
 
 namespace trb {
 
@@ -182,8 +183,9 @@ full_softmax_kernel(const __grid_constant__ CUtensorMap tmapX, const __grid_cons
   float* cols = reinterpret_cast<float*>(fs_smem + kFsSlots * kFsSlotBytes);  // FWD: the rows' maxima [128]; BWD: lse2 [2][128], g [2][128]
   FsBars* B = reinterpret_cast<FsBars*>(cols + 512);
   volatile int* abort_flag = &B->abort_flag;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int n_valid = *p.n_valid;
+  // values that are alike in a warp are taken from lane 0, which tells the compiler so
+  const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+  const int n_valid = __shfl_sync(0xffffffffu, *p.n_valid, 0);
   const int nx = MODE == FS_BWD ? p.V : n_valid, ny = MODE == FS_BWD ? n_valid : p.V;
   const FsSchedule sc = fs_schedule(nx, ny, kAcc ? (p.D + kFsAcc - 1) / kFsAcc : 1, p.grid);
   const int spu = p.kb == 1 ? 1 : 2;                       // slots of a unit of the ring
@@ -226,7 +228,7 @@ full_softmax_kernel(const __grid_constant__ CUtensorMap tmapX, const __grid_cons
   tcgen05_fence_before();
   __syncthreads();
   tcgen05_fence_after();
-  const uint32_t tmem = B->tmem_base;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, B->tmem_base, 0);
   bool ok = *abort_flag == 0;
 
   // item -> (tile of X, piece of the accumulator's columns, split of the streamed axis).  The split is the slow index: blocks that run
@@ -295,8 +297,11 @@ full_softmax_kernel(const __grid_constant__ CUtensorMap tmapX, const __grid_cons
   } else if (warp == 1) {
     // ---------------- MMA issuer ----------------
     // S(t + 1) is issued before ACC(t), so the tensor cores work while the softmax warps turn S(t) into E(t).  Descriptors advance by
-    // additions (addresses in units of 16 bytes): one thread issues an instruction every 32 to 64 cycles.
-    if (lane == 0) {
+    // additions (addresses in units of 16 bytes).  The whole warp runs the loop, one elected lane issues.
+    {
+      auto wait_all = [&](uint64_t* bar, uint32_t parity, int code) {
+        return __all_sync(0xffffffffu, fs_wait(bar, parity, abort_flag, code)) != 0;
+      };
       FsRing r(units);
       uint32_t item = 0, tc = 0;  // tc: tile whose S is issued next
       constexpr uint32_t idesc_s = fs_idesc(kFsTile, false);
@@ -306,81 +311,81 @@ full_softmax_kernel(const __grid_constant__ CUtensorMap tmapX, const __grid_cons
       for (int w = blockIdx.x; w < sc.items && ok; w += gridDim.x, ++item) {
         const int split = w / base, rem = w - split * base, piece = rem / sc.tx;
         const int t0 = split * sc.per, nt = min(sc.ty, t0 + sc.per) - t0;
-        if (p.x_resident && nt > 0 && !fs_wait(&B->x_full, item & 1, abort_flag, FS_ERR_X)) { ok = false; break; }
+        if (p.x_resident && nt > 0 && !wait_all(&B->x_full, item & 1, FS_ERR_X)) { ok = false; break; }
         const int pu0 = piece * (kFsAcc / 128), pu1 = min(upt, pu0 + kFsAcc / 128);
-        uint32_t held[2] = {0, 0};  // first stage of a held tile
+        uint32_t held = 0, held_before = 0;  // first stages of the held tiles
         for (int t = 0; t <= nt && ok; ++t) {
           if (t < nt) {
             const uint32_t b = tc & (kBufs - 1), use = tc >> kBufShift;
             // the buffer's previous tile: with ACC its E was consumed by an MMA issued before this one; without, its readers must be done
-            if (!kAcc && use > 0 && !fs_wait(&B->p_full[b], (use - 1) & 1, abort_flag, FS_ERR_P)) { ok = false; break; }
-            tcgen05_fence_after();
+            if (!kAcc && use > 0 && !wait_all(&B->p_full[b], (use - 1) & 1, FS_ERR_P)) { ok = false; break; }
+            if constexpr (!kAcc) tcgen05_fence_after();
             const uint32_t d = tmem + b * kFsTile;
-            held[t & 1] = r.stage;
+            held_before = held;
+            held = r.stage;
             for (int u = 0; u < upt; ++u) {
               uint64_t dx = desc_k + x16 + u * unit16;
               const uint32_t xs = r.stage;
               if (!p.x_resident) {
-                if (!fs_wait(&B->full[xs], r.phase, abort_flag, FS_ERR_FULL)) { ok = false; break; }
+                if (!wait_all(&B->full[xs], r.phase, FS_ERR_FULL)) { ok = false; break; }
                 dx = desc_k + ring16 + xs * unit16;
                 r.next();
               }
               const uint32_t ys = r.stage;
-              if (!fs_wait(&B->full[ys], r.phase, abort_flag, FS_ERR_FULL)) { ok = false; break; }
+              if (!wait_all(&B->full[ys], r.phase, FS_ERR_FULL)) { ok = false; break; }
               r.next();
-              tcgen05_fence_after();
               const uint64_t dy = desc_k + ring16 + ys * unit16;
               const int steps = min(4 * spu, (p.D - u * spu * 64 + 15) / 16);  // 16 columns each
               if (steps == 8) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                   const uint32_t off = (i >> 2) * kSlot16 + (i & 3) * 2;
-                  umma_bf16(d, dx + off, dy + off, idesc_s, (i > 0 || u > 0) ? 1u : 0u);
+                  umma_bf16_elect(d, dx + off, dy + off, idesc_s, (i > 0 || u > 0) ? 1u : 0u);
                 }
               } else {
+#pragma unroll 1
                 for (int i = 0; i < steps; ++i) {
                   const uint32_t off = (i >> 2) * kSlot16 + (i & 3) * 2;
-                  umma_bf16(d, dx + off, dy + off, idesc_s, (i > 0 || u > 0) ? 1u : 0u);
+                  umma_bf16_elect(d, dx + off, dy + off, idesc_s, (i > 0 || u > 0) ? 1u : 0u);
                 }
               }
-              if (!p.x_resident) tcgen05_commit(&B->empty[xs]);
-              if (!p.hold) tcgen05_commit(&B->empty[ys]);
+              if (!p.x_resident) tcgen05_commit_elect(&B->empty[xs]);
+              if (!p.hold) tcgen05_commit_elect(&B->empty[ys]);
             }
             if (!ok) break;
-            tcgen05_commit(&B->s_full[b]);
-            if (p.x_resident && t == nt - 1) tcgen05_commit(&B->x_empty);
+            tcgen05_commit_elect(&B->s_full[b]);
+            if (p.x_resident && t == nt - 1) tcgen05_commit_elect(&B->x_empty);
             ++tc;
           }
           if (kAcc && t > 0) {
             const uint32_t tt = (t < nt) ? tc - 2 : tc - 1;  // tile whose E is multiplied now
-            if (t == 1 && item > 0 && !fs_wait(&B->o_empty, (item - 1) & 1, abort_flag, FS_ERR_ACC)) { ok = false; break; }
-            if (!fs_wait(&B->p_full[tt & 1], (tt >> 1) & 1, abort_flag, FS_ERR_P)) { ok = false; break; }
+            if (t == 1 && item > 0 && !wait_all(&B->o_empty, (item - 1) & 1, FS_ERR_ACC)) { ok = false; break; }
+            if (!wait_all(&B->p_full[tt & 1], (tt >> 1) & 1, FS_ERR_P)) { ok = false; break; }
             tcgen05_fence_after();
             const uint32_t e = tmem + (tt & 1) * kFsTile;
-            uint32_t hs = held[(t - 1) & 1];
+            uint32_t hs = t < nt ? held_before : held;
             for (int u = pu0; u < pu1; ++u) {
               uint32_t ys = hs;
               if (p.hold) {
                 if (++hs == units) hs = 0;
               } else {
                 ys = r.stage;
-                if (!fs_wait(&B->full[ys], r.phase, abort_flag, FS_ERR_FULL)) { ok = false; break; }
+                if (!wait_all(&B->full[ys], r.phase, FS_ERR_FULL)) { ok = false; break; }
                 r.next();
-                tcgen05_fence_after();
               }
               const int n = min(64 * spu, (p.D - u * 64 * spu + 15) / 16 * 16);
               const uint32_t idesc = fs_idesc(n, true), d = tmem + 256 + (u - pu0) * 128;
               const uint64_t dy = desc_mn + ring16 + ys * unit16;
 #pragma unroll
-              for (int i = 0; i < 8; ++i) umma_bf16_ts(d, e + i * 8, dy + i * 128, idesc, (i > 0 || t > 1) ? 1u : 0u);
-              tcgen05_commit(&B->empty[ys]);
+              for (int i = 0; i < 8; ++i) umma_bf16_ts_elect(d, e + i * 8, dy + i * 128, idesc, (i > 0 || t > 1) ? 1u : 0u);
+              tcgen05_commit_elect(&B->empty[ys]);
             }
-            if (ok) tcgen05_commit(&B->acc_done[tt & 1]);
+            if (ok) tcgen05_commit_elect(&B->acc_done[tt & 1]);
           }
         }
       }
       if (!ok) {  // products already issued must end before the tensor memory is freed
-        tcgen05_commit(&B->drain);
+        tcgen05_commit_elect(&B->drain);
         const long long begin = clock64();
         while (!mbar_try_wait(&B->drain, 0) && clock64() - begin < kWaitCycles) {
         }
@@ -681,301 +686,387 @@ full_softmax_kernel(const __grid_constant__ CUtensorMap tmapX, const __grid_cons
   }
 }
 
+// ---- workspace ----------------------------------------------------------------------------------------
+// What the forward leaves for the backward, in one allocation: counters, targets, the rows' places, statistics, the padded bias, the
+// compacted rows of h and (with a gradient of h wanted) dh without the upstream factor.
+enum FsCounter : int { FS_N_VALID = 0, FS_N_BAD = 1, FS_JOINED = 2, FS_COUNTERS = 8 };
+
+struct FsState {
+  int* counters;        // [FS_COUNTERS + Ppad / 128]: joined rows of every tile behind the first ones
+  int* target;          // [Ppad] of the compacted rows, -1 behind the last
+  int* orig;            // [Ppad] their rows of h
+  int* slot;            // [P] place of every row of h, or -1
+  float* lse2;          // [Ppad] log sum (base 2), +inf behind the last
+  float* wex;           // [Ppad] 1 - p_t
+  float* bias;          // [Vpad], or null
+  __nv_bfloat16* hc;    // [Ppad, Dp]
+  float* unit;          // [Ppad, Dp], or null
+  int64_t bytes;
+
+  FsState(void* base, int64_t P, int64_t V, int64_t Dp, bool has_bias, bool has_unit) {
+    const int64_t Ppad = (P + kFsTile - 1) / kFsTile * kFsTile, Vpad = (V + kFsTile - 1) / kFsTile * kFsTile;
+    int64_t at = 0;
+    auto take = [&](int64_t n) {
+      uint8_t* r = reinterpret_cast<uint8_t*>(base) + at;
+      at += (n + 255) / 256 * 256;
+      return r;
+    };
+    counters = reinterpret_cast<int*>(take(4 * (FS_COUNTERS + Ppad / kFsTile)));
+    target = reinterpret_cast<int*>(take(4 * Ppad));
+    orig = reinterpret_cast<int*>(take(4 * Ppad));
+    slot = reinterpret_cast<int*>(take(4 * P));
+    lse2 = reinterpret_cast<float*>(take(4 * Ppad));
+    wex = reinterpret_cast<float*>(take(4 * Ppad));
+    bias = has_bias ? reinterpret_cast<float*>(take(4 * Vpad)) : nullptr;
+    hc = reinterpret_cast<__nv_bfloat16*>(take(2 * Ppad * Dp));
+    unit = has_unit ? reinterpret_cast<float*>(take(4 * Ppad * Dp)) : nullptr;
+    bytes = at;
+  }
+};
+
 // ---- before the forward -----------------------------------------------------------------------------
-// Blocks 0..row_blocks-1 put the rows whose target counts one behind the other (in their order), as bf16 with zero columns up to Dp;
-// slot[i] is row i's place or -1.  The remaining blocks copy the bias with -inf behind V.  Every row block counts the targets before
-// its own itself: P targets are at most a few hundred KB in L2, cheaper than another launch.
+// Blocks 0..row_blocks-1 put the rows whose target counts one behind the other (in their order), as bf16 with zero columns up to Dp.
+// The remaining blocks copy the bias with -inf behind V.  Every row block counts the targets before its own itself: P targets are at
+// most a few hundred KB in L2, cheaper than another launch.
 constexpr int kPrepRows = 512;
 
 struct PrepParams {
   const void* h;
   int64_t h_row, h_col;  // strides
   int h_fp32, vec;
-  const int64_t* targets;
+  const void* targets;
   int64_t t_stride, ignore;
+  int t_int32;
   int P, V, D, Dp;
-  __nv_bfloat16* hc;
-  int* n_valid;
-  int* slot;
-  int* target;
-  float* loss_rows;
-  const float* bias_in;
-  float* bias_out;
+  FsState st;
+  float* loss;   // [P] without a reduction, one value with it
+  int reduction;
+  const void* bias_in;
+  int64_t bias_stride;
+  int bias_bf16;
   int row_blocks;
 };
 
-__device__ __forceinline__ int fs_target_kind(int64_t t, const PrepParams& p) { return t == p.ignore ? 0 : (t < 0 || t >= p.V ? 2 : 1); }
+__device__ __forceinline__ int64_t fs_target(int64_t i, const PrepParams& p) {
+  return p.t_int32 ? int64_t(reinterpret_cast<const int*>(p.targets)[i * p.t_stride]) : reinterpret_cast<const int64_t*>(p.targets)[i * p.t_stride];
+}
+// 0 ignored, 1 counts, 1 << 32 outside the classes (so that a sum counts both)
+__device__ __forceinline__ int64_t fs_target_kind(int64_t t, const PrepParams& p) { return t == p.ignore ? 0 : (t < 0 || t >= p.V ? int64_t(1) << 32 : 1); }
 
 __global__ void __launch_bounds__(kPrepRows) full_softmax_prep_kernel(const PrepParams p) {
   if (int(blockIdx.x) >= p.row_blocks) {
-    const int vpad = (p.V + kFsTile - 1) / kFsTile * kFsTile;
-    for (int v = (blockIdx.x - p.row_blocks) * kPrepRows + threadIdx.x; v < vpad; v += (gridDim.x - p.row_blocks) * kPrepRows)
-      p.bias_out[v] = v < p.V ? p.bias_in[v] : -INFINITY;
+    const int64_t vpad = (int64_t(p.V) + kFsTile - 1) / kFsTile * kFsTile;
+    for (int64_t v = int64_t(blockIdx.x - p.row_blocks) * kPrepRows + threadIdx.x; v < vpad; v += int64_t(gridDim.x - p.row_blocks) * kPrepRows)
+      p.st.bias[v] = v >= p.V        ? -INFINITY
+                     : p.bias_bf16 ? __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p.bias_in)[v * p.bias_stride])
+                                   : reinterpret_cast<const float*>(p.bias_in)[v * p.bias_stride];
     return;
   }
-  __shared__ int counts[kPrepRows / 32];
+  constexpr int kWarps = kPrepRows / 32;
+  __shared__ int64_t counts[kWarps], befores[kWarps];
   __shared__ int slots[kPrepRows];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int begin = blockIdx.x * kPrepRows, row = begin + threadIdx.x;
-  int before = 0;
-  for (int i = threadIdx.x; i < begin; i += kPrepRows) before += fs_target_kind(p.targets[i * p.t_stride], p) == 1;
-  const int64_t t = row < p.P ? p.targets[row * p.t_stride] : p.ignore;
-  const int kind = row < p.P ? fs_target_kind(t, p) : 0;
-  const uint32_t mine = __ballot_sync(0xffffffffu, kind == 1);
+  const int64_t begin = int64_t(blockIdx.x) * kPrepRows, row = begin + threadIdx.x;
+  int64_t before = 0;
+  for (int64_t i = threadIdx.x; i < begin; i += kPrepRows) before += fs_target_kind(fs_target(i, p), p);
+  const int64_t t = row < p.P ? fs_target(row, p) : p.ignore;
+  const int64_t kind = fs_target_kind(t, p);
+  const uint32_t mine = __ballot_sync(0xffffffffu, kind == 1), bad = __ballot_sync(0xffffffffu, kind > 1);
   const int in_warp = __popc(mine & ((1u << lane) - 1));
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
-  // base of the block: the sum of every warp's `before`; base of the warp: the valid rows of the warps in front
   if (lane == 0) {
-    counts[warp] = __popc(mine);
-    slots[warp] = before;
+    counts[warp] = __popc(mine) + (int64_t(__popc(bad)) << 32);
+    befores[warp] = before;
   }
   __syncthreads();
-  int first = 0, total = 0;
+  int64_t first = 0, total = 0, block_total = 0;
 #pragma unroll
-  for (int w = 0; w < kPrepRows / 32; ++w) {
-    total += slots[w];
+  for (int w = 0; w < kWarps; ++w) {
+    total += befores[w];
+    block_total += counts[w];
     if (w < warp) first += counts[w];
   }
-  int block_valid = 0;
-#pragma unroll
-  for (int w = 0; w < kPrepRows / 32; ++w) block_valid += counts[w];
-  __syncthreads();
-  const int at = kind == 1 ? total + first + in_warp : -1;
+  const int at = kind == 1 ? int(total & 0x7fffffff) + int(first & 0x7fffffff) + in_warp : -1;
   slots[threadIdx.x] = at;
   if (row < p.P) {
-    p.slot[row] = at;
-    if (at >= 0) p.target[at] = int(t);
-    p.loss_rows[row] = kind == 2 ? __int_as_float(0x7fc00000) : 0.f;
-    if (kind == 2) atomicCAS(&g_fs_error, 0, FS_ERR_TARGET);
+    p.st.slot[row] = at;
+    if (at >= 0) {
+      p.st.target[at] = int(t);
+      p.st.orig[at] = int(row);
+    } else if (p.reduction == 0) {
+      p.loss[row] = kind > 1 ? __int_as_float(0x7fc00000) : 0.f;
+    }
+    if (kind > 1) atomicCAS(&g_fs_error, 0, FS_ERR_TARGET);
   }
+  if (threadIdx.x < kPrepRows / kFsTile && begin + int64_t(threadIdx.x) * kFsTile < p.P) p.st.counters[FS_COUNTERS + begin / kFsTile + threadIdx.x] = 0;
   __syncthreads();
   const bool last = int(blockIdx.x) == p.row_blocks - 1;
-  const int n = total + block_valid, padded = (n + kFsTile - 1) / kFsTile * kFsTile;
+  const int n = int((total + block_total) & 0x7fffffff), padded = (n + kFsTile - 1) / kFsTile * kFsTile;
   if (last) {
-    if (threadIdx.x == 0) *p.n_valid = n;
-    if (n + int(threadIdx.x) < padded) p.target[n + threadIdx.x] = -1;
+    if (threadIdx.x == 0) {
+      const int n_bad = int((total + block_total) >> 32);
+      p.st.counters[FS_N_VALID] = n;
+      p.st.counters[FS_N_BAD] = n_bad;
+      p.st.counters[FS_JOINED] = 0;
+      if (p.reduction != 0 && n == 0) *p.loss = n_bad > 0 ? __int_as_float(0x7fc00000) : 0.f;
+    }
+    if (n + int(threadIdx.x) < padded) p.st.target[n + threadIdx.x] = -1;
   }
   const int vecs = p.Dp / 8;
-  const int rows = min(kPrepRows, p.P - begin);
+  const int rows = int(min(int64_t(kPrepRows), p.P - begin));
   // eight columns at a time
   for (int i = threadIdx.x; i < rows * vecs; i += kPrepRows) {
     const int r = i / vecs, c = (i - r * vecs) * 8, to = slots[r];
     if (to < 0) continue;
     uint4 o;
-    if (p.vec && !p.h_fp32) {
-      o = *reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(p.h) + int64_t(begin + r) * p.h_row + c);
+    if (p.vec) {
+      o = *reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(p.h) + (begin + r) * p.h_row + c);
     } else {
       float v[8];
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        const int64_t e = int64_t(begin + r) * p.h_row + int64_t(c + k) * p.h_col;
+        const int64_t e = (begin + r) * p.h_row + int64_t(c + k) * p.h_col;
         v[k] = c + k < p.D ? (p.h_fp32 ? reinterpret_cast<const float*>(p.h)[e] : __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p.h)[e])) : 0.f;
       }
       o = make_uint4(fs_pack(v[0], v[1]), fs_pack(v[2], v[3]), fs_pack(v[4], v[5]), fs_pack(v[6], v[7]));
     }
-    *reinterpret_cast<uint4*>(p.hc + int64_t(to) * p.Dp + c) = o;
+    *reinterpret_cast<uint4*>(p.st.hc + int64_t(to) * p.Dp + c) = o;
   }
   if (last)
-    for (int i = threadIdx.x; i < (padded - n) * vecs; i += kPrepRows) *reinterpret_cast<uint4*>(p.hc + int64_t(n) * p.Dp + int64_t(i) * 8) = make_uint4(0, 0, 0, 0);
+    for (int i = threadIdx.x; i < (padded - n) * vecs; i += kPrepRows) *reinterpret_cast<uint4*>(p.st.hc + int64_t(n) * p.Dp + int64_t(i) * 8) = make_uint4(0, 0, 0, 0);
 }
 
 // ---- after the forward: join the splits of every row --------------------------------------------------
-// One block per row: the splits' weights 2^(m_s - max) go to shared memory, then the threads walk (group of splits, 4 columns).
+// One block per row: the splits' weights 2^(m_s - max) go to shared memory, then the threads walk (group of splits, 4 columns).  The
+// block that finishes a tile of rows last adds up their losses, and the last of those the tiles', in a fixed order.
 constexpr int kJoinThreads = 128;
+static_assert(kJoinThreads == kFsTile, "a tile's losses are added up by one block, a row per thread");
+
+struct JoinParams {
+  FsState st;
+  int V, D, grid, pieces, reduction;
+  const float* part_acc;
+  const float* part_m;
+  const float* part_l;
+  const float* zt;
+  float* loss_c;     // [Ppad]
+  float* tile_loss;  // [Ppad / 128]
+  const __nv_bfloat16* W;
+  int64_t ldw;
+  float* loss;
+};
 
 template <bool ACC>
-__global__ void __launch_bounds__(kJoinThreads) full_softmax_join_kernel(const int* __restrict__ n_valid_p, int V, int D, int grid, int pieces, const float* __restrict__ part_acc,
-                                                                         const float* __restrict__ part_m, const float* __restrict__ part_l, const float* __restrict__ zt,
-                                                                         const int* __restrict__ target, const __nv_bfloat16* __restrict__ W, int64_t ldw,
-                                                                         float* __restrict__ lse2, float* __restrict__ wex, float* __restrict__ loss_c, float* __restrict__ unit) {
+__global__ void __launch_bounds__(kJoinThreads) full_softmax_join_kernel(const JoinParams p) {
   extern __shared__ __align__(16) float js[];  // [splits] weights, then [threads * 4] partial sums
-  const int n = *n_valid_p, row = blockIdx.x;
+  const int n = p.st.counters[FS_N_VALID], row = blockIdx.x;
   const int padded = (n + kFsTile - 1) / kFsTile * kFsTile;
   if (row >= padded) return;
-  if (row >= n) {  // a streamed row of zeros: exp(0 - inf) = 0
-    if (threadIdx.x == 0) lse2[row] = INFINITY;
-    return;
-  }
-  const FsSchedule sc = fs_schedule(n, V, pieces, grid);
-  const int64_t prow = int64_t(sc.tx) * kFsTile;
   __shared__ float red[kJoinThreads / 32];
+  __shared__ int arrived;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  float m = -INFINITY;
-  for (int s = threadIdx.x; s < 2 * sc.splits; s += kJoinThreads) m = fmaxf(m, part_m[s * prow + row]);
-  m = warp_max(m);
-  if (lane == 0) red[warp] = m;
-  __syncthreads();
-  m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-  __syncthreads();
-  const float ms = m == -INFINITY ? 0.f : m;
-  float l = 0.f;
-  for (int s = threadIdx.x; s < 2 * sc.splits; s += kJoinThreads) {
-    const float f = exp2f(part_m[s * prow + row] - ms);
-    l += f * part_l[s * prow + row];
-    if (ACC && !(s & 1)) js[s >> 1] = f;
-  }
-  l = warp_sum(l);
-  if (lane == 0) red[warp] = l;
-  __syncthreads();
-  l = (red[0] + red[1]) + (red[2] + red[3]);
-  // others' log sum a, target's score z (base 2): lse = max + log2(1 + 2^-|a - z|)
-  const float a = ms + log2f(l), z = zt[row], d = a - z;
-  const float tail = log1pf(exp2f(-fabsf(d)));
-  const float loss = (d > 0.f ? d * kLn2 : 0.f) + tail;
-  const float w = d > 0.f ? 1.f / (1.f + exp2f(-d)) : exp2f(d) / (1.f + exp2f(d));  // 1 - p_t
-  if (threadIdx.x == 0) {
-    lse2[row] = fmaxf(a, z) + tail * kLog2e;
-    wex[row] = w;
-    loss_c[row] = d != d ? d : loss;
-  }
-  if constexpr (ACC) {
-    float4* buf = reinterpret_cast<float4*>(js + ((sc.splits + 3) & ~3));
-    const int vecs = D / 4;
-    int lanes = 1;
-    while (lanes < vecs && lanes < kJoinThreads) lanes <<= 1;
-    const int groups = sc.splits > 1 ? kJoinThreads / lanes : 1;
-    const int g = threadIdx.x / lanes, c = threadIdx.x % lanes;
-    const float inv = l > 0.f ? w / l : (l == 0.f ? 0.f : l);
-    const int64_t t = target[row];
-    for (int v0 = 0; v0 < vecs; v0 += lanes) {
-      const int v = v0 + c;
-      float4 s4 = f4zero();
-      if (v < vecs && g < groups)
-        for (int s = g; s < sc.splits; s += groups) {
-          const float4 x = *reinterpret_cast<const float4*>(part_acc + (s * prow + row) * D + v * 4);
-          const float f = js[s];
-          s4.x += f * x.x;
-          s4.y += f * x.y;
-          s4.z += f * x.z;
-          s4.w += f * x.w;
-        }
-      if (groups > 1) {
-        buf[threadIdx.x] = s4;
-        __syncthreads();
-        if (g == 0)
-          for (int k = 1; k < groups; ++k) {
-            const float4 x = buf[k * lanes + c];
-            s4.x += x.x;
-            s4.y += x.y;
-            s4.z += x.z;
-            s4.w += x.w;
-          }
-        __syncthreads();
-      }
-      if (g == 0 && v < vecs) {
-        const float4 wt = Vec4<__nv_bfloat16>::load(W + t * ldw + v * 4);
-        *reinterpret_cast<float4*>(unit + int64_t(row) * D + v * 4) =
-            make_float4(s4.x * inv - w * wt.x, s4.y * inv - w * wt.y, s4.z * inv - w * wt.z, s4.w * inv - w * wt.w);
-      }
-    }
-  }
-}
-
-// rows' losses at their own places, and their sum in a fixed order (one block: P values)
-__global__ void __launch_bounds__(1024) full_softmax_reduce_kernel(int P, const int* __restrict__ n_valid, const int* __restrict__ slot, const float* __restrict__ loss_c,
-                                                                   float* __restrict__ rows, float* __restrict__ out, int mean) {
-  __shared__ float red[32];
-  float s = 0.f;
-  for (int i = threadIdx.x; i < P; i += 1024) {
-    const int at = slot[i];
-    s += at >= 0 ? loss_c[at] : rows[i];
-  }
-  s = warp_sum(s);
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = s;
-  __syncthreads();
-  if (threadIdx.x < 32) {
-    s = warp_sum(red[threadIdx.x]);
-    if (threadIdx.x == 0) *out = mean ? s / float(max(*n_valid, 1)) : s;
-  }
-}
-
-__global__ void full_softmax_rows_kernel(int P, const int* __restrict__ slot, const float* __restrict__ loss_c, float* __restrict__ rows) {
-  const int i = blockIdx.x * blockDim.x + threadIdx.x;
-  if (i < P && slot[i] >= 0) rows[i] = loss_c[slot[i]];
-}
-
-// ---- backward: dh = g * unit at the rows' own places, and the per-row factors of the compacted rows --------
-template <typename T>
-__global__ void full_softmax_dh_kernel(int P, int D, int Dp, const int* __restrict__ n_valid, const int* __restrict__ slot, const float* __restrict__ unit,
-                                       const float* __restrict__ dloss, int64_t dl_stride, int per_row, int mean, T* __restrict__ dh, float* __restrict__ gcol) {
-  const int vecs = Dp / 8;
-  const int64_t idx = int64_t(blockIdx.x) * blockDim.x + threadIdx.x;
-  const int n = *n_valid;
-  if (gcol != nullptr && blockIdx.x == 0) {
-    const int padded = (n + kFsTile - 1) / kFsTile * kFsTile;
-    if (n + int(threadIdx.x) < padded) gcol[n + threadIdx.x] = 0.f;  // 256 threads cover the at most 127 rows
-  }
-  const int64_t row = idx / vecs;
-  if (row >= P) return;
-  const int c = int(idx - row * vecs) * 8;
-  const int at = slot[row];
-  const float g = per_row ? dloss[row * dl_stride] : *dloss / (mean ? float(max(n, 1)) : 1.f);
-  if (gcol != nullptr && c == 0 && at >= 0) gcol[at] = g;
-  if (dh == nullptr) return;
-  float v[8];
-#pragma unroll
-  for (int k = 0; k < 8; ++k) v[k] = 0.f;
-  if (at >= 0) {
-    const float4* u = reinterpret_cast<const float4*>(unit + int64_t(at) * Dp + c);
-    const float4 a = u[0], b = u[1];
-    v[0] = a.x * g; v[1] = a.y * g; v[2] = a.z * g; v[3] = a.w * g;
-    v[4] = b.x * g; v[5] = b.y * g; v[6] = b.z * g; v[7] = b.w * g;
-  }
-  T* o = dh + row * D + c;
-  if (D == Dp) {
-    if constexpr (sizeof(T) == 2) {
-      *reinterpret_cast<uint4*>(o) = make_uint4(fs_pack(v[0], v[1]), fs_pack(v[2], v[3]), fs_pack(v[4], v[5]), fs_pack(v[6], v[7]));
-    } else {
-      reinterpret_cast<float4*>(o)[0] = make_float4(v[0], v[1], v[2], v[3]);
-      reinterpret_cast<float4*>(o)[1] = make_float4(v[4], v[5], v[6], v[7]);
-    }
+  auto block_sum = [&](float v) {
+    v = warp_sum(v);
+    __syncthreads();
+    if (lane == 0) red[warp] = v;
+    __syncthreads();
+    return (red[0] + red[1]) + (red[2] + red[3]);
+  };
+  if (row >= n) {  // a streamed row of zeros: exp(0 - inf) = 0
+    if (threadIdx.x == 0) p.st.lse2[row] = INFINITY;
   } else {
-    for (int k = 0; k < 8 && c + k < D; ++k) o[k] = T(v[k]);
-  }
-}
-
-// ---- backward: join the splits of dW, and db ----------------------------------------------------------------
-template <typename T>
-__global__ void full_softmax_dw_kernel(const int* __restrict__ n_valid, int V, int D, int grid, int pieces, const float* __restrict__ part_acc, const float* __restrict__ dloss,
-                                       int per_row, int mean, T* __restrict__ dw) {
-  const FsSchedule sc = fs_schedule(V, *n_valid, pieces, grid);
-  if (sc.splits == 1) return;  // written by the main kernel
-  const int64_t stride = int64_t(sc.tx) * kFsTile * D;
-  const float scale = per_row ? 1.f : *dloss / (mean ? float(max(*n_valid, 1)) : 1.f);
-  for (int64_t i = (int64_t(blockIdx.x) * blockDim.x + threadIdx.x) * 4; i < int64_t(V) * D; i += int64_t(gridDim.x) * blockDim.x * 4) {
-    float4 s4 = f4zero();
-    for (int s = 0; s < sc.splits; ++s) {
-      const float4 x = *reinterpret_cast<const float4*>(part_acc + s * stride + i);
-      s4.x += x.x;
-      s4.y += x.y;
-      s4.z += x.z;
-      s4.w += x.w;
+    const FsSchedule sc = fs_schedule(n, p.V, p.pieces, p.grid);
+    const int64_t prow = int64_t(sc.tx) * kFsTile;
+    float m = -INFINITY;
+    for (int s = threadIdx.x; s < 2 * sc.splits; s += kJoinThreads) m = fmaxf(m, p.part_m[s * prow + row]);
+    m = warp_max(m);
+    if (lane == 0) red[warp] = m;
+    __syncthreads();
+    m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    const float ms = m == -INFINITY ? 0.f : m;
+    float l = 0.f;
+    for (int s = threadIdx.x; s < 2 * sc.splits; s += kJoinThreads) {
+      const float f = exp2f(p.part_m[s * prow + row] - ms);
+      l += f * p.part_l[s * prow + row];
+      if (ACC && !(s & 1)) js[s >> 1] = f;
     }
-    Vec4<T>::store(dw + i, make_float4(s4.x * scale, s4.y * scale, s4.z * scale, s4.w * scale));
+    l = block_sum(l);
+    // others' log sum a, target's score z (base 2): lse = max + log2(1 + 2^-|a - z|)
+    const float a = ms + log2f(l), z = p.zt[row], d = a - z;
+    const float tail = log1pf(exp2f(-fabsf(d)));
+    const float w = d > 0.f ? 1.f / (1.f + exp2f(-d)) : exp2f(d) / (1.f + exp2f(d));  // 1 - p_t
+    if (threadIdx.x == 0) {
+      const float loss = d != d ? d : (d > 0.f ? d * kLn2 : 0.f) + tail;
+      p.st.lse2[row] = fmaxf(a, z) + tail * kLog2e;
+      p.st.wex[row] = w;
+      if (p.reduction == 0) p.loss[p.st.orig[row]] = loss;
+      else p.loss_c[row] = loss;
+    }
+    if constexpr (ACC) {
+      float4* buf = reinterpret_cast<float4*>(js + ((sc.splits + 3) & ~3));
+      const int vecs = p.D / 4;
+      int lanes = 1;
+      while (lanes < vecs && lanes < kJoinThreads) lanes <<= 1;
+      const int groups = sc.splits > 1 ? kJoinThreads / lanes : 1;
+      const int g = threadIdx.x / lanes, c = threadIdx.x % lanes;
+      const float inv = l > 0.f ? w / l : (l == 0.f ? 0.f : l);
+      const int64_t t = p.st.target[row];
+      for (int v0 = 0; v0 < vecs; v0 += lanes) {
+        const int v = v0 + c;
+        float4 s4 = f4zero();
+        if (v < vecs && g < groups)
+          for (int s = g; s < sc.splits; s += groups) {
+            const float4 x = *reinterpret_cast<const float4*>(p.part_acc + (s * prow + row) * p.D + v * 4);
+            const float f = js[s];
+            s4.x += f * x.x;
+            s4.y += f * x.y;
+            s4.z += f * x.z;
+            s4.w += f * x.w;
+          }
+        if (groups > 1) {
+          buf[threadIdx.x] = s4;
+          __syncthreads();
+          if (g == 0)
+            for (int k = 1; k < groups; ++k) {
+              const float4 x = buf[k * lanes + c];
+              s4.x += x.x;
+              s4.y += x.y;
+              s4.z += x.z;
+              s4.w += x.w;
+            }
+          __syncthreads();
+        }
+        if (g == 0 && v < vecs) {
+          const float4 wt = Vec4<__nv_bfloat16>::load(p.W + t * p.ldw + v * 4);
+          *reinterpret_cast<float4*>(p.st.unit + int64_t(row) * p.D + v * 4) =
+              make_float4(s4.x * inv - w * wt.x, s4.y * inv - w * wt.y, s4.z * inv - w * wt.z, s4.w * inv - w * wt.w);
+        }
+      }
+    }
+  }
+  if (p.reduction == 0) return;
+  auto last_of = [&](int* counter, int count) {
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      __threadfence();
+      arrived = atomicAdd(counter, 1);
+    }
+    __syncthreads();
+    if (arrived != count - 1) return false;
+    __threadfence();
+    return true;
+  };
+  const int tile = row / kFsTile;
+  if (!last_of(p.st.counters + FS_COUNTERS + tile, kFsTile)) return;
+  const int i = tile * kFsTile + threadIdx.x;
+  float s = block_sum(i < n ? __ldcg(p.loss_c + i) : 0.f);
+  if (threadIdx.x == 0) p.tile_loss[tile] = s;
+  if (!last_of(p.st.counters + FS_JOINED, padded / kFsTile)) return;
+  s = 0.f;
+  for (int k = threadIdx.x; k < padded / kFsTile; k += kJoinThreads) s += __ldcg(p.tile_loss + k);
+  s = block_sum(s);
+  if (threadIdx.x == 0) *p.loss = p.st.counters[FS_N_BAD] > 0 ? __int_as_float(0x7fc00000) : (p.reduction == 1 ? s / float(n) : s);
+}
+
+// ---- backward ---------------------------------------------------------------------------------------------
+// upstream gradients of the compacted rows (no reduction), zero behind the last
+__global__ void full_softmax_gcol_kernel(FsState st, const float* __restrict__ dloss, int64_t stride, float* __restrict__ gcol) {
+  const int n = st.counters[FS_N_VALID], i = blockIdx.x * blockDim.x + threadIdx.x;
+  if (i < (n + kFsTile - 1) / kFsTile * kFsTile) gcol[i] = i < n ? dloss[st.orig[i] * stride] : 0.f;
+}
+
+struct FinishParams {
+  FsState st;
+  int P, V, D, Dp, grid, pieces, per_row, mean;
+  const float* dloss;
+  int64_t dl_stride;
+  const float* part_acc;  // or null: dW was written by the main kernel
+  const float* part_l;
+  void* dh;               // [P, D] or null
+  void* dw;               // [V, Dp]
+  void* db;               // [V] or null
+  int db_bf16;
+};
+
+template <typename T>
+__device__ __forceinline__ void fs_store8(T* o, const float (&v)[8]) {
+  if constexpr (sizeof(T) == 2) {
+    *reinterpret_cast<uint4*>(o) = make_uint4(fs_pack(v[0], v[1]), fs_pack(v[2], v[3]), fs_pack(v[4], v[5]), fs_pack(v[6], v[7]));
+  } else {
+    reinterpret_cast<float4*>(o)[0] = make_float4(v[0], v[1], v[2], v[3]);
+    reinterpret_cast<float4*>(o)[1] = make_float4(v[4], v[5], v[6], v[7]);
   }
 }
 
-__global__ void full_softmax_db_kernel(const int* __restrict__ n_valid, int V, int grid, int pieces, const float* __restrict__ part_l, const float* __restrict__ dloss, int per_row,
-                                       int mean, float* __restrict__ db) {
-  const FsSchedule sc = fs_schedule(V, *n_valid, pieces, grid);
-  const int v = blockIdx.x * blockDim.x + threadIdx.x;
-  if (v >= V) return;
+// dh = g * unit at the rows' own places; the splits of dW and db joined in their order
+template <typename TH, typename TW>
+__global__ void __launch_bounds__(256) full_softmax_finish_kernel(const FinishParams p) {
+  const int n = p.st.counters[FS_N_VALID], vecs = p.Dp / 8;
+  const int64_t step = int64_t(gridDim.x) * blockDim.x, me = int64_t(blockIdx.x) * blockDim.x + threadIdx.x;
+  const float g_all = p.per_row ? 1.f : *p.dloss / (p.mean ? float(max(n, 1)) : 1.f);
+  if (p.dh != nullptr) {
+    for (int64_t i = me; i < int64_t(p.P) * vecs; i += step) {
+      const int64_t row = i / vecs;
+      const int c = int(i - row * vecs) * 8, at = p.st.slot[row];
+      float v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = 0.f;
+      if (at >= 0) {
+        const float g = p.per_row ? p.dloss[row * p.dl_stride] : g_all;
+        const float4* u = reinterpret_cast<const float4*>(p.st.unit + int64_t(at) * p.Dp + c);
+        const float4 a = u[0], b = u[1];
+        v[0] = a.x * g; v[1] = a.y * g; v[2] = a.z * g; v[3] = a.w * g;
+        v[4] = b.x * g; v[5] = b.y * g; v[6] = b.z * g; v[7] = b.w * g;
+      }
+      TH* o = reinterpret_cast<TH*>(p.dh) + row * p.D + c;
+      if (p.D == p.Dp) {
+        fs_store8(o, v);
+      } else {
+        for (int k = 0; k < 8 && c + k < p.D; ++k) o[k] = TH(v[k]);
+      }
+    }
+  }
+  if (p.part_acc == nullptr && p.db == nullptr) return;
+  const FsSchedule sc = fs_schedule(p.V, n, p.pieces, p.grid);
   const int64_t prow = int64_t(sc.tx) * kFsTile;
-  float s = 0.f;
-  for (int k = 0; k < 2 * sc.splits; ++k) s += part_l[k * prow + v];
-  db[v] = per_row ? s : s * (*dloss / (mean ? float(max(*n_valid, 1)) : 1.f));
+  if (p.part_acc != nullptr && sc.splits > 1) {
+    for (int64_t i = me; i < int64_t(p.V) * vecs; i += step) {
+      float v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = 0.f;
+      for (int s = 0; s < sc.splits; ++s) {
+        const float4* x = reinterpret_cast<const float4*>(p.part_acc + s * prow * p.Dp + i * 8);
+        const float4 a = x[0], b = x[1];
+        v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
+        v[4] += b.x; v[5] += b.y; v[6] += b.z; v[7] += b.w;
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] *= g_all;
+      fs_store8(reinterpret_cast<TW*>(p.dw) + i * 8, v);
+    }
+  }
+  if (p.db != nullptr)
+    for (int64_t v = me; v < p.V; v += step) {
+      float s = 0.f;
+      for (int k = 0; k < 2 * sc.splits; ++k) s += p.part_l[k * prow + v];
+      s *= g_all;
+      if (p.db_bf16) reinterpret_cast<__nv_bfloat16*>(p.db)[v] = __float2bfloat16(s);
+      else reinterpret_cast<float*>(p.db)[v] = s;
+    }
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------
-static int fs_grid(const at::Device& dev) {
-  return at::cuda::getDeviceProperties(dev.index())->multiProcessorCount;
-}
+static int fs_grid(const at::Device& dev) { return at::cuda::getDeviceProperties(dev.index())->multiProcessorCount; }
 
 template <int MODE, bool BIAS, bool ROWG>
-static void fs_launch(const CUtensorMap& tx, const CUtensorMap& ty, const FsParams& p) {
+static void fs_launch(const CUtensorMap& tx, const CUtensorMap& ty, const FsParams& p, int device) {
   auto kernel = full_softmax_kernel<MODE, BIAS, ROWG>;
-  TRB_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kFsSmem));
+  static bool set[64] = {};  // the attribute is per kernel and device; setting it twice is harmless
+  if (device >= 64 || !set[device]) {
+    TRB_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kFsSmem));
+    if (device < 64) set[device] = true;
+  }
   kernel<<<p.grid, kFsThreads, kFsSmem, at::cuda::getCurrentCUDAStream()>>>(tx, ty, p);
   TRB_CUDA_CHECK(cudaGetLastError());
 }
@@ -991,204 +1082,158 @@ static void fs_shape(FsParams& p, int64_t V, int64_t D, bool acc) {
 constexpr int64_t kFsMaxRows = (int64_t(1) << 31) - 2 * kFsTile;
 
 static void fs_check_weight(const at::Tensor& w) {
-  TORCH_CHECK(w.is_cuda() && w.scalar_type() == at::kBFloat16 && w.dim() == 2 && w.stride(1) == 1 && w.size(0) >= 1 && w.size(0) < kFsMaxRows,
-              "full_softmax: the weight is a bf16 [V, D] matrix with contiguous rows");
-  TORCH_CHECK(w.size(1) >= 8 && w.size(1) % 8 == 0 && w.size(1) <= kFsMaxD && w.stride(0) % 8 == 0 && w.stride(0) >= w.size(1) &&
-                  reinterpret_cast<uintptr_t>(w.data_ptr()) % 16 == 0,
-              "full_softmax: D and the row pitch of the weight are multiples of 8 (D at most ", kFsMaxD, "), its rows start on 16 bytes");
+  TORCH_CHECK_VALUE(w.is_cuda() && w.scalar_type() == at::kBFloat16 && w.dim() == 2 && w.stride(1) == 1 && w.size(0) >= 1 && w.size(0) < kFsMaxRows,
+                    "full_softmax: the weight is a bf16 [V, D] matrix with contiguous rows");
+  TORCH_CHECK_VALUE(w.size(1) >= 8 && w.size(1) % 8 == 0 && w.size(1) <= kFsMaxD && w.stride(0) % 8 == 0 && w.stride(0) >= w.size(1) &&
+                        reinterpret_cast<uintptr_t>(w.data_ptr()) % 16 == 0,
+                    "full_softmax: D and the row pitch of the weight are multiples of 8 (D at most ", kFsMaxD, "), its rows start on 16 bytes");
 }
 
-// h [P, D] bf16 or fp32 (any strides), weight [V, Dp] bf16 with Dp = D rounded up to 8 (zero columns behind D), targets [P] int64,
-// bias [V] fp32 or none.  reduction: 0 none, 1 mean, 2 sum.  grad: 0 loss only, 1 prepare the backward of W and b, 2 of h too.
-// Returns (loss, hc, meta, stat, unit): the compacted rows [Ppad, Dp], meta = n_valid (4 ints) | targets [Ppad] | slot [P], stat =
-// lse2 [Ppad] | 1 - p_t [Ppad] | padded bias, unit [Ppad, Dp] = dh without the upstream factor (empty unless grad == 2).
-std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> full_softmax_fwd(const at::Tensor& h, const at::Tensor& weight, const at::Tensor& targets,
-                                                                                        const c10::optional<at::Tensor>& bias, int64_t ignore_index, int64_t reduction,
-                                                                                        int64_t grad) {
+// h [P, D] bf16 or fp32 (any strides), weight [V, Dp] bf16 with Dp = D rounded up to 8 (zero columns behind D), targets [P] int64 or
+// int32, bias [V] fp32 or bf16 or none.  reduction: 0 none, 1 mean, 2 sum.  grad: 0 loss only, 1 prepare the backward of W and b, 2 of h
+// too.  Returns the loss and the state for the backward.
+std::tuple<at::Tensor, at::Tensor> full_softmax_fwd(const at::Tensor& h, const at::Tensor& weight, const at::Tensor& targets, const c10::optional<at::Tensor>& bias,
+                                                    int64_t ignore_index, int64_t reduction, int64_t grad) {
   fs_check_weight(weight);
-  TORCH_CHECK(h.is_cuda() && h.dim() == 2 && (h.scalar_type() == at::kBFloat16 || h.scalar_type() == at::kFloat), "full_softmax: h is bf16 or fp32 [P, D]");
-  TORCH_CHECK(targets.is_cuda() && targets.dim() == 1 && targets.scalar_type() == at::kLong && targets.size(0) == h.size(0), "full_softmax: targets is int64 [P]");
-  TORCH_CHECK(h.device() == weight.device() && h.device() == targets.device(), "full_softmax: operands on different devices");
-  TORCH_CHECK(reduction >= 0 && reduction <= 2 && grad >= 0 && grad <= 2);
+  TORCH_CHECK_VALUE(h.is_cuda() && h.dim() == 2 && (h.scalar_type() == at::kBFloat16 || h.scalar_type() == at::kFloat), "full_softmax: h is a bf16 or fp32 CUDA tensor [P, D]");
+  TORCH_CHECK_VALUE(targets.is_cuda() && targets.dim() == 1 && (targets.scalar_type() == at::kLong || targets.scalar_type() == at::kInt) && targets.size(0) == h.size(0),
+                    "full_softmax: targets is an int32 or int64 [P]");
+  TORCH_CHECK_VALUE(h.device() == weight.device() && h.device() == targets.device(), "full_softmax: operands on different devices");
+  TORCH_CHECK_VALUE(reduction >= 0 && reduction <= 2 && grad >= 0 && grad <= 2, "full_softmax: unknown reduction or gradient level");
   const int64_t P = h.size(0), D = h.size(1), V = weight.size(0), Dp = weight.size(1);
-  TORCH_CHECK(P < kFsMaxRows && D >= 1 && D <= Dp && Dp - D < 8, "full_softmax: h and weight differ in width");
+  TORCH_CHECK_VALUE(P < kFsMaxRows && D >= 1 && D <= Dp && Dp - D < 8, "full_softmax: h and weight differ in width");
   const bool has_bias = bias.has_value() && bias->defined();
   if (has_bias)
-    TORCH_CHECK(bias->is_cuda() && bias->device() == h.device() && bias->scalar_type() == at::kFloat && bias->dim() == 1 && bias->size(0) == V && bias->is_contiguous(),
-                "full_softmax: bias is fp32 [V]");
+    TORCH_CHECK_VALUE(bias->is_cuda() && bias->device() == h.device() && (bias->scalar_type() == at::kFloat || bias->scalar_type() == at::kBFloat16) && bias->dim() == 1 &&
+                          bias->size(0) == V,
+                      "full_softmax: bias is an fp32 or bf16 [V]");
   c10::cuda::CUDAGuard guard(h.device());
   auto stream = at::cuda::getCurrentCUDAStream();
   const int64_t Ppad = (P + kFsTile - 1) / kFsTile * kFsTile, Vpad = (V + kFsTile - 1) / kFsTile * kFsTile;
   const auto f32 = h.options().dtype(at::kFloat);
-  at::Tensor hc = at::empty({Ppad, Dp}, h.options().dtype(at::kBFloat16));
-  at::Tensor meta = at::empty({4 + Ppad + P}, h.options().dtype(at::kInt));
-  at::Tensor stat = at::empty({2 * Ppad + (has_bias ? Vpad : 0)}, f32);
-  at::Tensor unit = at::empty({grad == 2 ? Ppad : 0, Dp}, f32);
-  at::Tensor rows = at::empty({P}, f32);
+  const bool acc = grad == 2;
+  at::Tensor state = at::empty({FsState(nullptr, P, V, Dp, has_bias, acc).bytes}, h.options().dtype(at::kByte));
+  const FsState st(state.data_ptr(), P, V, Dp, has_bias, acc);
+  at::Tensor loss = reduction == 0 ? at::empty({P}, f32) : at::empty({}, f32);
   if (P == 0) {
-    meta.zero_();
-    return {reduction == 0 ? rows : at::zeros({}, f32), hc, meta, stat, unit};
+    state.zero_();
+    if (reduction != 0) loss.zero_();
+    return {loss, state};
   }
   const int grid = fs_grid(h.device());
-  const bool acc = grad == 2;
   const int pieces = acc ? int((Dp + kFsAcc - 1) / kFsAcc) : 1;
   const int64_t prows = fs_partial_rows(P, V, grid);
-  at::Tensor part_acc = acc ? at::empty({prows, Dp}, f32) : at::Tensor();
-  at::Tensor part = at::empty({4 * prows + 2 * Ppad}, f32);  // maxima, sums (two halves each); targets' scores, compacted losses
-  float* part_m = part.data_ptr<float>();
+  at::Tensor part = at::empty({(acc ? prows * Dp : 0) + 4 * prows + 2 * Ppad + Ppad / kFsTile}, f32);  // accumulators, maxima, sums, targets' scores, losses
+  float* part_acc = part.data_ptr<float>();
+  float* part_m = part_acc + (acc ? prows * Dp : 0);
   float* part_l = part_m + 2 * prows;
   float* zt = part_l + 2 * prows;
   float* loss_c = zt + Ppad;
-  int* n_valid = meta.data_ptr<int>();
-  int* target = n_valid + 4;
-  int* slot = target + Ppad;
-  float* lse2 = stat.data_ptr<float>();
-  float* wex = lse2 + Ppad;
-  float* bias_ws = has_bias ? wex + Ppad : nullptr;
   {
-    PrepParams q{};
-    q.h = h.data_ptr();
-    q.h_row = h.stride(0);
-    q.h_col = h.stride(1);
-    q.h_fp32 = h.scalar_type() == at::kFloat;
-    q.vec = !q.h_fp32 && D == Dp && q.h_col == 1 && q.h_row % 8 == 0 && reinterpret_cast<uintptr_t>(q.h) % 16 == 0;
-    q.targets = targets.data_ptr<int64_t>();
-    q.t_stride = targets.stride(0);
-    q.ignore = ignore_index;
-    q.P = int(P);
-    q.V = int(V);
-    q.D = int(D);
-    q.Dp = int(Dp);
-    q.hc = reinterpret_cast<__nv_bfloat16*>(hc.data_ptr());
-    q.n_valid = n_valid;
-    q.slot = slot;
-    q.target = target;
-    q.loss_rows = rows.data_ptr<float>();
-    q.bias_in = has_bias ? bias->data_ptr<float>() : nullptr;
-    q.bias_out = bias_ws;
-    q.row_blocks = int((P + kPrepRows - 1) / kPrepRows);
+    const int row_blocks = int((P + kPrepRows - 1) / kPrepRows);
     const int bias_blocks = has_bias ? int(std::min<int64_t>((Vpad + kPrepRows - 1) / kPrepRows, 2 * grid)) : 0;
-    full_softmax_prep_kernel<<<q.row_blocks + bias_blocks, kPrepRows, 0, stream>>>(q);
+    const bool fp32 = h.scalar_type() == at::kFloat;
+    const bool vec = !fp32 && D == Dp && h.stride(1) == 1 && h.stride(0) % 8 == 0 && reinterpret_cast<uintptr_t>(h.data_ptr()) % 16 == 0;
+    const PrepParams q{h.data_ptr(), h.stride(0), h.stride(1), fp32, vec, targets.data_ptr(), targets.stride(0), ignore_index, targets.scalar_type() == at::kInt,
+                       int(P), int(V), int(D), int(Dp), st, loss.data_ptr<float>(), int(reduction), has_bias ? bias->data_ptr() : nullptr, has_bias ? bias->stride(0) : 0,
+                       has_bias && bias->scalar_type() == at::kBFloat16, row_blocks};
+    full_softmax_prep_kernel<<<row_blocks + bias_blocks, kPrepRows, 0, stream>>>(q);
     TRB_CUDA_CHECK(cudaGetLastError());
   }
   FsParams p{};
   fs_shape(p, V, Dp, acc);
-  p.n_valid = n_valid;
+  p.n_valid = st.counters + FS_N_VALID;
   p.grid = grid;
-  p.target = target;
-  p.bias = bias_ws;
-  p.part_acc = acc ? part_acc.data_ptr<float>() : nullptr;
+  p.target = st.target;
+  p.bias = st.bias;
+  p.part_acc = part_acc;
   p.part_m = part_m;
   p.part_l = part_l;
   p.zt = zt;
-  const CUtensorMap tx = make_tmap(hc.data_ptr(), Ppad, Dp, Dp, 64, kFsTile);
+  const CUtensorMap tx = make_tmap(st.hc, Ppad, Dp, Dp, 64, kFsTile);
   const CUtensorMap ty = make_tmap(weight.data_ptr(), V, Dp, weight.stride(0), 64, kFsTile);
-  if (acc) has_bias ? fs_launch<FS_FWD, true, false>(tx, ty, p) : fs_launch<FS_FWD, false, false>(tx, ty, p);
-  else has_bias ? fs_launch<FS_LSE, true, false>(tx, ty, p) : fs_launch<FS_LSE, false, false>(tx, ty, p);
-  {
-    const int smem = (kFsItemsPerSm * grid + 8) * 4 + kJoinThreads * 16;
-    const auto* w = reinterpret_cast<const __nv_bfloat16*>(weight.data_ptr());
-    auto join = acc ? full_softmax_join_kernel<true> : full_softmax_join_kernel<false>;
-    join<<<unsigned(Ppad), kJoinThreads, smem, stream>>>(n_valid, int(V), int(Dp), grid, pieces, p.part_acc, part_m, part_l, zt, target, w, weight.stride(0), lse2, wex, loss_c,
-                                                         acc ? unit.data_ptr<float>() : nullptr);
-    TRB_CUDA_CHECK(cudaGetLastError());
-  }
-  if (reduction == 0) {
-    full_softmax_rows_kernel<<<unsigned((P + 255) / 256), 256, 0, stream>>>(int(P), slot, loss_c, rows.data_ptr<float>());
-    TRB_CUDA_CHECK(cudaGetLastError());
-    return {rows, hc, meta, stat, unit};
-  }
-  at::Tensor loss = at::empty({}, f32);
-  full_softmax_reduce_kernel<<<1, 1024, 0, stream>>>(int(P), n_valid, slot, loss_c, rows.data_ptr<float>(), loss.data_ptr<float>(), reduction == 1);
+  const int dev = h.device().index();
+  if (acc) has_bias ? fs_launch<FS_FWD, true, false>(tx, ty, p, dev) : fs_launch<FS_FWD, false, false>(tx, ty, p, dev);
+  else has_bias ? fs_launch<FS_LSE, true, false>(tx, ty, p, dev) : fs_launch<FS_LSE, false, false>(tx, ty, p, dev);
+  const JoinParams j{st, int(V), int(Dp), grid, pieces, int(reduction), part_acc, part_m, part_l, zt, loss_c, loss_c + Ppad, reinterpret_cast<const __nv_bfloat16*>(weight.data_ptr()),
+                     weight.stride(0), loss.data_ptr<float>()};
+  const int smem = (kFsItemsPerSm * grid + 8) * 4 + kJoinThreads * 16;
+  if (acc) full_softmax_join_kernel<true><<<unsigned(Ppad), kJoinThreads, smem, stream>>>(j);
+  else full_softmax_join_kernel<false><<<unsigned(Ppad), kJoinThreads, 0, stream>>>(j);
   TRB_CUDA_CHECK(cudaGetLastError());
-  return {loss, hc, meta, stat, unit};
+  return {loss, state};
 }
 
 // dloss: fp32, [P] for reduction 0, a scalar otherwise.  Outputs that are not wanted come back empty.  dh [P, D] in bf16 or fp32,
-// dW [V, Dp] in bf16 or fp32, db [V] in fp32.
-std::tuple<at::Tensor, at::Tensor, at::Tensor> full_softmax_bwd(const at::Tensor& dloss, const at::Tensor& weight, const at::Tensor& hc, const at::Tensor& meta, const at::Tensor& stat,
-                                                                const at::Tensor& unit, int64_t P, int64_t D, bool has_bias, int64_t reduction, bool want_h, bool want_w, bool want_b,
-                                                                bool dh_fp32, bool dw_fp32) {
+// dW [V, Dp] in bf16 or fp32, db [V] in fp32 or bf16.
+std::tuple<at::Tensor, at::Tensor, at::Tensor> full_softmax_bwd(const at::Tensor& dloss, const at::Tensor& weight, const at::Tensor& state, int64_t P, int64_t D, bool has_bias,
+                                                                int64_t reduction, bool has_unit, bool want_h, bool want_w, bool want_b, bool dh_fp32, bool dw_fp32, bool db_fp32) {
   fs_check_weight(weight);
-  const int64_t V = weight.size(0), Dp = weight.size(1), Ppad = (P + kFsTile - 1) / kFsTile * kFsTile, Vpad = (V + kFsTile - 1) / kFsTile * kFsTile;
-  const at::Device dev = weight.device();
-  TORCH_CHECK(dloss.device() == dev && dloss.scalar_type() == at::kFloat && (reduction == 0 ? dloss.dim() == 1 && dloss.size(0) == P : dloss.numel() == 1),
-              "full_softmax_bwd: the upstream gradient is fp32, [P] without a reduction and one value with it");
+  const int64_t V = weight.size(0), Dp = weight.size(1);
+  const at::Device device = weight.device();
   TORCH_CHECK(P >= 0 && P < kFsMaxRows && D >= 1 && D <= Dp && Dp - D < 8 && reduction >= 0 && reduction <= 2);
-  TORCH_CHECK(hc.device() == dev && hc.scalar_type() == at::kBFloat16 && hc.is_contiguous() && hc.dim() == 2 && hc.size(0) == Ppad && hc.size(1) == Dp);
-  TORCH_CHECK(meta.device() == dev && meta.scalar_type() == at::kInt && meta.is_contiguous() && meta.numel() == 4 + Ppad + P);
-  TORCH_CHECK(stat.device() == dev && stat.scalar_type() == at::kFloat && stat.is_contiguous() && stat.numel() == 2 * Ppad + (has_bias ? Vpad : 0));
-  TORCH_CHECK(!want_h || (unit.device() == dev && unit.scalar_type() == at::kFloat && unit.is_contiguous() && unit.numel() == Ppad * Dp));
-  TORCH_CHECK(!want_b || has_bias);
-  c10::cuda::CUDAGuard guard(dev);
+  TORCH_CHECK(dloss.device() == device && dloss.scalar_type() == at::kFloat && (reduction == 0 ? dloss.dim() == 1 && dloss.size(0) == P : dloss.numel() == 1),
+              "full_softmax_bwd: the upstream gradient is fp32, [P] without a reduction and one value with it");
+  TORCH_CHECK((!want_b || has_bias) && (!want_h || has_unit));
+  TORCH_CHECK(state.device() == device && state.scalar_type() == at::kByte && state.is_contiguous() && state.numel() == FsState(nullptr, P, V, Dp, has_bias, has_unit).bytes,
+              "full_softmax_bwd: not the state of this forward");
+  const FsState st(state.data_ptr(), P, V, Dp, has_bias, has_unit);
+  c10::cuda::CUDAGuard guard(device);
   auto stream = at::cuda::getCurrentCUDAStream();
-  const auto f32 = hc.options().dtype(at::kFloat);
-  at::Tensor dh = at::empty({want_h ? P : 0, D}, dh_fp32 ? f32 : hc.options());
+  const auto f32 = weight.options().dtype(at::kFloat);
   const bool main = want_w || want_b;
-  at::Tensor dw = at::empty({main ? V : 0, Dp}, dw_fp32 ? f32 : hc.options());  // the kernel that sums db computes dW on the way
-  at::Tensor db = at::empty({want_b ? V : 0}, f32);
+  at::Tensor dh = at::empty({want_h ? P : 0, D}, dh_fp32 ? f32 : weight.options());
+  at::Tensor dw = at::empty({main ? V : 0, Dp}, dw_fp32 ? f32 : weight.options());  // the kernel that sums db computes dW on the way
+  at::Tensor db = at::empty({want_b ? V : 0}, db_fp32 ? f32 : weight.options());
   if (P == 0) {
     dw.zero_();
     db.zero_();
     return {dh, dw, db};
   }
-  const int grid = fs_grid(dev);
-  const int* n_valid = meta.data_ptr<int>();
-  const int* target = n_valid + 4;
-  const int* slot = target + Ppad;
-  const float* lse2 = stat.data_ptr<float>();
+  const int64_t Ppad = (P + kFsTile - 1) / kFsTile * kFsTile, Vpad = (V + kFsTile - 1) / kFsTile * kFsTile;
+  const int grid = fs_grid(device), dev = device.index();
   const bool per_row = reduction == 0, mean = reduction == 1;
-  at::Tensor gcol = per_row && main ? at::empty({Ppad}, f32) : at::Tensor();
-  if (want_h || gcol.defined()) {
-    const int64_t work = P * (Dp / 8);
-    const unsigned blocks = unsigned((work + 255) / 256);
-    const int64_t stride = per_row ? dloss.stride(0) : 0;
-    float* gc = gcol.defined() ? gcol.data_ptr<float>() : nullptr;
-    const float* u = want_h ? unit.data_ptr<float>() : nullptr;
-    if (dh_fp32)
-      full_softmax_dh_kernel<float><<<blocks, 256, 0, stream>>>(int(P), int(D), int(Dp), n_valid, slot, u, dloss.data_ptr<float>(), stride, per_row, mean,
-                                                                want_h ? dh.data_ptr<float>() : nullptr, gc);
-    else
-      full_softmax_dh_kernel<__nv_bfloat16><<<blocks, 256, 0, stream>>>(int(P), int(D), int(Dp), n_valid, slot, u, dloss.data_ptr<float>(), stride, per_row, mean,
-                                                                        want_h ? reinterpret_cast<__nv_bfloat16*>(dh.data_ptr()) : nullptr, gc);
-    TRB_CUDA_CHECK(cudaGetLastError());
-  }
-  if (!main) return {dh, dw, db};
   const int pieces = int((Dp + kFsAcc - 1) / kFsAcc);
   const int64_t prows = fs_partial_rows(V, P, grid);
-  const bool may_split = int64_t(kFsItemsPerSm) * grid / (Vpad / kFsTile) > 1 && Ppad > kFsTile;  // mirrors fs_schedule
-  at::Tensor part_acc = may_split ? at::empty({prows, Dp}, f32) : at::Tensor();
-  at::Tensor part_l = want_b || has_bias ? at::empty({2 * prows}, f32) : at::Tensor();
-  FsParams p{};
-  fs_shape(p, V, Dp, true);
-  p.n_valid = n_valid;
-  p.grid = grid;
-  p.target = target;
-  p.bias = has_bias ? lse2 + 2 * Ppad : nullptr;
-  p.part_acc = may_split ? part_acc.data_ptr<float>() : nullptr;
-  p.part_l = part_l.defined() ? part_l.data_ptr<float>() : nullptr;
-  p.lse2 = lse2;
-  p.wex = lse2 + Ppad;
-  p.gcol = gcol.defined() ? gcol.data_ptr<float>() : nullptr;
-  p.dloss = dloss.data_ptr<float>();
-  p.mean = mean;
-  p.dw = dw.data_ptr();
-  p.dw_fp32 = dw_fp32;
-  const CUtensorMap tx = make_tmap(weight.data_ptr(), V, Dp, weight.stride(0), 64, kFsTile);
-  const CUtensorMap ty = make_tmap(hc.data_ptr(), Ppad, Dp, Dp, 64, kFsTile);
-  if (has_bias) per_row ? fs_launch<FS_BWD, true, true>(tx, ty, p) : fs_launch<FS_BWD, true, false>(tx, ty, p);
-  else per_row ? fs_launch<FS_BWD, false, true>(tx, ty, p) : fs_launch<FS_BWD, false, false>(tx, ty, p);
-  if (may_split) {
-    const unsigned blocks = unsigned(std::min<int64_t>((V * Dp / 4 + 255) / 256, 16 * grid));
-    if (dw_fp32)
-      full_softmax_dw_kernel<float><<<blocks, 256, 0, stream>>>(n_valid, int(V), int(Dp), grid, pieces, p.part_acc, p.dloss, per_row, mean, dw.data_ptr<float>());
-    else
-      full_softmax_dw_kernel<__nv_bfloat16><<<blocks, 256, 0, stream>>>(n_valid, int(V), int(Dp), grid, pieces, p.part_acc, p.dloss, per_row, mean,
-                                                                        reinterpret_cast<__nv_bfloat16*>(dw.data_ptr()));
-    TRB_CUDA_CHECK(cudaGetLastError());
+  const bool may_split = main && int64_t(kFsItemsPerSm) * grid / (Vpad / kFsTile) > 1 && Ppad > kFsTile;  // mirrors fs_schedule
+  const int64_t n_acc = may_split ? prows * Dp : 0, n_l = main && has_bias ? 2 * prows : 0, n_g = main && per_row ? Ppad : 0;
+  at::Tensor part = n_acc + n_l + n_g > 0 ? at::empty({n_acc + n_l + n_g}, f32) : at::Tensor();
+  float* part_acc = n_acc ? part.data_ptr<float>() : nullptr;
+  float* part_l = n_l ? part.data_ptr<float>() + n_acc : nullptr;
+  float* gcol = n_g ? part.data_ptr<float>() + n_acc + n_l : nullptr;
+  if (main) {
+    if (gcol != nullptr) {
+      full_softmax_gcol_kernel<<<unsigned((Ppad + 255) / 256), 256, 0, stream>>>(st, dloss.data_ptr<float>(), dloss.stride(0), gcol);
+      TRB_CUDA_CHECK(cudaGetLastError());
+    }
+    FsParams p{};
+    fs_shape(p, V, Dp, true);
+    p.n_valid = st.counters + FS_N_VALID;
+    p.grid = grid;
+    p.target = st.target;
+    p.bias = st.bias;
+    p.part_acc = part_acc;
+    p.part_l = part_l;
+    p.lse2 = st.lse2;
+    p.wex = st.wex;
+    p.gcol = gcol;
+    p.dloss = dloss.data_ptr<float>();
+    p.mean = mean;
+    p.dw = dw.data_ptr();
+    p.dw_fp32 = dw_fp32;
+    const CUtensorMap tx = make_tmap(weight.data_ptr(), V, Dp, weight.stride(0), 64, kFsTile);
+    const CUtensorMap ty = make_tmap(st.hc, Ppad, Dp, Dp, 64, kFsTile);
+    if (has_bias) per_row ? fs_launch<FS_BWD, true, true>(tx, ty, p, dev) : fs_launch<FS_BWD, true, false>(tx, ty, p, dev);
+    else per_row ? fs_launch<FS_BWD, false, true>(tx, ty, p, dev) : fs_launch<FS_BWD, false, false>(tx, ty, p, dev);
   }
-  if (want_b) {
-    full_softmax_db_kernel<<<unsigned((V + 255) / 256), 256, 0, stream>>>(n_valid, int(V), grid, pieces, p.part_l, p.dloss, per_row, mean, db.data_ptr<float>());
+  if (want_h || want_b || may_split) {
+    const FinishParams f{st, int(P), int(V), int(D), int(Dp), grid, pieces, per_row, mean, dloss.data_ptr<float>(), per_row ? dloss.stride(0) : 0, part_acc, part_l,
+                         want_h ? dh.data_ptr() : nullptr, dw.data_ptr(), want_b ? db.data_ptr() : nullptr, !db_fp32};
+    const int64_t most = std::max<int64_t>({want_h ? P * (Dp / 8) : 0, may_split ? V * (Dp / 8) : 0, want_b ? V : 0});
+    const unsigned blocks = unsigned(std::min<int64_t>((most + 255) / 256, 16 * grid));
+    if (dh_fp32) dw_fp32 ? full_softmax_finish_kernel<float, float><<<blocks, 256, 0, stream>>>(f) : full_softmax_finish_kernel<float, __nv_bfloat16><<<blocks, 256, 0, stream>>>(f);
+    else dw_fp32 ? full_softmax_finish_kernel<__nv_bfloat16, float><<<blocks, 256, 0, stream>>>(f)
+                 : full_softmax_finish_kernel<__nv_bfloat16, __nv_bfloat16><<<blocks, 256, 0, stream>>>(f);
     TRB_CUDA_CHECK(cudaGetLastError());
   }
   return {dh, dw, db};
@@ -1207,9 +1252,9 @@ int64_t full_softmax_status() {
 }  // namespace trb
 
 TORCH_LIBRARY_FRAGMENT(trb200, m) {
-  m.def("full_softmax_fwd(Tensor h, Tensor weight, Tensor targets, Tensor? bias, int ignore_index, int reduction, int grad) -> (Tensor, Tensor, Tensor, Tensor, Tensor)");
-  m.def("full_softmax_bwd(Tensor dloss, Tensor weight, Tensor hc, Tensor meta, Tensor stat, Tensor unit, int P, int D, bool has_bias, int reduction, bool want_h, bool want_w, "
-        "bool want_b, bool dh_fp32, bool dw_fp32) -> (Tensor, Tensor, Tensor)");
+  m.def("full_softmax_fwd(Tensor h, Tensor weight, Tensor targets, Tensor? bias, int ignore_index, int reduction, int grad) -> (Tensor, Tensor)");
+  m.def("full_softmax_bwd(Tensor dloss, Tensor weight, Tensor state, int P, int D, bool has_bias, int reduction, bool has_unit, bool want_h, bool want_w, bool want_b, "
+        "bool dh_fp32, bool dw_fp32, bool db_fp32) -> (Tensor, Tensor, Tensor)");
   m.def("full_softmax_status() -> int");
 }
 

@@ -17,6 +17,7 @@
 #include <torch/library.h>
 
 #include "common.cuh"
+#include "transformer_ops.h"
 
 namespace trb {
 

@@ -163,38 +163,15 @@ def packed_attention(qkv: torch.Tensor, offsets: torch.Tensor, num_heads: int, m
 # --------------------------------------------------------------------------------------
 # norm and rotation of queries and keys
 # --------------------------------------------------------------------------------------
+ROTARY_MAX_HEAD_DIM = 256  # widest head of the kernel
+_ROTARY_TYPES = (torch.bfloat16, torch.float16, torch.float32)
+
+
 def rotary_inv_freq(rotary_dim: int, base: float = 10000.0, device: Optional[torch.device] = None) -> torch.Tensor:
     """The usual frequencies ``base ** (-2 j / rotary_dim)``, ``j < rotary_dim / 2``, in fp64."""
     if rotary_dim < 2 or rotary_dim % 2 or not base > 0:
         raise ValueError(f"rotary_inv_freq: a positive even dimension and a positive base, got {rotary_dim} and {base}")
     return base ** (torch.arange(rotary_dim // 2, dtype=torch.float64, device=device) * (-2.0 / rotary_dim))
-
-
-def _rows16(t: torch.Tensor) -> torch.Tensor:
-    """``t [T, C]`` with contiguous rows that start on 16-byte boundaries (``t`` itself where it has them)."""
-    if t.stride(1) == 1 and t.data_ptr() % 16 == 0 and (t.stride(0) * t.element_size()) % 16 == 0 and (t.shape[0] <= 1 or t.stride(0) >= t.shape[1]):
-        return t
-    return t.clone(memory_format=torch.contiguous_format)
-
-
-class _QKNormRotary(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, qkv, positions, inv_freq, q_weight, k_weight, cfg):
-        qkv = _rows16(qkv)
-        sections, heads, kv_heads, eps, norm, interleaved = cfg
-        ctx.save_for_backward(qkv, positions, inv_freq, q_weight, k_weight)
-        ctx.cfg = cfg
-        return torch.ops.trb200.qk_norm_rotary_fwd(qkv, positions, inv_freq, q_weight, k_weight, sections, heads, kv_heads, eps, norm, interleaved)
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dy):
-        qkv, positions, inv_freq, q_weight, k_weight = ctx.saved_tensors
-        sections, heads, kv_heads, eps, norm, interleaved = ctx.cfg
-        want_q, want_k = ctx.needs_input_grad[3], ctx.needs_input_grad[4]
-        dqkv, dw = torch.ops.trb200.qk_norm_rotary_bwd(_rows16(dy), qkv, positions, inv_freq, q_weight, k_weight, sections, heads, kv_heads, eps, norm, interleaved,
-                                                       want_q or want_k)
-        return dqkv if ctx.needs_input_grad[0] else None, None, None, dw[0] if want_q else None, dw[1] if want_k else None, None
 
 
 def _qk_norm_rotary_plain(qkv, positions, inv_freq, q_weight, k_weight, cfg):
@@ -233,6 +210,11 @@ def qk_norm_rotary(qkv: torch.Tensor, positions: torch.Tensor, inv_freq: torch.T
     Gradients reach ``qkv`` and the weights.  CUDA tensors in bf16, fp16 or fp32 with a head dimension that is a multiple of 8 up to 256
     run in one kernel; others in plain torch."""
     kv_heads = num_heads if num_kv_heads is None else num_kv_heads
+    sections = [inv_freq.shape[0] if inv_freq.dim() else 0] if sections is None else [int(n) for n in sections]
+    if qkv.is_cuda and qkv.dtype in _ROTARY_TYPES and qkv.dim() == 2 and num_heads + 2 * kv_heads > 0:
+        dim = qkv.shape[1] // (num_heads + 2 * kv_heads)
+        if dim % 8 == 0 and dim <= ROTARY_MAX_HEAD_DIM and _ext.use_cuda_kernel(qkv, "qk_norm_rotary"):  # arguments are checked there
+            return torch.ops.trb200.qk_norm_rotary(qkv, positions, inv_freq, q_weight, k_weight, sections, num_heads, kv_heads, eps, norm, interleaved)
     if num_heads < 1 or kv_heads < 1 or qkv.dim() != 2 or qkv.shape[1] == 0 or qkv.shape[1] % (num_heads + 2 * kv_heads):
         raise ValueError(f"qk_norm_rotary: qkv is [T, (heads + 2 kv_heads) * head_dim], got {tuple(qkv.shape)} for {num_heads} and {kv_heads} heads")
     T, dim = qkv.shape[0], qkv.shape[1] // (num_heads + 2 * kv_heads)
@@ -240,7 +222,6 @@ def qk_norm_rotary(qkv: torch.Tensor, positions: torch.Tensor, inv_freq: torch.T
         raise ValueError(f"qk_norm_rotary: qkv is a floating-point tensor, got {qkv.dtype}")
     if inv_freq.dim() != 1 or not inv_freq.is_floating_point() or not 1 <= inv_freq.shape[0] <= dim // 2:
         raise ValueError(f"qk_norm_rotary: inv_freq holds 1 to head_dim / 2 = {dim // 2} frequencies, got {inv_freq.dtype} {tuple(inv_freq.shape)}")
-    sections = [inv_freq.shape[0]] if sections is None else [int(n) for n in sections]
     if positions.dtype not in (torch.int64, torch.int32) or tuple(positions.shape) not in ({(T,), (1, T)} if len(sections) == 1 else {(len(sections), T)}):
         raise ValueError(f"qk_norm_rotary: positions is an int32 or int64 [T] or [axes, T], got {positions.dtype} {tuple(positions.shape)} for {T} tokens and "
                          f"{len(sections)} axes")
@@ -254,13 +235,8 @@ def qk_norm_rotary(qkv: torch.Tensor, positions: torch.Tensor, inv_freq: torch.T
             raise ValueError(f"qk_norm_rotary: {name} is on {t.device}, qkv on {qkv.device}")
     if eps < 0:
         raise ValueError(f"qk_norm_rotary: eps is not negative, got {eps}")
-    positions = positions.reshape(len(sections), T)
-    inv_freq = inv_freq.detach().to(torch.float64).contiguous()
-    cfg = (sections, int(num_heads), int(kv_heads), float(eps), bool(norm), bool(interleaved))
-    if _ext.use_cuda_kernel(qkv, "qk_norm_rotary") and qkv.dtype in (torch.bfloat16, torch.float16, torch.float32) and dim % 8 == 0 and dim <= 256 and max(num_heads, kv_heads) <= 4096:
-        q_weight, k_weight = (w if w is None else w.float().contiguous() for w in (q_weight, k_weight))
-        return _QKNormRotary.apply(qkv, positions, inv_freq, q_weight, k_weight, cfg)
-    return _qk_norm_rotary_plain(qkv, positions, inv_freq, q_weight, k_weight, cfg)
+    return _qk_norm_rotary_plain(qkv, positions.reshape(len(sections), T), inv_freq.detach().to(torch.float64), q_weight, k_weight,
+                                 (sections, int(num_heads), int(kv_heads), float(eps), bool(norm), bool(interleaved)))
 
 
 # --------------------------------------------------------------------------------------
@@ -321,6 +297,7 @@ def sampled_softmax_loss(h: torch.Tensor, positive: torch.Tensor, negatives: tor
 # --------------------------------------------------------------------------------------
 FULL_SOFTMAX_MAX_DIM = 1024  # widest row of the tensor-core kernel
 _REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
+_KERNEL_TYPES = (torch.bfloat16, torch.float32)
 
 
 def full_softmax_error(device: torch.device) -> int:
@@ -331,51 +308,6 @@ def full_softmax_error(device: torch.device) -> int:
         return 0
     with torch.cuda.device(device):
         return int(torch.ops.trb200.full_softmax_status())
-
-
-def _weight_rows(weight: torch.Tensor) -> torch.Tensor:
-    """The weight as the kernel reads it: bf16 rows on 16-byte boundaries, zero columns up to a multiple of 8.  fp32 parameters go
-    through the cache that the dense layers use, so they are rounded once per optimizer step."""
-    from torchrec_b200.ops import dense_ops
-
-    if weight.dtype == torch.bfloat16:
-        w = weight.detach()
-    elif isinstance(weight, torch.nn.Parameter):
-        w = dense_ops.bf16_cache.get(weight)
-    else:
-        w = weight.detach().to(torch.bfloat16)
-    if w.shape[1] % 8:
-        return torch.nn.functional.pad(w, (0, -w.shape[1] % 8))
-    if w.stride(1) != 1 or w.stride(0) % 8 or w.stride(0) < w.shape[1] or w.data_ptr() % 16:
-        w = w.clone(memory_format=torch.contiguous_format)
-    return w
-
-
-class _FullSoftmaxLoss(torch.autograd.Function):
-    """The tensor-core path.  With a gradient of ``h`` wanted the forward already leaves it, up to the upstream factor, in fp32."""
-
-    @staticmethod
-    def forward(ctx, h, weight, bias, targets, ignore_index: int, reduction: int, grad: int):
-        w16 = _weight_rows(weight)
-        loss, hc, meta, stat, unit = torch.ops.trb200.full_softmax_fwd(h, w16, targets, bias, ignore_index, reduction, grad)
-        if grad:
-            # the caller's weight is saved too where the kernel read a copy, so that a change in place is noticed
-            ctx.save_for_backward(hc, meta, stat, unit, weight, *(() if w16.data_ptr() == weight.data_ptr() else (w16,)))
-            ctx.cfg = (tuple(h.shape), h.dtype, bias is not None, reduction)
-        return loss
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, g):
-        hc, meta, stat, unit, weight, *copy = ctx.saved_tensors
-        (P, D), h_dtype, has_bias, reduction = ctx.cfg
-        w16 = copy[0] if copy else weight
-        want_h, want_w, want_b = ctx.needs_input_grad[:3]
-        dh, dw, db = torch.ops.trb200.full_softmax_bwd(g, w16, hc, meta, stat, unit, P, D, has_bias, reduction, want_h, want_w, want_b and has_bias,
-                                                       h_dtype == torch.float32, weight.dtype == torch.float32)
-        if want_w and dw.shape[1] != D:
-            dw = dw[:, :D].contiguous()
-        return dh if want_h else None, dw if want_w else None, db if want_b and has_bias else None, None, None, None, None
 
 
 class _FullSoftmaxPieces(torch.autograd.Function):
@@ -451,28 +383,25 @@ def full_softmax_loss(h: torch.Tensor, weight: torch.Tensor, targets: torch.Tens
     on the tensor cores with bf16 operands and fp32 sums; an fp32 ``weight`` is rounded to bf16 for the products and gets an fp32
     gradient.  Everything else is computed in fp32 (fp64 for fp64 ``h``), a piece of the rows at a time.  A target outside ``[0, V)``
     raises on the CPU; on CUDA it makes the row's loss NaN and its gradient zero, and ``full_softmax_error`` reports it."""
+    if reduction not in _REDUCTIONS:
+        raise ValueError(f"full_softmax_loss: reduction is one of {sorted(_REDUCTIONS)}, got {reduction!r}")
+    if h.is_cuda and h.dim() == 2 and h.shape[1] <= FULL_SOFTMAX_MAX_DIM and weight.dtype in _KERNEL_TYPES and (bias is None or bias.dtype in _KERNEL_TYPES):
+        from torchrec_b200.ops import dense_ops
+
+        if (h.dtype == torch.bfloat16 or (h.dtype == torch.float32 and dense_ops.fused_dense_enabled(h))) and _ext.use_cuda_kernel(h, "full_softmax_loss"):
+            # fp32 parameters go through the cache that the dense layers use: rounded once per optimizer step
+            rounded = dense_ops.bf16_cache.get(weight) if weight.dtype == torch.float32 and weight.is_cuda and isinstance(weight, torch.nn.Parameter) else None
+            return torch.ops.trb200.full_softmax_loss(h, weight, bias, targets, rounded, ignore_index, _REDUCTIONS[reduction])  # arguments are checked there
     if h.dim() != 2 or weight.dim() != 2 or h.shape[1] != weight.shape[1] or weight.shape[0] == 0 or h.shape[1] == 0:
         raise ValueError(f"full_softmax_loss: h [P, D] and weight [V, D] with V, D > 0, got {tuple(h.shape)} and {tuple(weight.shape)}")
     if targets.shape != h.shape[:1] or targets.dtype not in (torch.int64, torch.int32):
         raise ValueError(f"full_softmax_loss: targets is an int32 or int64 [P], got {targets.dtype} {tuple(targets.shape)}")
     if bias is not None and bias.shape != weight.shape[:1]:
         raise ValueError(f"full_softmax_loss: bias is [V], got {tuple(bias.shape)} for {weight.shape[0]} classes")
-    if reduction not in _REDUCTIONS:
-        raise ValueError(f"full_softmax_loss: reduction is one of {sorted(_REDUCTIONS)}, got {reduction!r}")
     for name, t in (("h", h), ("weight", weight), ("bias", bias)):
         if t is not None and not t.is_floating_point():
             raise ValueError(f"full_softmax_loss: {name} is a floating-point tensor, got {t.dtype}")
     for name, t in (("weight", weight), ("targets", targets), ("bias", bias)):
         if t is not None and t.device != h.device:
             raise ValueError(f"full_softmax_loss: {name} is on {t.device}, h on {h.device}")
-    from torchrec_b200.ops import dense_ops
-
-    targets = targets.to(torch.int64)
-    if _ext.use_cuda_kernel(h, "full_softmax_loss") and h.shape[1] <= FULL_SOFTMAX_MAX_DIM and weight.dtype in (torch.bfloat16, torch.float32) and (
-            h.dtype == torch.bfloat16 or (h.dtype == torch.float32 and dense_ops.fused_dense_enabled(h))):
-        bias = None if bias is None else bias.float().contiguous()
-        grad = 0
-        if torch.is_grad_enabled():
-            grad = 2 if h.requires_grad else int(weight.requires_grad or (bias is not None and bias.requires_grad))
-        return _FullSoftmaxLoss.apply(h, weight, bias, targets, int(ignore_index), _REDUCTIONS[reduction], grad)
-    return _FullSoftmaxPieces.apply(h, weight, bias, targets, int(ignore_index), _REDUCTIONS[reduction])
+    return _FullSoftmaxPieces.apply(h, weight, bias, targets.to(torch.int64), int(ignore_index), _REDUCTIONS[reduction])

@@ -5,16 +5,20 @@
 // The library route is a dozen passes over fp32 copies of the tokens; both directions here are bound by memory: every value is read
 // once and written once.
 //
-// A warp takes a token (or, when tokens are few, some heads of one).  First its lanes compute one angle each - once per token, shared by
-// all heads - then groups of lanes take a head each, eight values per lane.  Angles are formed and reduced to a turn in 64 bits, so that
-// far positions (seconds, not only places in a sequence) keep full accuracy; sine and cosine of the remainder are fp32.  A rotation and
-// its scale are two factors per value (A x + B x_partner), so that a head costs little more than its loads; the partner values come
-// from L1.  Statistics and sums are fp32, one rounding at the end.
-// dw is summed in registers over a warp's tokens, then over the block and by a second kernel over the blocks, in a fixed order.
+// A group of lanes takes a token (eight values of a head per lane) and walks its heads; when tokens are few their heads are dealt to several
+// warps.  The angles are computed once per token, each by one lane, in 64 bits and reduced to a turn there, so that far positions (seconds,
+// not only places in a sequence) keep full accuracy.  What is the same for all heads - factors, weights - stays in registers, so that a
+// head costs its loads, one sum over the group and two products per value; the partner's values come from the neighbouring lanes.  (With a
+// warp per token and the factors fetched anew for every head, the kernel issued 600 to 900 instructions per token of 12 heads and was
+// bound by that.)  Statistics and sums are fp32, one rounding at the end.
+// dw is summed per token in registers, over a thread's tokens in shared memory, then over the block and by a second kernel over the
+// blocks, in a fixed order.
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/library.h>
+
+#include <type_traits>
 
 #include "common.cuh"
 #include "transformer_ops.h"
@@ -44,40 +48,61 @@ struct RotaryParams {
   int norm;
   int64_t T;
   int Hq, Hk, Dh;
-  int split;    // warps per token
+  int split;    // warps that share a token's heads
   int lp_log2;  // lanes of a head: power of two >= Dh / 8
   float* dw_part;  // backward: [blocks, 2, Dh]
 };
 
+// eight values as they lie in memory, loaded ahead of their use
 template <typename T>
-__device__ __forceinline__ void rot_load8(const T* p, float (&v)[8]);
-template <>
-__device__ __forceinline__ void rot_load8<float>(const float* p, float (&v)[8]) {
-  const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
-  v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-  v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-}
-template <>
-__device__ __forceinline__ void rot_load8<__nv_bfloat16>(const __nv_bfloat16* p, float (&v)[8]) {
-  const uint4 r = __ldg(reinterpret_cast<const uint4*>(p));
-  const uint32_t u[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    v[2 * k] = __uint_as_float(u[k] << 16);
-    v[2 * k + 1] = __uint_as_float(u[k] & 0xffff0000u);
+struct RotRaw {
+  uint4 u;
+  __device__ __forceinline__ void load(const T* p) { u = __ldg(reinterpret_cast<const uint4*>(p)); }
+  __device__ __forceinline__ void zero() { u = make_uint4(0, 0, 0, 0); }
+  __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<uint4*>(p) = u; }
+  __device__ __forceinline__ RotRaw from_lane(int lane) const {
+    RotRaw r;
+    r.u = make_uint4(__shfl_sync(0xffffffffu, u.x, lane), __shfl_sync(0xffffffffu, u.y, lane), __shfl_sync(0xffffffffu, u.z, lane), __shfl_sync(0xffffffffu, u.w, lane));
+    return r;
   }
-}
-template <>
-__device__ __forceinline__ void rot_load8<__half>(const __half* p, float (&v)[8]) {
-  const uint4 r = __ldg(reinterpret_cast<const uint4*>(p));
-  const uint32_t u[4] = {r.x, r.y, r.z, r.w};
+  __device__ __forceinline__ void unpack(float (&v)[8]) const {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u[k]));
-    v[2 * k] = f.x;
-    v[2 * k + 1] = f.y;
+    for (int k = 0; k < 4; ++k) {
+      if constexpr (std::is_same<T, __half>::value) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[k]));
+        v[2 * k] = f.x;
+        v[2 * k + 1] = f.y;
+      } else {
+        v[2 * k] = __uint_as_float(w[k] << 16);
+        v[2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
+      }
+    }
   }
-}
+};
+template <>
+struct RotRaw<float> {
+  float4 a, b;
+  __device__ __forceinline__ void load(const float* p) {
+    a = __ldg(reinterpret_cast<const float4*>(p));
+    b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+  }
+  __device__ __forceinline__ void zero() { a = b = f4zero(); }
+  __device__ __forceinline__ void store(float* p) const {
+    reinterpret_cast<float4*>(p)[0] = a;
+    reinterpret_cast<float4*>(p)[1] = b;
+  }
+  __device__ __forceinline__ RotRaw from_lane(int lane) const {
+    RotRaw r;
+    r.a = make_float4(__shfl_sync(0xffffffffu, a.x, lane), __shfl_sync(0xffffffffu, a.y, lane), __shfl_sync(0xffffffffu, a.z, lane), __shfl_sync(0xffffffffu, a.w, lane));
+    r.b = make_float4(__shfl_sync(0xffffffffu, b.x, lane), __shfl_sync(0xffffffffu, b.y, lane), __shfl_sync(0xffffffffu, b.z, lane), __shfl_sync(0xffffffffu, b.w, lane));
+    return r;
+  }
+  __device__ __forceinline__ void unpack(float (&v)[8]) const {
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+  }
+};
 
 __device__ __forceinline__ float rot_load1(const float* p) { return __ldg(p); }
 __device__ __forceinline__ float rot_load1(const __nv_bfloat16* p) { return __bfloat162float(*p); }
@@ -106,53 +131,86 @@ __device__ __forceinline__ void rot_store8(__half* p, const float (&v)[8]) {
 // consecutive values of another lane when that half is a multiple of eight, and single values otherwise.
 enum RotPairs : int { ROT_NEIGHBOURS = 0, ROT_HALVES = 1, ROT_HALVES_ODD = 2 };
 
+__device__ __forceinline__ void rot_smem8(const float* p, float (&v)[8]) {
+  const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+  v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+  v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+}
+
 // c[k], s[k]: factors of the lane's values d0..d0+7 and of their partners (sign of the forward turn included)
 template <int PAIRS>
 __device__ __forceinline__ void rot_factors(const float2* cs, int d0, int n_freq, float (&c)[8], float (&s)[8]) {
   const int R = 2 * n_freq;
+  if constexpr (PAIRS == ROT_HALVES) {
+    // eight consecutive angles, or none
+    if (d0 < R) {
+      const float4* f = reinterpret_cast<const float4*>(cs + (d0 < n_freq ? d0 : d0 - n_freq));
+      const float sign = d0 < n_freq ? -1.f : 1.f;
 #pragma unroll
-  for (int k = 0; k < 8; ++k) {
-    const int d = d0 + k;
-    const bool in = d < R;
-    int j;
-    bool first;
-    if constexpr (PAIRS == ROT_NEIGHBOURS) {
-      j = d >> 1;
-      first = (k & 1) == 0;
+      for (int k = 0; k < 4; ++k) {
+        const float4 v = f[k];
+        c[2 * k] = v.x;
+        s[2 * k] = sign * v.y;
+        c[2 * k + 1] = v.z;
+        s[2 * k + 1] = sign * v.w;
+      }
     } else {
-      first = d < n_freq;
-      j = first ? d : d - n_freq;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        c[k] = 1.f;
+        s[k] = 0.f;
+      }
     }
-    const float2 f = in ? cs[j] : make_float2(1.f, 0.f);
-    c[k] = f.x;
-    s[k] = first ? -f.y : f.y;
+  } else if constexpr (PAIRS == ROT_NEIGHBOURS) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float2 f = d0 + 2 * k < R ? cs[d0 / 2 + k] : make_float2(1.f, 0.f);
+      c[2 * k] = c[2 * k + 1] = f.x;
+      s[2 * k] = -f.y;
+      s[2 * k + 1] = f.y;
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int d = d0 + k;
+      const float2 f = d < R ? cs[d < n_freq ? d : d - n_freq] : make_float2(1.f, 0.f);
+      c[k] = f.x;
+      s[k] = d < n_freq ? -f.y : f.y;
+    }
   }
 }
 
 template <typename T, int PAIRS>
-__device__ __forceinline__ void rot_partner(const T* head, int d0, int n_freq, const float (&x)[8], float (&xp)[8]) {
+__device__ __forceinline__ void rot_partner(const T* head, bool act, int d0, int partner_lane, int n_freq, const RotRaw<T>& raw, const float (&x)[8], float (&xp)[8]) {
   if constexpr (PAIRS == ROT_NEIGHBOURS) {
 #pragma unroll
     for (int k = 0; k < 8; ++k) xp[k] = x[k ^ 1];
   } else if constexpr (PAIRS == ROT_HALVES) {
-    const int p = d0 < n_freq ? d0 + n_freq : (d0 < 2 * n_freq ? d0 - n_freq : d0);
-    rot_load8(head + p, xp);
+    raw.from_lane(partner_lane).unpack(xp);
   } else {
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       const int d = d0 + k, p = d < n_freq ? d + n_freq : (d < 2 * n_freq ? d - n_freq : d);
-      xp[k] = rot_load1(head + p);
+      xp[k] = act ? rot_load1(head + p) : 0.f;
     }
   }
 }
 
+// weights of the lane's values and of their partners (p0: where the partners start when they are consecutive)
 template <int PAIRS>
-__device__ __forceinline__ void rot_partner_weight(const float* w, int d0, int n_freq, float (&wp)[8]) {
+__device__ __forceinline__ void rot_weights(const float* w, int d0, int p0, int n_freq, float (&own)[8], float (&partner)[8]) {
+  rot_smem8(w + d0, own);
+  if constexpr (PAIRS == ROT_NEIGHBOURS) {
 #pragma unroll
-  for (int k = 0; k < 8; ++k) {
-    const int d = d0 + k;
-    const int p = PAIRS == ROT_NEIGHBOURS ? d ^ 1 : (d < n_freq ? d + n_freq : (d < 2 * n_freq ? d - n_freq : d));
-    wp[k] = w[p];
+    for (int k = 0; k < 8; ++k) partner[k] = own[k ^ 1];
+  } else if constexpr (PAIRS == ROT_HALVES) {
+    rot_smem8(w + p0, partner);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int d = d0 + k;
+      partner[k] = w[d < n_freq ? d + n_freq : (d < 2 * n_freq ? d - n_freq : d)];
+    }
   }
 }
 
@@ -162,148 +220,187 @@ __device__ __forceinline__ float rot_group_sum(float v, int lp_log2) {
   return v;
 }
 
+// sine and cosine of `turn` turns, |turn| <= 1/2: to 2^-23 for fp32 outputs; for 16-bit ones the hardware functions, 2^-20 off, which is
+// far below half a step of the output
+template <typename T>
+__device__ __forceinline__ float2 rot_cos_sin(float turn) {
+  float s, c;
+  if constexpr (sizeof(T) == 4) sincospif(2.f * turn, &s, &c);
+  else __sincosf(6.283185307179586f * turn, &s, &c);
+  return make_float2(c, s);
+}
+
+// Registers are bounded so that 32 (forward) or 24 (backward) warps share an SM.
 template <typename T, int PAIRS, bool BWD>
-__global__ void __launch_bounds__(kRotThreads) qk_norm_rotary_kernel(const RotaryParams p) {
-  __shared__ __align__(16) float2 cs_all[kRotWarps][kRotMaxDim / 2];
+__global__ void __launch_bounds__(kRotThreads, BWD ? 3 : 4) qk_norm_rotary_kernel(const RotaryParams p) {
+  constexpr int kBatch = sizeof(T) == 4 ? (BWD ? 1 : 2) : (BWD ? 2 : 4);  // heads whose loads are in flight together
+  __shared__ __align__(16) float2 cs_all[kRotWarps][kRotMaxDim / 2];  // a warp's tokens x frequencies (their product is at most 128)
   __shared__ __align__(16) float w_s[2][kRotMaxDim];
+  __shared__ double freq_s[kRotMaxDim / 2];   // in turns
+  __shared__ int64_t axis_s[kRotMaxDim / 2];  // offset of the axis' positions
+  __shared__ __align__(16) float dw_s[BWD ? 2 * kRotThreads * 8 : 4];  // [q, k][thread][8]
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  float2* cs = cs_all[warp];
   for (int d = threadIdx.x; d < p.Dh; d += kRotThreads) {
     w_s[0][d] = p.qw ? p.qw[d] : 1.f;
     w_s[1][d] = p.kw ? p.kw[d] : 1.f;
   }
-  // this lane's frequencies in turns, and the axis whose position each takes
-  double freq[4];
-  int axis[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int j = lane + 32 * i;
-    freq[i] = j < p.n_freq ? p.inv_freq[j] * 0.15915494309189533577 : 0.0;
+  for (int j = threadIdx.x; j < p.n_freq; j += kRotThreads) {
+    freq_s[j] = p.inv_freq[j] * 0.15915494309189533577;
     int a = 0;
     while (a < p.axes - 1 && j >= p.axis_end[a]) ++a;
-    axis[i] = a;
+    axis_s[j] = a * p.pos_axis;
   }
-  __syncthreads();
-  const int lp = 1 << p.lp_log2, group = lane >> p.lp_log2, li = lane & (lp - 1), d0 = li * 8;
-  const bool in_head = d0 < p.Dh;
-  const int per_pass = 32 >> p.lp_log2, heads = p.Hq + 2 * p.Hk, turned = p.Hq + p.Hk, passes = (heads + per_pass - 1) / per_pass;
-  const float inv_dim = 1.f / float(p.Dh);
-  float dwq[8], dwk[8];
   if constexpr (BWD) {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) dwq[k] = dwk[k] = 0.f;
+    for (int k = 0; k < 16; ++k) dw_s[k * kRotThreads + threadIdx.x] = 0.f;
   }
-  const int64_t items = p.T * p.split, step = int64_t(gridDim.x) * kRotWarps;
+  __syncthreads();
+  const int lp = 1 << p.lp_log2, group = lane >> p.lp_log2, li = lane & (lp - 1), tokens = 32 >> p.lp_log2;
+  const bool in_head = li * 8 < p.Dh;
+  const int d0 = in_head ? li * 8 : 0;  // lanes behind the head's last follow the first and store nothing
+  const int p0 = d0 >= 2 * p.n_freq ? d0 : (d0 < p.n_freq ? d0 + p.n_freq : d0 - p.n_freq);
+  const int partner_lane = in_head ? lane + (p0 - d0) / 8 : lane;
+  const int turned = p.Hq + p.Hk, heads = turned + p.Hk;
+  const int stride = p.split * p.Dh;
+  float2* cs = cs_all[warp] + group * p.n_freq;
+  const float inv_dim = 1.f / float(p.Dh);
+  const int64_t blocks_of_tokens = (p.T + tokens - 1) / tokens, items = blocks_of_tokens * p.split, step = int64_t(gridDim.x) * kRotWarps;
   for (int64_t item = int64_t(blockIdx.x) * kRotWarps + warp; item < items; item += step) {
-    const int64_t token = p.split == 1 ? item : item / p.split;
-    const int part = p.split == 1 ? 0 : int(item - token * p.split);
-    __syncwarp();  // the previous token's angles have been read
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int j = lane + 32 * i;
-      if (j < p.n_freq) {
-        const int64_t at = axis[i] * p.pos_axis + token * p.pos_token;
-        const double pos = p.pos64 ? double(reinterpret_cast<const int64_t*>(p.positions)[at]) : double(reinterpret_cast<const int*>(p.positions)[at]);
-        double turn = pos * freq[i];
-        turn -= rint(turn);
-        float s, c;
-        sincospif(2.f * float(turn), &s, &c);
-        cs[j] = make_float2(c, s);
-      }
+    int64_t first = item;
+    int part = 0;
+    if (p.split > 1) {
+      first = item / p.split;
+      part = int(item - first * p.split);
     }
+    const int64_t token = first * tokens + group;
+    const bool live = token < p.T, act = live && in_head;
+    const T* row = reinterpret_cast<const T*>(p.qkv) + token * p.ld + part * p.Dh;
+    T* out = reinterpret_cast<T*>(p.out) + (token * heads + part) * p.Dh + d0;
+    const T* drow = BWD ? reinterpret_cast<const T*>(p.dy) + token * p.ld_dy + part * p.Dh : nullptr;
+    RotRaw<T> rx[kBatch], rg[BWD ? kBatch : 1];
+    auto load = [&](int head) {  // the heads head, head + split, ...; `row` and `drow` are at the first of them
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        const int h = head + i * p.split;
+        if constexpr (BWD) {
+          rx[i].zero();
+          rg[i].zero();
+          if (act && h < turned) rx[i].load(row + i * stride + d0);
+          if (act && h < heads) rg[i].load(drow + i * stride + d0);
+        } else {
+          rx[i].zero();
+          if (act && h < heads) rx[i].load(row + i * stride + d0);
+        }
+      }
+    };
+    load(part);  // on its way while the angles are computed
+    __syncwarp();  // the previous tokens' angles have been read
+    if (live)
+      for (int j = li; j < p.n_freq; j += lp) {
+        const int64_t at = axis_s[j] + token * p.pos_token;
+        double turn = (p.pos64 ? double(reinterpret_cast<const int64_t*>(p.positions)[at]) : double(reinterpret_cast<const int*>(p.positions)[at])) * freq_s[j];
+        turn -= rint(turn);
+        cs[j] = rot_cos_sin<T>(float(turn));
+      }
     __syncwarp();
-    const T* row = reinterpret_cast<const T*>(p.qkv) + token * p.ld;
-    T* out = reinterpret_cast<T*>(p.out) + token * heads * p.Dh;
-    const T* drow = BWD ? reinterpret_cast<const T*>(p.dy) + token * p.ld_dy : nullptr;
-    float c[8], s[8];
-    rot_factors<PAIRS>(cs, in_head ? d0 : 0, p.n_freq, c, s);
-    for (int pass = part; pass < passes; pass += p.split) {
-      const int head = pass * per_pass + group;
-      const bool here = in_head && head < heads;
-      const int off = head * p.Dh;
-      if (here && head >= turned) {  // v
-        float v[8];
-        rot_load8((BWD ? drow : row) + off + d0, v);
-        rot_store8(out + off + d0, v);
-      }
-      const bool act = here && head < turned;
-      if (!__any_sync(0xffffffffu, act)) continue;
-      const float* w = w_s[head < p.Hq ? 0 : 1];
-      float x[8];
-      if (act) {
-        rot_load8(row + off + d0, x);
-      } else {
+    float c[8], s[8], w[8], wp[8], acc[8];
+    int type = -1;  // whose weights (and, forward, factors times weights) are in the registers: 0 q, 1 k
+    rot_factors<PAIRS>(cs, d0, p.n_freq, c, s);
+    auto flush = [&]() {  // dw of the heads of one type
+      float* d = dw_s + (type * kRotThreads + threadIdx.x) * 8;
+      float v[8];
+      rot_smem8(d, v);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) x[k] = 0.f;
-      }
-      if constexpr (!BWD) {
-        float xp[8], wp[8];
-        if (act) rot_partner<T, PAIRS>(row + off, d0, p.n_freq, x, xp);
-        float sq = 0.f;
+      for (int k = 0; k < 8; ++k) v[k] += acc[k];
+      reinterpret_cast<float4*>(d)[0] = make_float4(v[0], v[1], v[2], v[3]);
+      reinterpret_cast<float4*>(d)[1] = make_float4(v[4], v[5], v[6], v[7]);
+    };
+#pragma unroll 1
+    for (int head = part; head < heads; head += kBatch * p.split) {  // the same for all lanes
 #pragma unroll
-        for (int k = 0; k < 8; ++k) sq += x[k] * x[k];
-        sq = rot_group_sum(sq, p.lp_log2);
-        if (act) {
-          const float rstd = p.norm ? 1.f / sqrtf(sq * inv_dim + p.eps) : 1.f;
-          rot_partner_weight<PAIRS>(w, d0, p.n_freq, wp);
-          float y[8];
-#pragma unroll
-          for (int k = 0; k < 8; ++k) y[k] = rstd * (c[k] * w[d0 + k] * x[k] + s[k] * wp[k] * xp[k]);
-          rot_store8(out + off + d0, y);
+      for (int i = 0; i < kBatch; ++i) {
+        const int h = head + i * p.split;
+        if (h >= heads) break;
+        T* o = out + i * stride;
+        if (h >= turned) {
+          if (act) (BWD ? rg[BWD ? i : 0] : rx[i]).store(o);
+          continue;
         }
-      } else {
-        float g[8], gp[8];
-        float sq = 0.f, dot = 0.f;
-        if (act) {
-          rot_load8(drow + off + d0, g);
-          rot_partner<T, PAIRS>(drow + off, d0, p.n_freq, g, gp);
+        const int now = h < p.Hq ? 0 : 1;
+        if (now != type) {
+          if constexpr (BWD) {
+            if (p.dw_part != nullptr && type >= 0) flush();
 #pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            g[k] = c[k] * g[k] - s[k] * gp[k];
-            sq += x[k] * x[k];
-            dot += w[d0 + k] * g[k] * x[k];
-          }
-        }
-        sq = rot_group_sum(sq, p.lp_log2);
-        dot = rot_group_sum(dot, p.lp_log2);
-        if (act) {
-          const float rstd = p.norm ? 1.f / sqrtf(sq * inv_dim + p.eps) : 1.f;
-          const float back = p.norm ? rstd * rstd * dot * inv_dim : 0.f;
-          float dx[8];
-#pragma unroll
-          for (int k = 0; k < 8; ++k) dx[k] = rstd * (w[d0 + k] * g[k] - x[k] * back);
-          rot_store8(out + off + d0, dx);
-          if (p.dw_part != nullptr) {
-            const bool q = head < p.Hq;
+            for (int k = 0; k < 8; ++k) acc[k] = 0.f;
+            rot_smem8(w_s[now] + d0, w);
+          } else {
+            rot_factors<PAIRS>(cs, d0, p.n_freq, c, s);
+            rot_weights<PAIRS>(w_s[now], d0, p0, p.n_freq, w, wp);
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
-              const float v = g[k] * x[k] * rstd;
-              dwq[k] += q ? v : 0.f;
-              dwk[k] += q ? 0.f : v;
+              c[k] *= w[k];
+              s[k] *= wp[k];
             }
+          }
+          type = now;
+        }
+        float x[8];
+        rx[i].unpack(x);
+        if constexpr (!BWD) {
+          float xp[8];
+          rot_partner<T, PAIRS>(row + i * stride, act, d0, partner_lane, p.n_freq, rx[i], x, xp);
+          float sq = 0.f;
+#pragma unroll
+          for (int k = 0; k < 8; ++k) sq += x[k] * x[k];
+          sq = rot_group_sum(sq, p.lp_log2);  // lanes without a part of the head hold zeros
+          const float rstd = p.norm ? rsqrtf(sq * inv_dim + p.eps) : 1.f;
+#pragma unroll
+          for (int k = 0; k < 8; ++k) x[k] = rstd * (c[k] * x[k] + s[k] * xp[k]);
+          if (act) rot_store8(o, x);
+        } else {
+          float g[8], gp[8];
+          rg[i].unpack(g);
+          rot_partner<T, PAIRS>(drow + i * stride, act, d0, partner_lane, p.n_freq, rg[i], g, gp);
+          float sq = 0.f, dot = 0.f;
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            g[k] = (c[k] * g[k] - s[k] * gp[k]);
+            sq += x[k] * x[k];
+            gp[k] = g[k] * x[k];
+            dot += w[k] * gp[k];
+          }
+          sq = rot_group_sum(sq, p.lp_log2);
+          dot = rot_group_sum(dot, p.lp_log2);
+          const float rstd = p.norm ? rsqrtf(sq * inv_dim + p.eps) : 1.f;
+          const float back = p.norm ? rstd * rstd * dot * inv_dim : 0.f;
+          if (act) {  // (elsewhere rstd may be infinite)
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              acc[k] += gp[k] * rstd;
+              x[k] = rstd * (w[k] * g[k] - x[k] * back);
+            }
+            rot_store8(o, x);
           }
         }
       }
+      row += kBatch * stride;
+      out += kBatch * stride;
+      if constexpr (BWD) drow += kBatch * stride;
+      if (head + kBatch * p.split < heads) load(head + kBatch * p.split);
+    }
+    if constexpr (BWD) {
+      if (p.dw_part != nullptr && type >= 0) flush();
     }
   }
   if constexpr (BWD) {
     if (p.dw_part == nullptr) return;
-    // over the groups of the warp, then over the warps of the block, in a fixed order
-    float* red = reinterpret_cast<float*>(cs_all);  // [warps][Dh]: the angles are done with
-    for (int which = 0; which < 2; ++which) {
-      __syncthreads();
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        float v = which ? dwk[k] : dwq[k];
-        for (int o = lp; o < 32; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-        if (group == 0 && in_head) red[warp * kRotMaxDim + d0 + k] = v;
-      }
-      __syncthreads();
-      for (int d = threadIdx.x; d < p.Dh; d += kRotThreads) {
-        float v = 0.f;
-        for (int q = 0; q < kRotWarps; ++q) v += red[q * kRotMaxDim + d];
-        p.dw_part[(int64_t(blockIdx.x) * 2 + which) * p.Dh + d] = v;
-      }
+    // over the block's threads that hold the same eight columns, in a fixed order
+    __syncthreads();
+    for (int d = threadIdx.x; d < 2 * p.Dh; d += kRotThreads) {
+      const int which = d >= p.Dh ? 1 : 0, col = d - which * p.Dh;
+      float v = 0.f;
+      for (int t = col / 8; t < kRotThreads; t += lp) v += dw_s[(which * kRotThreads + t) * 8 + (col & 7)];
+      p.dw_part[int64_t(blockIdx.x) * 2 * p.Dh + d] = v;
     }
   }
 }
@@ -395,12 +492,12 @@ static std::tuple<at::Tensor, at::Tensor> rot_run(const at::Tensor& qkv, const c
   p.Hk = int(Hk);
   p.Dh = int(Dh);
   while ((8 << p.lp_log2) < Dh) ++p.lp_log2;
-  // a warp per token, or, when the tokens would not give every SM 16 warps, its heads dealt to several
+  // a group of lanes per token, or, when the tokens would not give every SM 16 warps, its heads dealt to several warps
   const int sms = at::cuda::getDeviceProperties(qkv.device().index())->multiProcessorCount;
-  const int64_t per_pass = 32 >> p.lp_log2, passes = (Hq + 2 * Hk + per_pass - 1) / per_pass;
-  p.split = int(std::max<int64_t>(1, std::min<int64_t>(passes, 16LL * sms / T)));
-  const int64_t warps = T * p.split;
-  const int blocks = int(std::min<int64_t>((warps + kRotWarps - 1) / kRotWarps, (bwd ? 4 : 6) * sms));
+  const int64_t groups = (T + (32 >> p.lp_log2) - 1) / (32 >> p.lp_log2);
+  p.split = int(std::max<int64_t>(1, std::min<int64_t>(Hq + 2 * Hk, 16LL * sms / groups)));
+  const int64_t warps = groups * p.split;
+  const int blocks = int(std::min<int64_t>((warps + kRotWarps - 1) / kRotWarps, (bwd ? 3 : 4) * sms));
   at::Tensor part;
   if (want_dw) {
     part = at::empty({blocks, 2, Dh}, dw.options());

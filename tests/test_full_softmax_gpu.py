@@ -114,6 +114,20 @@ def test_many_pieces_of_either_axis():
     _check(*_inputs(5000, 300, 256, False, 0.5, seed=3))
 
 
+@pytest.mark.parametrize("D", [64, 128, 200, 256, 320, 640])
+def test_long_runs_of_tiles(D):
+    """More tiles of rows (classes) than the GPU has SMs: every block streams all classes (rows) past each of its tiles, through many uses
+    of its buffers, and takes a second tile.  The maxima rise on the way in some rows."""
+    g = torch.Generator().manual_seed(D)
+    P, V = 19300, 1500
+    level = (torch.arange(V) // 100).float() * 20
+    h, w, t, b = _inputs(P, V, D, True, 0.01, seed=D)
+    h[:, 0] = torch.where(torch.rand(P, generator=g) < 0.02, 1.0, 0.0).cuda().bfloat16()
+    w[:, 0] = level.cuda().bfloat16()
+    _check(h, w, t, b, "mean")
+    _check(h[:1500].contiguous(), torch.cat([w] * 13)[:19300].contiguous(), t[:1500], None, "none")
+
+
 def test_maximum_that_keeps_rising():
     """Scores that grow from tile to tile force the rescaling of the accumulator, in some rows more often than in others."""
     h, w, t, b = _inputs(200, 1500, 256, False, seed=5)

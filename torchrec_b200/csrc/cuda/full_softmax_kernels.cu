@@ -44,7 +44,7 @@ constexpr int kFsMaxD = 1024;
 constexpr int kFsAcc = 256;                         // accumulator columns
 constexpr int kFsExtra = 3072;                      // per-column values of a tile, exchange of maxima, barriers
 constexpr int kFsSmem = kFsSlots * kFsSlotBytes + kFsExtra;
-constexpr int kFsItemsPerSm = 4;                    // bounds the workspace of partial results
+constexpr int kFsItemsPerSm = 8;                    // bounds the workspace of partial results
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 // Base-2 growth of a row's maximum that forces a rescale.  The terms have bf16's and fp32's exponents: 2^40 over 2^31 columns is far
@@ -71,7 +71,7 @@ __host__ __device__ inline FsSchedule fs_schedule(int nx, int ny, int pieces, in
   s.per = s.ty;
   const int base = s.tx * pieces;
   if (base > 0 && s.ty > 1) {
-    // rounds of blocks x (tiles of an item + its start, end and share of the join).  Candidates fill 1..4 rounds.
+    // rounds of blocks x (tiles of an item + its start, end and share of the join).  Candidates fill 1..8 rounds.
     const int most = s.tx > 0 ? (kFsItemsPerSm * grid) / s.tx : 1;
     float best = float((base + grid - 1) / grid) * (s.ty + 2.f);
     for (int r = 1; r <= kFsItemsPerSm; ++r) {
@@ -144,8 +144,8 @@ struct FsBars {
   uint64_t full[kFsMaxUnits], empty[kFsMaxUnits];
   uint64_t x_full, x_empty;
   uint64_t s_full[4], p_full[4];
-  uint64_t acc_done[2], o_empty;  // acc_done by the tile's parity: a waiter may be one tile behind the last commit
-  uint64_t c_full[2], c_empty[2];
+  uint64_t acc_done[4], o_empty;  // acc_done by the tile's number: a waiter may know no more than that the product four tiles back is done
+  uint64_t c_full[4], c_empty[4];
   uint64_t m_done[4], drain;
   uint32_t tmem_base;
   int abort_flag;
@@ -177,10 +177,15 @@ __global__ void __launch_bounds__(kFsThreads, 1)
 full_softmax_kernel(const __grid_constant__ CUtensorMap tmapX, const __grid_constant__ CUtensorMap tmapY, const FsParams p) {
   constexpr bool kAcc = MODE != FS_LSE;
   constexpr uint32_t kTmemCols = 512;
-  constexpr int kBufs = kAcc ? 2 : 4;       // score tiles in TMEM; the accumulator takes the other half
-  constexpr int kBufShift = kAcc ? 1 : 2;
+  // Score tiles in TMEM: two beside an accumulator of up to 256 columns, three beside one of up to 128 (S then runs two tiles ahead, so
+  // that neither group of softmax warps waits for the products of the tile that it has just handed over: rows of 64 to 128 values are
+  // bound by the exponentials), four without an accumulator.
+  const uint32_t bufs = kAcc ? (p.D <= 128 ? 3 : 2) : 4;
+  const uint32_t o_col = bufs * kFsTile;
+  constexpr uint32_t kCols = ROWG ? 2 : 4, kColShift = ROWG ? 1 : 2;  // tiles whose per-column values are in shared memory
+  constexpr int kPair = kAcc ? 1 : 2;  // without an accumulator two tiles are one product of 256 columns, which reads X half as often
   extern __shared__ __align__(1024) uint8_t fs_smem[];
-  float* cols = reinterpret_cast<float*>(fs_smem + kFsSlots * kFsSlotBytes);  // FWD: the rows' maxima [128]; BWD: lse2 [2][128], g [2][128]
+  float* cols = reinterpret_cast<float*>(fs_smem + kFsSlots * kFsSlotBytes);  // FWD: the rows' maxima [128]; BWD: lse2 [4][128], or lse2 [2][128], g [2][128]
   FsBars* B = reinterpret_cast<FsBars*>(cols + 512);
   volatile int* abort_flag = &B->abort_flag;
   // values that are alike in a warp are taken from lane 0, which tells the compiler so
@@ -188,8 +193,9 @@ full_softmax_kernel(const __grid_constant__ CUtensorMap tmapX, const __grid_cons
   const int n_valid = __shfl_sync(0xffffffffu, *p.n_valid, 0);
   const int nx = MODE == FS_BWD ? p.V : n_valid, ny = MODE == FS_BWD ? n_valid : p.V;
   const FsSchedule sc = fs_schedule(nx, ny, kAcc ? (p.D + kFsAcc - 1) / kFsAcc : 1, p.grid);
-  const int spu = p.kb == 1 ? 1 : 2;                       // slots of a unit of the ring
-  const int upt = (p.kb + spu - 1) / spu;                  // units of a streamed tile
+  // a unit of the ring: two blocks of 64 columns of a tile (one for rows of up to 64), or one block of a pair of tiles
+  const int spu = kAcc && p.kb == 1 ? 1 : 2;               // its slots
+  const int upt = kAcc ? (p.kb + spu - 1) / spu : p.kb;    // units of a streamed tile or pair
   const int x_slots = p.x_resident ? p.kb : 0;
   const uint32_t units = min((kFsSlots - x_slots) / spu, kFsMaxUnits);
   uint8_t* ring = fs_smem + x_slots * kFsSlotBytes;
@@ -205,8 +211,6 @@ full_softmax_kernel(const __grid_constant__ CUtensorMap tmapX, const __grid_cons
       mbar_init(&B->s_full[i], 1);
       mbar_init(&B->p_full[i], 4);
       mbar_init(&B->m_done[i], 1);
-    }
-    for (int i = 0; i < 2; ++i) {
       mbar_init(&B->acc_done[i], 1);
       mbar_init(&B->c_full[i], 1);
       mbar_init(&B->c_empty[i], 4);
@@ -240,13 +244,13 @@ full_softmax_kernel(const __grid_constant__ CUtensorMap tmapX, const __grid_cons
     if (lane == 0) {
       FsRing r(units);
       uint32_t item = 0, tc = 0, loads = 0;
-      auto load_unit = [&](const CUtensorMap* map, int u, int row) {
+      auto load_unit = [&](const CUtensorMap* map, int u, int row, bool pair) {
         if (!fs_wait(&B->empty[r.stage], r.phase ^ 1, abort_flag, FS_ERR_EMPTY)) return false;
-        const int n = min(spu, p.kb - u * spu);
+        const int n = kAcc ? min(spu, p.kb - u * spu) : (pair ? 2 : 1), col = kAcc ? u * spu * 64 : u * 64;
         uint8_t* dst = ring + r.stage * spu * kFsSlotBytes;
         mbar_expect_tx(&B->full[r.stage], n * kFsSlotBytes);
-        tma_load_2d(dst, map, &B->full[r.stage], u * spu * 64, row);
-        if (n > 1) tma_load_2d(dst + kFsSlotBytes, map, &B->full[r.stage], u * spu * 64 + 64, row);
+        tma_load_2d(dst, map, &B->full[r.stage], col, row);
+        if (n > 1) tma_load_2d(dst + kFsSlotBytes, map, &B->full[r.stage], kAcc ? col + 64 : col, kAcc ? row : row + kFsTile);
         r.next();
         ++loads;
         return true;
@@ -260,23 +264,24 @@ full_softmax_kernel(const __grid_constant__ CUtensorMap tmapX, const __grid_cons
           for (int k = 0; k < p.kb; ++k) tma_load_2d(fs_smem + k * kFsSlotBytes, &tmapX, &B->x_full, k * 64, x * kFsTile);
         }
         const int pu0 = piece * (kFsAcc / 128), pu1 = min(upt, pu0 + kFsAcc / 128);
-        for (int t = 0; t <= nt && ok; ++t) {
-          if (t < nt) {
-            if constexpr (MODE == FS_BWD) {
-              const int b = tc & 1;
-              if (!fs_wait(&B->c_empty[b], ((tc >> 1) & 1) ^ 1, abort_flag, FS_ERR_COL)) { ok = false; break; }
+        const int groups = (nt + kPair - 1) / kPair, ahead = kAcc ? int(bufs) - 1 : 0;
+        for (int t = 0; t < groups + ahead && ok; ++t) {
+          if (t < groups) {
+            for (int u = 0; u < upt && ok; ++u) {
+              if (!p.x_resident) ok = load_unit(&tmapX, u, x * kFsTile, false);
+              ok = ok && load_unit(&tmapY, u, (t0 + t * kPair) * kFsTile, true);  // behind the last row zeros arrive
+            }
+            if constexpr (MODE == FS_BWD) {  // after the tile, whose product does not need them
+              const uint32_t b = tc & (kCols - 1);
+              if (!ok || !fs_wait(&B->c_empty[b], ((tc >> kColShift) & 1) ^ 1, abort_flag, FS_ERR_COL)) { ok = false; break; }
               mbar_expect_tx(&B->c_full[b], ROWG ? 1024 : 512);
               fs_bulk_load(cols + b * 128, p.lse2 + int64_t(t0 + t) * kFsTile, 512, &B->c_full[b]);
               if constexpr (ROWG) fs_bulk_load(cols + 256 + b * 128, p.gcol + int64_t(t0 + t) * kFsTile, 512, &B->c_full[b]);
               ++tc;
             }
-            for (int u = 0; u < upt && ok; ++u) {
-              if (!p.x_resident) ok = load_unit(&tmapX, u, x * kFsTile);
-              ok = ok && load_unit(&tmapY, u, (t0 + t) * kFsTile);
-            }
           }
-          if (kAcc && !p.hold && t > 0)
-            for (int u = pu0; u < pu1 && ok; ++u) ok = load_unit(&tmapY, u, (t0 + t - 1) * kFsTile);
+          if (kAcc && !p.hold && t >= ahead)
+            for (int u = pu0; u < pu1 && ok; ++u) ok = load_unit(&tmapY, u, (t0 + t - ahead) * kFsTile, true);
         }
       }
       if (!ok) {
@@ -289,22 +294,23 @@ full_softmax_kernel(const __grid_constant__ CUtensorMap tmapX, const __grid_cons
           while (!mbar_try_wait(&B->x_full, item & 1) && clock64() - begin < kWaitCycles) {
           }
         if constexpr (MODE == FS_BWD)
-          for (uint32_t j = tc > 2 ? tc - 2 : 0; j < tc; ++j)
-            while (!mbar_try_wait(&B->c_full[j & 1], (j >> 1) & 1) && clock64() - begin < kWaitCycles) {
+          for (uint32_t j = tc > kCols ? tc - kCols : 0; j < tc; ++j)
+            while (!mbar_try_wait(&B->c_full[j & (kCols - 1)], (j >> kColShift) & 1) && clock64() - begin < kWaitCycles) {
             }
       }
     }
   } else if (warp == 1) {
     // ---------------- MMA issuer ----------------
-    // S(t + 1) is issued before ACC(t), so the tensor cores work while the softmax warps turn S(t) into E(t).  Descriptors advance by
+    // S of the next one or two tiles is issued before ACC(t), so the tensor cores work while the softmax warps turn S(t) into E(t).  Descriptors advance by
     // additions (addresses in units of 16 bytes).  The whole warp runs the loop, one elected lane issues.
     {
       auto wait_all = [&](uint64_t* bar, uint32_t parity, int code) {
         return __all_sync(0xffffffffu, fs_wait(bar, parity, abort_flag, code)) != 0;
       };
       FsRing r(units);
-      uint32_t item = 0, tc = 0;  // tc: tile whose S is issued next
-      constexpr uint32_t idesc_s = fs_idesc(kFsTile, false);
+      uint32_t item = 0, tc = 0;  // tc: tile whose E is multiplied next
+      constexpr uint32_t idesc_s = fs_idesc(kPair * kFsTile, false);
+      uint32_t sb = 0, sb_use = 0, eb = 0, eb_phase = 0;  // buffer of the next S and how often it was used, buffer and phase of the next E
       constexpr uint32_t kSlot16 = kFsSlotBytes / 16;
       const uint64_t desc_k = make_smem_desc(0, 16, 1024), desc_mn = make_smem_desc(0, kFsSlotBytes, 1024);
       const uint32_t x16 = smem_u32(fs_smem) >> 4, ring16 = smem_u32(ring) >> 4, unit16 = spu * kSlot16;
@@ -313,18 +319,18 @@ full_softmax_kernel(const __grid_constant__ CUtensorMap tmapX, const __grid_cons
         const int t0 = split * sc.per, nt = min(sc.ty, t0 + sc.per) - t0;
         if (p.x_resident && nt > 0 && !wait_all(&B->x_full, item & 1, FS_ERR_X)) { ok = false; break; }
         const int pu0 = piece * (kFsAcc / 128), pu1 = min(upt, pu0 + kFsAcc / 128);
-        uint32_t held = 0, held_before = 0;  // first stages of the held tiles
-        for (int t = 0; t <= nt && ok; ++t) {
-          if (t < nt) {
-            const uint32_t b = tc & (kBufs - 1), use = tc >> kBufShift;
+        const int groups = (nt + kPair - 1) / kPair, ahead = kAcc ? int(bufs) - 1 : 0;
+        uint32_t held = r.stage;  // first unit of the tile whose E is multiplied next
+        for (int t = 0; t < groups + ahead && ok; ++t) {
+          if (t < groups) {
             // the buffer's previous tile: with ACC its E was consumed by an MMA issued before this one; without, its readers must be done
-            if (!kAcc && use > 0 && !wait_all(&B->p_full[b], (use - 1) & 1, FS_ERR_P)) { ok = false; break; }
-            if constexpr (!kAcc) tcgen05_fence_after();
-            const uint32_t d = tmem + b * kFsTile;
-            held_before = held;
-            held = r.stage;
+            if constexpr (!kAcc) {
+              if (sb_use > 0 && (!wait_all(&B->p_full[sb], (sb_use - 1) & 1, FS_ERR_P) || !wait_all(&B->p_full[sb + 1], (sb_use - 1) & 1, FS_ERR_P))) { ok = false; break; }
+              tcgen05_fence_after();
+            }
+            const uint32_t d = tmem + sb * kFsTile;
             for (int u = 0; u < upt; ++u) {
-              uint64_t dx = desc_k + x16 + u * unit16;
+              uint64_t dx = desc_k + x16 + u * (kAcc ? unit16 : kSlot16);
               const uint32_t xs = r.stage;
               if (!p.x_resident) {
                 if (!wait_all(&B->full[xs], r.phase, FS_ERR_FULL)) { ok = false; break; }
@@ -335,10 +341,10 @@ full_softmax_kernel(const __grid_constant__ CUtensorMap tmapX, const __grid_cons
               if (!wait_all(&B->full[ys], r.phase, FS_ERR_FULL)) { ok = false; break; }
               r.next();
               const uint64_t dy = desc_k + ring16 + ys * unit16;
-              const int steps = min(4 * spu, (p.D - u * spu * 64 + 15) / 16);  // 16 columns each
-              if (steps == 8) {
+              const int steps = kAcc ? min(4 * spu, (p.D - u * spu * 64 + 15) / 16) : min(4, (p.D - u * 64 + 15) / 16);  // 16 columns each
+              if (steps == (kAcc ? 8 : 4)) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
+                for (int i = 0; i < (kAcc ? 8 : 4); ++i) {
                   const uint32_t off = (i >> 2) * kSlot16 + (i & 3) * 2;
                   umma_bf16_elect(d, dx + off, dy + off, idesc_s, (i > 0 || u > 0) ? 1u : 0u);
                 }
@@ -353,34 +359,48 @@ full_softmax_kernel(const __grid_constant__ CUtensorMap tmapX, const __grid_cons
               if (!p.hold) tcgen05_commit_elect(&B->empty[ys]);
             }
             if (!ok) break;
-            tcgen05_commit_elect(&B->s_full[b]);
-            if (p.x_resident && t == nt - 1) tcgen05_commit_elect(&B->x_empty);
-            ++tc;
+            tcgen05_commit_elect(&B->s_full[sb]);
+            if constexpr (!kAcc) tcgen05_commit_elect(&B->s_full[sb + 1]);
+            if (p.x_resident && t == groups - 1) tcgen05_commit_elect(&B->x_empty);
+            sb += kPair;
+            if (sb == bufs) {
+              sb = 0;
+              ++sb_use;
+            }
           }
-          if (kAcc && t > 0) {
-            const uint32_t tt = (t < nt) ? tc - 2 : tc - 1;  // tile whose E is multiplied now
-            if (t == 1 && item > 0 && !wait_all(&B->o_empty, (item - 1) & 1, FS_ERR_ACC)) { ok = false; break; }
-            if (!wait_all(&B->p_full[tt & 1], (tt >> 1) & 1, FS_ERR_P)) { ok = false; break; }
+          if (kAcc && t >= ahead) {
+            const bool first = t == ahead;
+            if (first && item > 0 && !wait_all(&B->o_empty, (item - 1) & 1, FS_ERR_ACC)) { ok = false; break; }
+            if (!wait_all(&B->p_full[eb], eb_phase, FS_ERR_P)) { ok = false; break; }
             tcgen05_fence_after();
-            const uint32_t e = tmem + (tt & 1) * kFsTile;
-            uint32_t hs = t < nt ? held_before : held;
-            for (int u = pu0; u < pu1; ++u) {
-              uint32_t ys = hs;
+            const uint32_t e = tmem + eb * kFsTile;
+            for (int u = pu0; u < pu1;) {
+              uint32_t ys = held;
+              int n_units = 1;
               if (p.hold) {
-                if (++hs == units) hs = 0;
+                // both units of a tile in one product where they lie side by side in the ring
+                if (pu1 - u == 2 && held + 1 < units) n_units = 2;
+                held += n_units;
+                if (held >= units) held -= units;
               } else {
                 ys = r.stage;
                 if (!wait_all(&B->full[ys], r.phase, FS_ERR_FULL)) { ok = false; break; }
                 r.next();
               }
-              const int n = min(64 * spu, (p.D - u * 64 * spu + 15) / 16 * 16);
-              const uint32_t idesc = fs_idesc(n, true), d = tmem + 256 + (u - pu0) * 128;
+              const int n = min(64 * spu * n_units, (p.D - u * 64 * spu + 15) / 16 * 16);
+              const uint32_t idesc = fs_idesc(n, true), d = tmem + o_col + (u - pu0) * 128;
               const uint64_t dy = desc_mn + ring16 + ys * unit16;
 #pragma unroll
-              for (int i = 0; i < 8; ++i) umma_bf16_ts_elect(d, e + i * 8, dy + i * 128, idesc, (i > 0 || t > 1) ? 1u : 0u);
-              tcgen05_commit_elect(&B->empty[ys]);
+              for (int i = 0; i < 8; ++i) umma_bf16_ts_elect(d, e + i * 8, dy + i * 128, idesc, (i > 0 || !first) ? 1u : 0u);
+              for (int k = 0; k < n_units; ++k) tcgen05_commit_elect(&B->empty[ys + k]);
+              u += n_units;
             }
-            if (ok) tcgen05_commit_elect(&B->acc_done[tt & 1]);
+            if (ok) tcgen05_commit_elect(&B->acc_done[tc & 3]);
+            ++tc;
+            if (++eb == bufs) {
+              eb = 0;
+              eb_phase ^= 1;
+            }
           }
         }
       }
@@ -415,25 +435,38 @@ full_softmax_kernel(const __grid_constant__ CUtensorMap tmapX, const __grid_cons
         tgt = p.target[row];
       }
       float m2 = -INFINITY, l = 0.f;  // m2: reference of the exponentials, a whole number, so that rescaling is exact
-      const uint32_t tc0 = tc, tc1 = tc + nt;
-      for (tc += (tc ^ half) & 1; tc < tc1 && ok; tc += 2) {
+      const uint32_t tc0 = tc, tc1 = tc + (nt + kPair - 1) / kPair * kPair;
+      tc += (tc ^ half) & 1;
+      uint32_t b = tc % bufs, ph = (tc / bufs) & 1;  // the tile's buffer
+      auto next_buffer = [&] {
+        b += 2;
+        if (b >= bufs) {
+          b -= bufs;
+          ph ^= 1;
+        }
+      };
+      for (; tc < tc1 && ok; tc += 2, next_buffer()) {
         const int t = int(tc - tc0);
-        const uint32_t b = tc & (kBufs - 1), ph = (tc >> kBufShift) & 1;
         const int col0 = (t0 + t) * kFsTile;
         if (!wait_all(&B->s_full[b], ph, FS_ERR_S)) { ok = false; break; }
         tcgen05_fence_after();
+        if (!kAcc && t >= nt) {  // the pair's second tile lies behind the last
+          if (lane == 0) mbar_arrive(&B->p_full[b]);
+          continue;
+        }
         const uint32_t ts = tmem + lanes + b * kFsTile;
         uint32_t r[32];
         tmem_ld_32x32_issue(ts, r);
         if constexpr (MODE == FS_BWD) {
           const int v0 = x * kFsTile + q * 32;
           int tg = __ldg(p.target + col0 + lane);  // targets of 32 rows of h, one per lane
-          if (!wait_all(&B->c_full[b], ph, FS_ERR_COL)) { ok = false; break; }
+          const uint32_t cb = tc & (kCols - 1);
+          if (!wait_all(&B->c_full[cb], (tc >> kColShift) & 1, FS_ERR_COL)) { ok = false; break; }
 #pragma unroll 1
           for (int c = 0; c < 4; ++c) {
             float z[32];
             tmem_ld_wait(r);
-            const float4* lp = reinterpret_cast<const float4*>(cols + b * 128 + c * 32);
+            const float4* lp = reinterpret_cast<const float4*>(cols + cb * 128 + c * 32);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
               const float4 v = lp[j];
@@ -464,7 +497,7 @@ full_softmax_kernel(const __grid_constant__ CUtensorMap tmapX, const __grid_cons
               __syncwarp();
             }
             if constexpr (ROWG) {
-              const float4* gp = reinterpret_cast<const float4*>(cols + 256 + b * 128 + c * 32);
+              const float4* gp = reinterpret_cast<const float4*>(cols + 256 + cb * 128 + c * 32);
 #pragma unroll
               for (int j = 0; j < 8; ++j) {
                 const float4 v = gp[j];
@@ -487,7 +520,7 @@ full_softmax_kernel(const __grid_constant__ CUtensorMap tmapX, const __grid_cons
             tmem_st_32x16(ts + c * 16, e);
           }
           __syncwarp();
-          if (lane == 0) mbar_arrive(&B->c_empty[b]);
+          if (lane == 0) mbar_arrive(&B->c_empty[cb]);
         } else {
           const int rel = tgt - col0;  // the target's column in this tile
           const bool any_hit = __any_sync(0xffffffffu, tgt >= 0 && rel >= 0 && rel < kFsTile);
@@ -588,13 +621,13 @@ full_softmax_kernel(const __grid_constant__ CUtensorMap tmapX, const __grid_cons
                 rescale_terms(4, fe);
                 if (__any_sync(0xffffffffu, mn != mr)) {
                   // every ACC up to the previous tile has to be complete; this tile's has not been issued
-                  if (!wait_all(&B->acc_done[(tc - 1) & 1], ((tc - 1) >> 1) & 1, FS_ERR_ACC)) { ok = false; break; }
+                  if (!wait_all(&B->acc_done[(tc - 1) & 3], ((tc - 1) >> 2) & 1, FS_ERR_ACC)) { ok = false; break; }
                   tcgen05_fence_after();
                   const float f = mr == mn ? 1.f : fs_ex2(mr - mn);
                   const int groups = (min(kFsAcc, p.D - piece * kFsAcc) + 15) / 16;
 #pragma unroll 1
                   for (int g = 0; g < groups; ++g) {
-                    const uint32_t to = tmem + lanes + 256 + g * 16;
+                    const uint32_t to = tmem + lanes + o_col + g * 16;
                     uint32_t a[16];
                     tmem_ld_32x16_issue(to, a);
                     tmem_ld_wait(a);
@@ -634,10 +667,7 @@ full_softmax_kernel(const __grid_constant__ CUtensorMap tmapX, const __grid_cons
       }
       if constexpr (kAcc) {
         if (nt > 0) {
-          // the tile before the last first: a parity wait may lag behind by one use of its barrier, and the group that did not have the
-          // last tile knows no more than that the scores of the tile before it are done
-          if (nt > 1 && !wait_all(&B->acc_done[tc & 1], ((tc - 2) >> 1) & 1, FS_ERR_ACC)) { ok = false; break; }
-          if (!wait_all(&B->acc_done[(tc - 1) & 1], ((tc - 1) >> 1) & 1, FS_ERR_ACC)) { ok = false; break; }
+          if (!wait_all(&B->acc_done[(tc - 1) & 3], ((tc - 1) >> 2) & 1, FS_ERR_ACC)) { ok = false; break; }
           tcgen05_fence_after();
         }
         const int width = min(kFsAcc, p.D - piece * kFsAcc);
@@ -647,7 +677,7 @@ full_softmax_kernel(const __grid_constant__ CUtensorMap tmapX, const __grid_cons
         for (int g = half; g * 32 < width; g += 2) {
           uint32_t a[32];
           if (nt > 0) {
-            tmem_ld_32x32_issue(tmem + lanes + 256 + g * 32, a);
+            tmem_ld_32x32_issue(tmem + lanes + o_col + g * 32, a);
             tmem_ld_wait(a);
           } else {
 #pragma unroll
@@ -727,8 +757,9 @@ struct FsState {
 // ---- before the forward -----------------------------------------------------------------------------
 // Blocks 0..row_blocks-1 put the rows whose target counts one behind the other (in their order), as bf16 with zero columns up to Dp.
 // The remaining blocks copy the bias with -inf behind V.  Every row block counts the targets before its own itself: P targets are at
-// most a few hundred KB in L2, cheaper than another launch.
-constexpr int kPrepRows = 512;
+// most a few hundred KB in L2, cheaper than another launch.  A block takes 32 to 512 rows, so that two blocks per SM share the copying
+// (4096 rows of 512: 39 us with 512 rows a block).
+constexpr int kPrepThreads = 512;
 
 struct PrepParams {
   const void* h;
@@ -744,6 +775,7 @@ struct PrepParams {
   const void* bias_in;
   int64_t bias_stride;
   int bias_bf16;
+  int rows;  // of a block: a multiple of 32
   int row_blocks;
 };
 
@@ -753,22 +785,22 @@ __device__ __forceinline__ int64_t fs_target(int64_t i, const PrepParams& p) {
 // 0 ignored, 1 counts, 1 << 32 outside the classes (so that a sum counts both)
 __device__ __forceinline__ int64_t fs_target_kind(int64_t t, const PrepParams& p) { return t == p.ignore ? 0 : (t < 0 || t >= p.V ? int64_t(1) << 32 : 1); }
 
-__global__ void __launch_bounds__(kPrepRows) full_softmax_prep_kernel(const PrepParams p) {
+__global__ void __launch_bounds__(kPrepThreads) full_softmax_prep_kernel(const PrepParams p) {
   if (int(blockIdx.x) >= p.row_blocks) {
     const int64_t vpad = (int64_t(p.V) + kFsTile - 1) / kFsTile * kFsTile;
-    for (int64_t v = int64_t(blockIdx.x - p.row_blocks) * kPrepRows + threadIdx.x; v < vpad; v += int64_t(gridDim.x - p.row_blocks) * kPrepRows)
+    for (int64_t v = int64_t(blockIdx.x - p.row_blocks) * kPrepThreads + threadIdx.x; v < vpad; v += int64_t(gridDim.x - p.row_blocks) * kPrepThreads)
       p.st.bias[v] = v >= p.V        ? -INFINITY
                      : p.bias_bf16 ? __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p.bias_in)[v * p.bias_stride])
                                    : reinterpret_cast<const float*>(p.bias_in)[v * p.bias_stride];
     return;
   }
-  constexpr int kWarps = kPrepRows / 32;
+  constexpr int kWarps = kPrepThreads / 32;
   __shared__ int64_t counts[kWarps], befores[kWarps];
-  __shared__ int slots[kPrepRows];
+  __shared__ int slots[kPrepThreads];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t begin = int64_t(blockIdx.x) * kPrepRows, row = begin + threadIdx.x;
+  const int64_t begin = int64_t(blockIdx.x) * p.rows, row = int(threadIdx.x) < p.rows ? begin + threadIdx.x : p.P;  // P: no row
   int64_t before = 0;
-  for (int64_t i = threadIdx.x; i < begin; i += kPrepRows) before += fs_target_kind(fs_target(i, p), p);
+  for (int64_t i = threadIdx.x; i < begin; i += kPrepThreads) before += fs_target_kind(fs_target(i, p), p);
   const int64_t t = row < p.P ? fs_target(row, p) : p.ignore;
   const int64_t kind = fs_target_kind(t, p);
   const uint32_t mine = __ballot_sync(0xffffffffu, kind == 1), bad = __ballot_sync(0xffffffffu, kind > 1);
@@ -799,7 +831,7 @@ __global__ void __launch_bounds__(kPrepRows) full_softmax_prep_kernel(const Prep
     }
     if (kind > 1) atomicCAS(&g_fs_error, 0, FS_ERR_TARGET);
   }
-  if (threadIdx.x < kPrepRows / kFsTile && begin + int64_t(threadIdx.x) * kFsTile < p.P) p.st.counters[FS_COUNTERS + begin / kFsTile + threadIdx.x] = 0;
+  if (row < p.P && row % kFsTile == 0) p.st.counters[FS_COUNTERS + row / kFsTile] = 0;
   __syncthreads();
   const bool last = int(blockIdx.x) == p.row_blocks - 1;
   const int n = int((total + block_total) & 0x7fffffff), padded = (n + kFsTile - 1) / kFsTile * kFsTile;
@@ -814,9 +846,9 @@ __global__ void __launch_bounds__(kPrepRows) full_softmax_prep_kernel(const Prep
     if (n + int(threadIdx.x) < padded) p.st.target[n + threadIdx.x] = -1;
   }
   const int vecs = p.Dp / 8;
-  const int rows = int(min(int64_t(kPrepRows), p.P - begin));
+  const int rows = int(min(int64_t(p.rows), p.P - begin));
   // eight columns at a time
-  for (int i = threadIdx.x; i < rows * vecs; i += kPrepRows) {
+  for (int i = threadIdx.x; i < rows * vecs; i += kPrepThreads) {
     const int r = i / vecs, c = (i - r * vecs) * 8, to = slots[r];
     if (to < 0) continue;
     uint4 o;
@@ -834,7 +866,7 @@ __global__ void __launch_bounds__(kPrepRows) full_softmax_prep_kernel(const Prep
     *reinterpret_cast<uint4*>(p.st.hc + int64_t(to) * p.Dp + c) = o;
   }
   if (last)
-    for (int i = threadIdx.x; i < (padded - n) * vecs; i += kPrepRows) *reinterpret_cast<uint4*>(p.st.hc + int64_t(n) * p.Dp + int64_t(i) * 8) = make_uint4(0, 0, 0, 0);
+    for (int i = threadIdx.x; i < (padded - n) * vecs; i += kPrepThreads) *reinterpret_cast<uint4*>(p.st.hc + int64_t(n) * p.Dp + int64_t(i) * 8) = make_uint4(0, 0, 0, 0);
 }
 
 // ---- after the forward: join the splits of every row --------------------------------------------------
@@ -875,25 +907,34 @@ __global__ void __launch_bounds__(kJoinThreads) full_softmax_join_kernel(const J
   };
   if (row >= n) {  // a streamed row of zeros: exp(0 - inf) = 0
     if (threadIdx.x == 0) p.st.lse2[row] = INFINITY;
-  } else {
+    return;
+  }
+  const float z = p.zt[row];
+  {
     const FsSchedule sc = fs_schedule(n, p.V, p.pieces, p.grid);
     const int64_t prow = int64_t(sc.tx) * kFsTile;
-    float m = -INFINITY;
-    for (int s = threadIdx.x; s < 2 * sc.splits; s += kJoinThreads) m = fmaxf(m, p.part_m[s * prow + row]);
+    float m = -INFINITY, l = 0.f;
+    for (int s = threadIdx.x; s < 2 * sc.splits; s += kJoinThreads) {
+      const float ms = p.part_m[s * prow + row], ls = p.part_l[s * prow + row];
+      const float mn = fmaxf(m, ms);
+      if (mn != -INFINITY) l = l * exp2f(m - mn) + ls * exp2f(ms - mn);
+      else l += ls;
+      m = mn;
+      if (ACC && !(s & 1)) js[s >> 1] = ms;
+    }
+    const float mine = m;
     m = warp_max(m);
     if (lane == 0) red[warp] = m;
     __syncthreads();
     m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
     const float ms = m == -INFINITY ? 0.f : m;
-    float l = 0.f;
-    for (int s = threadIdx.x; s < 2 * sc.splits; s += kJoinThreads) {
-      const float f = exp2f(p.part_m[s * prow + row] - ms);
-      l += f * p.part_l[s * prow + row];
-      if (ACC && !(s & 1)) js[s >> 1] = f;
+    l = block_sum(mine == -INFINITY ? l : l * exp2f(mine - ms));
+    if (ACC) {
+      for (int s = threadIdx.x; s < sc.splits; s += kJoinThreads) js[s] = exp2f(js[s] - ms);
+      __syncthreads();
     }
-    l = block_sum(l);
     // others' log sum a, target's score z (base 2): lse = max + log2(1 + 2^-|a - z|)
-    const float a = ms + log2f(l), z = p.zt[row], d = a - z;
+    const float a = ms + log2f(l), d = a - z;
     const float tail = log1pf(exp2f(-fabsf(d)));
     const float w = d > 0.f ? 1.f / (1.f + exp2f(-d)) : exp2f(d) / (1.f + exp2f(d));  // 1 - p_t
     if (threadIdx.x == 0) {
@@ -958,14 +999,16 @@ __global__ void __launch_bounds__(kJoinThreads) full_softmax_join_kernel(const J
     return true;
   };
   const int tile = row / kFsTile;
-  if (!last_of(p.st.counters + FS_COUNTERS + tile, kFsTile)) return;
-  const int i = tile * kFsTile + threadIdx.x;
-  float s = block_sum(i < n ? __ldcg(p.loss_c + i) : 0.f);
-  if (threadIdx.x == 0) p.tile_loss[tile] = s;
-  if (!last_of(p.st.counters + FS_JOINED, padded / kFsTile)) return;
-  s = 0.f;
-  for (int k = threadIdx.x; k < padded / kFsTile; k += kJoinThreads) s += __ldcg(p.tile_loss + k);
-  s = block_sum(s);
+  const int in_tile = min(kFsTile, n - tile * kFsTile), tiles = padded / kFsTile;
+  if (in_tile > 1 && !last_of(p.st.counters + FS_COUNTERS + tile, in_tile)) return;
+  float s = block_sum(int(threadIdx.x) < in_tile ? __ldcg(p.loss_c + tile * kFsTile + threadIdx.x) : 0.f);
+  if (tiles > 1) {
+    if (threadIdx.x == 0) p.tile_loss[tile] = s;
+    if (!last_of(p.st.counters + FS_JOINED, tiles)) return;
+    s = 0.f;
+    for (int k = threadIdx.x; k < tiles; k += kJoinThreads) s += __ldcg(p.tile_loss + k);
+    s = block_sum(s);
+  }
   if (threadIdx.x == 0) *p.loss = p.st.counters[FS_N_BAD] > 0 ? __int_as_float(0x7fc00000) : (p.reduction == 1 ? s / float(n) : s);
 }
 
@@ -1130,14 +1173,16 @@ std::tuple<at::Tensor, at::Tensor> full_softmax_fwd(const at::Tensor& h, const a
   float* zt = part_l + 2 * prows;
   float* loss_c = zt + Ppad;
   {
-    const int row_blocks = int((P + kPrepRows - 1) / kPrepRows);
-    const int bias_blocks = has_bias ? int(std::min<int64_t>((Vpad + kPrepRows - 1) / kPrepRows, 2 * grid)) : 0;
+    int rows = 32;
+    while (rows < kPrepThreads && int64_t(rows) * 2 * grid < P) rows *= 2;
+    const int row_blocks = int((P + rows - 1) / rows);
+    const int bias_blocks = has_bias ? int(std::min<int64_t>((Vpad + kPrepThreads - 1) / kPrepThreads, 2 * grid)) : 0;
     const bool fp32 = h.scalar_type() == at::kFloat;
     const bool vec = !fp32 && D == Dp && h.stride(1) == 1 && h.stride(0) % 8 == 0 && reinterpret_cast<uintptr_t>(h.data_ptr()) % 16 == 0;
     const PrepParams q{h.data_ptr(), h.stride(0), h.stride(1), fp32, vec, targets.data_ptr(), targets.stride(0), ignore_index, targets.scalar_type() == at::kInt,
                        int(P), int(V), int(D), int(Dp), st, loss.data_ptr<float>(), int(reduction), has_bias ? bias->data_ptr() : nullptr, has_bias ? bias->stride(0) : 0,
-                       has_bias && bias->scalar_type() == at::kBFloat16, row_blocks};
-    full_softmax_prep_kernel<<<row_blocks + bias_blocks, kPrepRows, 0, stream>>>(q);
+                       has_bias && bias->scalar_type() == at::kBFloat16, rows, row_blocks};
+    full_softmax_prep_kernel<<<row_blocks + bias_blocks, kPrepThreads, 0, stream>>>(q);
     TRB_CUDA_CHECK(cudaGetLastError());
   }
   FsParams p{};

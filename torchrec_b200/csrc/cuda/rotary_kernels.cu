@@ -58,7 +58,6 @@ template <typename T>
 struct RotRaw {
   uint4 u;
   __device__ __forceinline__ void load(const T* p) { u = __ldg(reinterpret_cast<const uint4*>(p)); }
-  __device__ __forceinline__ void zero() { u = make_uint4(0, 0, 0, 0); }
   __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<uint4*>(p) = u; }
   __device__ __forceinline__ RotRaw from_lane(int lane) const {
     RotRaw r;
@@ -87,7 +86,6 @@ struct RotRaw<float> {
     a = __ldg(reinterpret_cast<const float4*>(p));
     b = __ldg(reinterpret_cast<const float4*>(p) + 1);
   }
-  __device__ __forceinline__ void zero() { a = b = f4zero(); }
   __device__ __forceinline__ void store(float* p) const {
     reinterpret_cast<float4*>(p)[0] = a;
     reinterpret_cast<float4*>(p)[1] = b;
@@ -214,12 +212,6 @@ __device__ __forceinline__ void rot_weights(const float* w, int d0, int p0, int 
   }
 }
 
-// sum over the lanes of a head (its power-of-two group of lanes)
-__device__ __forceinline__ float rot_group_sum(float v, int lp_log2) {
-  for (int o = 1 << lp_log2 >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
-}
-
 // sine and cosine of `turn` turns, |turn| <= 1/2: to 2^-23 for fp32 outputs; for 16-bit ones the hardware functions, 2^-20 off, which is
 // far below half a step of the output
 template <typename T>
@@ -230,9 +222,13 @@ __device__ __forceinline__ float2 rot_cos_sin(float turn) {
   return make_float2(c, s);
 }
 
-// Registers are bounded so that 32 (forward) or 24 (backward) warps share an SM.
+// Registers are bounded so that 32 warps share an SM (forward, 16-bit types), or 24 (fp32: 83 us with 32, 71 us with 24 for 20011 tokens of
+// 20 heads of 128; backward: 450 us with 24, 500 us with 16 and 524 us with 32 for 450563 tokens of 12 heads of 64).
+template <typename T, bool BWD>
+constexpr int kRotBlocks = BWD || sizeof(T) == 4 ? 3 : 4;
+
 template <typename T, int PAIRS, bool BWD>
-__global__ void __launch_bounds__(kRotThreads, BWD ? 3 : 4) qk_norm_rotary_kernel(const RotaryParams p) {
+__global__ void __launch_bounds__(kRotThreads, kRotBlocks<T, BWD>) qk_norm_rotary_kernel(const RotaryParams p) {
   constexpr int kBatch = sizeof(T) == 4 ? (BWD ? 1 : 2) : (BWD ? 2 : 4);  // heads whose loads are in flight together
   __shared__ __align__(16) float2 cs_all[kRotWarps][kRotMaxDim / 2];  // a warp's tokens x frequencies (their product is at most 128)
   __shared__ __align__(16) float w_s[2][kRotMaxDim];
@@ -261,7 +257,6 @@ __global__ void __launch_bounds__(kRotThreads, BWD ? 3 : 4) qk_norm_rotary_kerne
   const int p0 = d0 >= 2 * p.n_freq ? d0 : (d0 < p.n_freq ? d0 + p.n_freq : d0 - p.n_freq);
   const int partner_lane = in_head ? lane + (p0 - d0) / 8 : lane;
   const int turned = p.Hq + p.Hk, heads = turned + p.Hk;
-  const int stride = p.split * p.Dh;
   float2* cs = cs_all[warp] + group * p.n_freq;
   const float inv_dim = 1.f / float(p.Dh);
   const int64_t blocks_of_tokens = (p.T + tokens - 1) / tokens, items = blocks_of_tokens * p.split, step = int64_t(gridDim.x) * kRotWarps;
@@ -273,123 +268,125 @@ __global__ void __launch_bounds__(kRotThreads, BWD ? 3 : 4) qk_norm_rotary_kerne
       part = int(item - first * p.split);
     }
     const int64_t token = first * tokens + group;
-    const bool live = token < p.T, act = live && in_head;
-    const T* row = reinterpret_cast<const T*>(p.qkv) + token * p.ld + part * p.Dh;
-    T* out = reinterpret_cast<T*>(p.out) + (token * heads + part) * p.Dh + d0;
-    const T* drow = BWD ? reinterpret_cast<const T*>(p.dy) + token * p.ld_dy + part * p.Dh : nullptr;
+    const bool act = token < p.T && in_head;
+    const int64_t safe = min(token, p.T - 1);  // lane groups behind the last token follow it and store nothing
+    const T* row = reinterpret_cast<const T*>(p.qkv) + safe * p.ld;
+    const T* drow = BWD ? reinterpret_cast<const T*>(p.dy) + safe * p.ld_dy : nullptr;
+    T* out = reinterpret_cast<T*>(p.out) + safe * heads * p.Dh + d0;
     RotRaw<T> rx[kBatch], rg[BWD ? kBatch : 1];
-    auto load = [&](int head) {  // the heads head, head + split, ...; `row` and `drow` are at the first of them
+    auto load = [&](int head, int end) {
 #pragma unroll
-      for (int i = 0; i < kBatch; ++i) {
-        const int h = head + i * p.split;
-        if constexpr (BWD) {
-          rx[i].zero();
-          rg[i].zero();
-          if (act && h < turned) rx[i].load(row + i * stride + d0);
-          if (act && h < heads) rg[i].load(drow + i * stride + d0);
-        } else {
-          rx[i].zero();
-          if (act && h < heads) rx[i].load(row + i * stride + d0);
+      for (int i = 0; i < kBatch; ++i)
+        if (head + i * p.split < end) {
+          const int off = (head + i * p.split) * p.Dh + d0;
+          rx[i].load(row + off);
+          if constexpr (BWD) rg[i].load(drow + off);
         }
-      }
     };
-    load(part);  // on its way while the angles are computed
-    __syncwarp();  // the previous tokens' angles have been read
-    if (live)
-      for (int j = li; j < p.n_freq; j += lp) {
-        const int64_t at = axis_s[j] + token * p.pos_token;
-        double turn = (p.pos64 ? double(reinterpret_cast<const int64_t*>(p.positions)[at]) : double(reinterpret_cast<const int*>(p.positions)[at])) * freq_s[j];
-        turn -= rint(turn);
-        cs[j] = rot_cos_sin<T>(float(turn));
-      }
-    __syncwarp();
-    float c[8], s[8], w[8], wp[8], acc[8];
-    int type = -1;  // whose weights (and, forward, factors times weights) are in the registers: 0 q, 1 k
-    rot_factors<PAIRS>(cs, d0, p.n_freq, c, s);
-    auto flush = [&]() {  // dw of the heads of one type
-      float* d = dw_s + (type * kRotThreads + threadIdx.x) * 8;
-      float v[8];
-      rot_smem8(d, v);
-#pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] += acc[k];
-      reinterpret_cast<float4*>(d)[0] = make_float4(v[0], v[1], v[2], v[3]);
-      reinterpret_cast<float4*>(d)[1] = make_float4(v[4], v[5], v[6], v[7]);
-    };
-#pragma unroll 1
-    for (int head = part; head < heads; head += kBatch * p.split) {  // the same for all lanes
-#pragma unroll
-      for (int i = 0; i < kBatch; ++i) {
-        const int h = head + i * p.split;
-        if (h >= heads) break;
-        T* o = out + i * stride;
-        if (h >= turned) {
-          if (act) (BWD ? rg[BWD ? i : 0] : rx[i]).store(o);
-          continue;
-        }
-        const int now = h < p.Hq ? 0 : 1;
-        if (now != type) {
-          if constexpr (BWD) {
-            if (p.dw_part != nullptr && type >= 0) flush();
-#pragma unroll
-            for (int k = 0; k < 8; ++k) acc[k] = 0.f;
-            rot_smem8(w_s[now] + d0, w);
-          } else {
-            rot_factors<PAIRS>(cs, d0, p.n_freq, c, s);
-            rot_weights<PAIRS>(w_s[now], d0, p0, p.n_freq, w, wp);
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-              c[k] *= w[k];
-              s[k] *= wp[k];
-            }
-          }
-          type = now;
-        }
-        float x[8];
-        rx[i].unpack(x);
-        if constexpr (!BWD) {
-          float xp[8];
-          rot_partner<T, PAIRS>(row + i * stride, act, d0, partner_lane, p.n_freq, rx[i], x, xp);
-          float sq = 0.f;
-#pragma unroll
-          for (int k = 0; k < 8; ++k) sq += x[k] * x[k];
-          sq = rot_group_sum(sq, p.lp_log2);  // lanes without a part of the head hold zeros
-          const float rstd = p.norm ? rsqrtf(sq * inv_dim + p.eps) : 1.f;
-#pragma unroll
-          for (int k = 0; k < 8; ++k) x[k] = rstd * (c[k] * x[k] + s[k] * xp[k]);
-          if (act) rot_store8(o, x);
-        } else {
-          float g[8], gp[8];
-          rg[i].unpack(g);
-          rot_partner<T, PAIRS>(drow + i * stride, act, d0, partner_lane, p.n_freq, rg[i], g, gp);
-          float sq = 0.f, dot = 0.f;
-#pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            g[k] = (c[k] * g[k] - s[k] * gp[k]);
-            sq += x[k] * x[k];
-            gp[k] = g[k] * x[k];
-            dot += w[k] * gp[k];
-          }
-          sq = rot_group_sum(sq, p.lp_log2);
-          dot = rot_group_sum(dot, p.lp_log2);
-          const float rstd = p.norm ? rsqrtf(sq * inv_dim + p.eps) : 1.f;
-          const float back = p.norm ? rstd * rstd * dot * inv_dim : 0.f;
-          if (act) {  // (elsewhere rstd may be infinite)
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-              acc[k] += gp[k] * rstd;
-              x[k] = rstd * (w[k] * g[k] - x[k] * back);
-            }
-            rot_store8(o, x);
-          }
-        }
-      }
-      row += kBatch * stride;
-      out += kBatch * stride;
-      if constexpr (BWD) drow += kBatch * stride;
-      if (head + kBatch * p.split < heads) load(head + kBatch * p.split);
+    load(part, p.Hq);  // on its way while the angles are computed
+    __syncwarp();      // the previous tokens' angles have been read
+    for (int j = li; j < p.n_freq; j += lp) {
+      const int64_t at = axis_s[j] + safe * p.pos_token;
+      double turn = (p.pos64 ? double(reinterpret_cast<const int64_t*>(p.positions)[at]) : double(reinterpret_cast<const int*>(p.positions)[at])) * freq_s[j];
+      turn -= rint(turn);
+      cs[j] = rot_cos_sin<T>(float(turn));
     }
-    if constexpr (BWD) {
-      if (p.dw_part != nullptr && type >= 0) flush();
+    __syncwarp();
+    int head = part, end = p.Hq;
+#pragma unroll 1
+    for (int type = 0; type < 2; ++type) {  // queries, keys
+      float c[8], s[8], w[8], wp[8], acc[8];
+      rot_factors<PAIRS>(cs, d0, p.n_freq, c, s);
+      rot_weights<PAIRS>(w_s[type], d0, p0, p.n_freq, w, wp);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        if constexpr (BWD) {
+          acc[k] = 0.f;
+        } else {
+          c[k] *= w[k];
+          s[k] *= wp[k];
+        }
+      }
+      if (type == 1) {
+        end = turned;
+        load(head, end);
+      }
+#pragma unroll 1
+      while (head < end) {  // the same for all lanes
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+          if (head + i * p.split >= end) break;
+          const int off = (head + i * p.split) * p.Dh;
+          float x[8];
+          rx[i].unpack(x);
+          if constexpr (!BWD) {
+            float xp[8];
+            rot_partner<T, PAIRS>(row + off, true, d0, partner_lane, p.n_freq, rx[i], x, xp);
+            float sq = 0.f;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) sq += x[k] * x[k];
+            sq = in_head ? sq : 0.f;
+            for (int o = lp >> 1; o > 0; o >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, o);
+            const float rstd = p.norm ? rsqrtf(sq * inv_dim + p.eps) : 1.f;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) x[k] = rstd * (c[k] * x[k] + s[k] * xp[k]);
+            if (act) rot_store8(out + off, x);
+          } else {
+            float g[8], gp[8];
+            rg[i].unpack(g);
+            rot_partner<T, PAIRS>(drow + off, true, d0, partner_lane, p.n_freq, rg[i], g, gp);
+            float sq = 0.f, dot = 0.f;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              g[k] = c[k] * g[k] - s[k] * gp[k];
+              sq += x[k] * x[k];
+              gp[k] = g[k] * x[k];
+              dot += w[k] * gp[k];
+            }
+            sq = in_head ? sq : 0.f;
+            dot = in_head ? dot : 0.f;
+            for (int o = lp >> 1; o > 0; o >>= 1) {
+              sq += __shfl_xor_sync(0xffffffffu, sq, o);
+              dot += __shfl_xor_sync(0xffffffffu, dot, o);
+            }
+            const float rstd = p.norm ? rsqrtf(sq * inv_dim + p.eps) : 1.f;
+            const float back = p.norm ? rstd * rstd * dot * inv_dim : 0.f;
+            if (act) {
+#pragma unroll
+              for (int k = 0; k < 8; ++k) {
+                acc[k] += gp[k] * rstd;
+                x[k] = rstd * (w[k] * g[k] - x[k] * back);
+              }
+              rot_store8(out + off, x);
+            }
+          }
+        }
+        head += kBatch * p.split;
+        if (head < end) load(head, end);
+      }
+      // the first of this warp's heads of the next type
+      head = type == 0 ? part + (p.Hq - part + p.split - 1) / p.split * p.split : head;
+      if constexpr (BWD) {
+        if (p.dw_part != nullptr) {
+          float* d = dw_s + (type * kRotThreads + threadIdx.x) * 8;
+          float v[8];
+          rot_smem8(d, v);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) v[k] += acc[k];
+          rot_store8(d, v);
+        }
+      }
+    }
+    // v
+    const T* vrow = BWD ? drow : row;
+#pragma unroll 1
+    for (head = part + (turned - part + p.split - 1) / p.split * p.split; head < heads; head += kBatch * p.split) {
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i)
+        if (head + i * p.split < heads) rx[i].load(vrow + (head + i * p.split) * p.Dh + d0);
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i)
+        if (act && head + i * p.split < heads) rx[i].store(out + (head + i * p.split) * p.Dh);
     }
   }
   if constexpr (BWD) {
@@ -497,7 +494,7 @@ static std::tuple<at::Tensor, at::Tensor> rot_run(const at::Tensor& qkv, const c
   const int64_t groups = (T + (32 >> p.lp_log2) - 1) / (32 >> p.lp_log2);
   p.split = int(std::max<int64_t>(1, std::min<int64_t>(Hq + 2 * Hk, 16LL * sms / groups)));
   const int64_t warps = groups * p.split;
-  const int blocks = int(std::min<int64_t>((warps + kRotWarps - 1) / kRotWarps, (bwd ? 3 : 4) * sms));
+  const int blocks = int(std::min<int64_t>((warps + kRotWarps - 1) / kRotWarps, (bwd || qkv.scalar_type() == at::kFloat ? 3 : 4) * sms));
   at::Tensor part;
   if (want_dw) {
     part = at::empty({blocks, 2, Dh}, dw.options());

@@ -304,6 +304,7 @@ full_softmax_kernel(const __grid_constant__ CUtensorMap tmapX, const __grid_cons
     // S of the next one or two tiles is issued before ACC(t), so the tensor cores work while the softmax warps turn S(t) into E(t).  Descriptors advance by
     // additions (addresses in units of 16 bytes).  The whole warp runs the loop, one elected lane issues.
     {
+      const uint32_t leader = elect_one();
       auto wait_all = [&](uint64_t* bar, uint32_t parity, int code) {
         return __all_sync(0xffffffffu, fs_wait(bar, parity, abort_flag, code)) != 0;
       };
@@ -314,6 +315,15 @@ full_softmax_kernel(const __grid_constant__ CUtensorMap tmapX, const __grid_cons
       constexpr uint32_t kSlot16 = kFsSlotBytes / 16;
       const uint64_t desc_k = make_smem_desc(0, 16, 1024), desc_mn = make_smem_desc(0, kFsSlotBytes, 1024);
       const uint32_t x16 = smem_u32(fs_smem) >> 4, ring16 = smem_u32(ring) >> 4, unit16 = spu * kSlot16;
+      // 64 columns as four products of 16 (the last of them may hold zero columns only)
+      auto score_block = [&](uint32_t d, uint64_t dx, uint64_t dy, bool first) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) umma_bf16_by(leader, d, dx + i * 2, dy + i * 2, idesc_s, (i > 0 || !first) ? 1u : 0u);
+      };
+      // rows of up to 256: what does not change from tile to tile
+      const uint32_t n0 = min(64 * spu, (p.D + 15) / 16 * 16), n_all = (p.D + 15) / 16 * 16;
+      const uint32_t idesc_0 = fs_idesc(n0, true), idesc_1 = fs_idesc(n_all > 128 ? n_all - 128 : 16, true), idesc_all = fs_idesc(n_all & 0x1ff, true);
+      const bool two_units = upt == 2, slot_1 = p.kb > 1, slot_3 = p.kb > 3;
       for (int w = blockIdx.x; w < sc.items && ok; w += gridDim.x, ++item) {
         const int split = w / base, rem = w - split * base, piece = rem / sc.tx;
         const int t0 = split * sc.per, nt = min(sc.ty, t0 + sc.per) - t0;
@@ -321,6 +331,61 @@ full_softmax_kernel(const __grid_constant__ CUtensorMap tmapX, const __grid_cons
         const int pu0 = piece * (kFsAcc / 128), pu1 = min(upt, pu0 + kFsAcc / 128);
         const int groups = (nt + kPair - 1) / kPair, ahead = kAcc ? int(bufs) - 1 : 0;
         uint32_t held = r.stage;  // first unit of the tile whose E is multiplied next
+        if (kAcc && p.hold) {
+          for (int t = 0; t < groups + ahead; ++t) {
+            if (t < groups) {
+              const uint32_t d = tmem + sb * kFsTile;
+              if (!wait_all(&B->full[r.stage], r.phase, FS_ERR_FULL)) { ok = false; break; }
+              uint64_t dy = desc_k + ring16 + r.stage * unit16;
+              r.next();
+              score_block(d, desc_k + x16, dy, true);
+              if (slot_1) score_block(d, desc_k + x16 + kSlot16, dy + kSlot16, false);
+              if (two_units) {
+                if (!wait_all(&B->full[r.stage], r.phase, FS_ERR_FULL)) { ok = false; break; }
+                dy = desc_k + ring16 + r.stage * unit16;
+                r.next();
+                score_block(d, desc_k + x16 + 2 * kSlot16, dy, false);
+                if (slot_3) score_block(d, desc_k + x16 + 3 * kSlot16, dy + kSlot16, false);
+              }
+              tcgen05_commit_by(leader, &B->s_full[sb]);
+              if (t == groups - 1) tcgen05_commit_by(leader, &B->x_empty);
+              if (++sb == bufs) sb = 0;
+            }
+            if (t >= ahead) {
+              const uint32_t more = t == ahead ? 0u : 1u;
+              if (more == 0 && item > 0 && !wait_all(&B->o_empty, (item - 1) & 1, FS_ERR_ACC)) { ok = false; break; }
+              if (!wait_all(&B->p_full[eb], eb_phase, FS_ERR_P)) { ok = false; break; }
+              tcgen05_fence_after();
+              const uint32_t e = tmem + eb * kFsTile;
+              const uint32_t next = held + 1 == units ? 0 : held + 1;
+              const uint64_t dy = desc_mn + ring16 + held * unit16;
+              if (two_units && next != 0) {  // both units of the tile in one product where they lie side by side in the ring
+#pragma unroll
+                for (int i = 0; i < 8; ++i) umma_bf16_ts_by(leader, tmem + o_col, e + i * 8, dy + i * 128, idesc_all, i > 0 ? 1u : more);
+                tcgen05_commit_by(leader, &B->empty[held]);
+                tcgen05_commit_by(leader, &B->empty[next]);
+              } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) umma_bf16_ts_by(leader, tmem + o_col, e + i * 8, dy + i * 128, idesc_0, i > 0 ? 1u : more);
+                tcgen05_commit_by(leader, &B->empty[held]);
+                if (two_units) {
+                  const uint64_t dy1 = desc_mn + ring16 + next * unit16;
+#pragma unroll
+                  for (int i = 0; i < 8; ++i) umma_bf16_ts_by(leader, tmem + o_col + 128, e + i * 8, dy1 + i * 128, idesc_1, i > 0 ? 1u : more);
+                  tcgen05_commit_by(leader, &B->empty[next]);
+                }
+              }
+              held = two_units ? (next + 1 == units ? 0 : next + 1) : next;
+              tcgen05_commit_by(leader, &B->acc_done[tc & 3]);
+              ++tc;
+              if (++eb == bufs) {
+                eb = 0;
+                eb_phase ^= 1;
+              }
+            }
+          }
+          continue;
+        }
         for (int t = 0; t < groups + ahead && ok; ++t) {
           if (t < groups) {
             // the buffer's previous tile: with ACC its E was consumed by an MMA issued before this one; without, its readers must be done
@@ -346,22 +411,22 @@ full_softmax_kernel(const __grid_constant__ CUtensorMap tmapX, const __grid_cons
 #pragma unroll
                 for (int i = 0; i < (kAcc ? 8 : 4); ++i) {
                   const uint32_t off = (i >> 2) * kSlot16 + (i & 3) * 2;
-                  umma_bf16_elect(d, dx + off, dy + off, idesc_s, (i > 0 || u > 0) ? 1u : 0u);
+                  umma_bf16_by(leader, d, dx + off, dy + off, idesc_s, (i > 0 || u > 0) ? 1u : 0u);
                 }
               } else {
 #pragma unroll 1
                 for (int i = 0; i < steps; ++i) {
                   const uint32_t off = (i >> 2) * kSlot16 + (i & 3) * 2;
-                  umma_bf16_elect(d, dx + off, dy + off, idesc_s, (i > 0 || u > 0) ? 1u : 0u);
+                  umma_bf16_by(leader, d, dx + off, dy + off, idesc_s, (i > 0 || u > 0) ? 1u : 0u);
                 }
               }
-              if (!p.x_resident) tcgen05_commit_elect(&B->empty[xs]);
-              if (!p.hold) tcgen05_commit_elect(&B->empty[ys]);
+              if (!p.x_resident) tcgen05_commit_by(leader, &B->empty[xs]);
+              tcgen05_commit_by(leader, &B->empty[ys]);
             }
             if (!ok) break;
-            tcgen05_commit_elect(&B->s_full[sb]);
-            if constexpr (!kAcc) tcgen05_commit_elect(&B->s_full[sb + 1]);
-            if (p.x_resident && t == groups - 1) tcgen05_commit_elect(&B->x_empty);
+            tcgen05_commit_by(leader, &B->s_full[sb]);
+            if constexpr (!kAcc) tcgen05_commit_by(leader, &B->s_full[sb + 1]);
+            if (p.x_resident && t == groups - 1) tcgen05_commit_by(leader, &B->x_empty);
             sb += kPair;
             if (sb == bufs) {
               sb = 0;
@@ -374,28 +439,18 @@ full_softmax_kernel(const __grid_constant__ CUtensorMap tmapX, const __grid_cons
             if (!wait_all(&B->p_full[eb], eb_phase, FS_ERR_P)) { ok = false; break; }
             tcgen05_fence_after();
             const uint32_t e = tmem + eb * kFsTile;
-            for (int u = pu0; u < pu1;) {
-              uint32_t ys = held;
-              int n_units = 1;
-              if (p.hold) {
-                // both units of a tile in one product where they lie side by side in the ring
-                if (pu1 - u == 2 && held + 1 < units) n_units = 2;
-                held += n_units;
-                if (held >= units) held -= units;
-              } else {
-                ys = r.stage;
-                if (!wait_all(&B->full[ys], r.phase, FS_ERR_FULL)) { ok = false; break; }
-                r.next();
-              }
-              const int n = min(64 * spu * n_units, (p.D - u * 64 * spu + 15) / 16 * 16);
+            for (int u = pu0; u < pu1; ++u) {
+              const uint32_t ys = r.stage;
+              if (!wait_all(&B->full[ys], r.phase, FS_ERR_FULL)) { ok = false; break; }
+              r.next();
+              const int n = min(64 * spu, (p.D - u * 64 * spu + 15) / 16 * 16);
               const uint32_t idesc = fs_idesc(n, true), d = tmem + o_col + (u - pu0) * 128;
               const uint64_t dy = desc_mn + ring16 + ys * unit16;
 #pragma unroll
-              for (int i = 0; i < 8; ++i) umma_bf16_ts_elect(d, e + i * 8, dy + i * 128, idesc, (i > 0 || !first) ? 1u : 0u);
-              for (int k = 0; k < n_units; ++k) tcgen05_commit_elect(&B->empty[ys + k]);
-              u += n_units;
+              for (int i = 0; i < 8; ++i) umma_bf16_ts_by(leader, d, e + i * 8, dy + i * 128, idesc, (i > 0 || !first) ? 1u : 0u);
+              tcgen05_commit_by(leader, &B->empty[ys]);
             }
-            if (ok) tcgen05_commit_elect(&B->acc_done[tc & 3]);
+            if (ok) tcgen05_commit_by(leader, &B->acc_done[tc & 3]);
             ++tc;
             if (++eb == bufs) {
               eb = 0;
@@ -405,7 +460,7 @@ full_softmax_kernel(const __grid_constant__ CUtensorMap tmapX, const __grid_cons
         }
       }
       if (!ok) {  // products already issued must end before the tensor memory is freed
-        tcgen05_commit_elect(&B->drain);
+        tcgen05_commit_by(leader, &B->drain);
         const long long begin = clock64();
         while (!mbar_try_wait(&B->drain, 0) && clock64() - begin < kWaitCycles) {
         }

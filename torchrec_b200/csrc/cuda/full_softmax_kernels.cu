@@ -44,7 +44,6 @@ constexpr int kFsMaxD = 1024;
 constexpr int kFsAcc = 256;                         // accumulator columns
 constexpr int kFsExtra = 3072;                      // per-column values of a tile, exchange of maxima, barriers
 constexpr int kFsSmem = kFsSlots * kFsSlotBytes + kFsExtra;
-constexpr int kFsItemsPerSm = 8;                    // bounds the workspace of partial results
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 // Base-2 growth of a row's maximum that forces a rescale.  The terms have bf16's and fp32's exponents: 2^40 over 2^31 columns is far
@@ -56,47 +55,59 @@ enum FsErr : int { FS_ERR_EMPTY = 1, FS_ERR_FULL = 2, FS_ERR_X = 3, FS_ERR_S = 4
 
 __device__ int g_fs_error = 0;  // one word per device; never allocated, so it may first be touched inside a graph capture
 
-// How the tiles of X, pieces of the accumulator's columns and pieces of the streamed axis are dealt to the blocks.  Computed alike by
-// every block (the number of rows that are not ignored is only known on the device).
+// How the work is dealt to the blocks.  An item is a tile of X and a piece of the accumulator's columns; it streams `ty` tiles of Y.  Every
+// block takes the same number of whole items, and what is left over (fewer items than blocks) is cut along the streamed axis into one equal
+// run per block, which may cross from one item into the next: with whole items alone 313 items keep 148 SMs busy 70 % of the time.
+// Blocks work on whole items in step, so that a streamed tile that one of them fetched is in L2 for the others.  Computed alike by every
+// kernel (the number of rows that are not ignored is only known on the device), in whole numbers.
 struct FsSchedule {
-  int tx, ty, pieces, splits, per, items;
+  int tx, ty, steps, whole, rest, run;  // steps: tiles of an item, at least 1; whole: items per block; rest: items left over; run: steps of a block's share of them
+
+  __host__ __device__ FsSchedule(int nx, int ny, int pieces, int grid) {
+    tx = (nx + kFsTile - 1) / kFsTile;
+    ty = (ny + kFsTile - 1) / kFsTile;
+    steps = ty > 0 ? ty : 1;
+    whole = tx * pieces / grid;
+    rest = tx * pieces - whole * grid;
+    run = int((int64_t(rest) * steps + grid - 1) / grid);
+  }
+  // the runs that an item left over (`rel`: counted from the first of them) is cut into
+  __host__ __device__ int first_run(int rel) const { return int(int64_t(rel) * steps / run); }
+  __host__ __device__ int last_run(int rel) const { return int((int64_t(rel + 1) * steps - 1) / run); }
 };
 
-__host__ __device__ inline FsSchedule fs_schedule(int nx, int ny, int pieces, int grid) {
-  FsSchedule s;
-  s.tx = (nx + kFsTile - 1) / kFsTile;
-  s.ty = (ny + kFsTile - 1) / kFsTile;
-  s.pieces = pieces;
-  s.splits = 1;
-  s.per = s.ty;
-  const int base = s.tx * pieces;
-  if (base > 0 && s.ty > 1) {
-    // rounds of blocks x (tiles of an item + its start, end and share of the join).  Candidates fill 1..8 rounds.
-    const int most = s.tx > 0 ? (kFsItemsPerSm * grid) / s.tx : 1;
-    float best = float((base + grid - 1) / grid) * (s.ty + 2.f);
-    for (int r = 1; r <= kFsItemsPerSm; ++r) {
-      int c = r * grid / base;
-      c = c < s.ty ? c : s.ty;
-      c = c < most ? c : most;
-      if (c <= 1) continue;
-      const int per = (s.ty + c - 1) / c, eff = (s.ty + per - 1) / per;
-      const float cost = float((base * eff + grid - 1) / grid) * (per + 5.f);
-      if (cost < best) {
-        best = cost;
-        s.splits = eff;
-        s.per = per;
-      }
-    }
-  }
-  s.items = base * s.splits;
-  return s;
-}
+// A block's share.  Every part of an item has a slot for partial results: whole items their own number, the parts of items left over
+// (number of whole items) + rel + run.
+struct FsWalk {
+  int block, grid, k = 0, item = 0, t0 = 0, nt = 0, slot = 0;
+  bool all = false;  // the item is not cut
+  int64_t at, end;
 
-// rows of partial results that any schedule for at most `nx` rows of X needs
-static int64_t fs_partial_rows(int64_t nx, int64_t ny, int grid) {
-  const int64_t tx = (nx + kFsTile - 1) / kFsTile, ty = std::max<int64_t>(1, (ny + kFsTile - 1) / kFsTile);
-  return std::max(tx, std::min<int64_t>(tx * ty, int64_t(kFsItemsPerSm) * grid)) * kFsTile;
-}
+  __device__ FsWalk(const FsSchedule& sc, int block_, int grid_) : block(block_), grid(grid_) {
+    at = int64_t(block) * sc.run;
+    end = min(at + sc.run, int64_t(sc.rest) * sc.steps);
+  }
+  __device__ bool next(const FsSchedule& sc) {
+    if (k < sc.whole) {
+      item = slot = k * grid + block;
+      ++k;
+      t0 = 0;
+      nt = sc.ty;
+      all = true;
+      return true;
+    }
+    if (at >= end) return false;
+    const int rel = int(at / sc.steps);
+    t0 = int(at - int64_t(rel) * sc.steps);
+    nt = int(min(int64_t(sc.steps - t0), end - at));
+    at += nt;
+    item = sc.whole * grid + rel;
+    slot = item + block;
+    all = nt == sc.steps;
+    nt = min(nt, sc.ty);  // no tiles at all: an item without terms
+    return true;
+  }
+};
 
 struct FsParams {
   const int* n_valid;      // rows of h that take part
@@ -106,9 +117,9 @@ struct FsParams {
   int grid;
   const int* target;       // [Ppad] targets of the compacted rows
   const float* bias;       // [Vpad] (-inf behind V), or null
-  float* part_acc;         // [splits, tx * 128, D]
-  float* part_m;           // [splits, 2, tx * 128]  running maximum (base 2) of a row's half tiles
-  float* part_l;           // [splits, 2, tx * 128]  sum; BWD: db
+  float* part_acc;         // [slots, 128, min(D, 256)]; BWD: of the items left over only
+  float* part_m;           // [slots, 2, 128]  reference (base 2) of either group of warps
+  float* part_l;           // [slots, 2, 128]  their sums; BWD: db
   float* zt;               // [Ppad] score of the target (base 2)
   const float* lse2;       // BWD [Ppad] (+inf behind n_valid)
   const float* wex;        // BWD [Ppad] 1 - p_t
@@ -192,7 +203,7 @@ full_softmax_kernel(const __grid_constant__ CUtensorMap tmapX, const __grid_cons
   const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   const int n_valid = __shfl_sync(0xffffffffu, *p.n_valid, 0);
   const int nx = MODE == FS_BWD ? p.V : n_valid, ny = MODE == FS_BWD ? n_valid : p.V;
-  const FsSchedule sc = fs_schedule(nx, ny, kAcc ? (p.D + kFsAcc - 1) / kFsAcc : 1, p.grid);
+  const FsSchedule sc(nx, ny, kAcc ? (p.D + kFsAcc - 1) / kFsAcc : 1, p.grid);
   // a unit of the ring: two blocks of 64 columns of a tile (one for rows of up to 64), or one block of a pair of tiles
   const int spu = kAcc && p.kb == 1 ? 1 : 2;               // its slots
   const int upt = kAcc ? (p.kb + spu - 1) / spu : p.kb;    // units of a streamed tile or pair
@@ -235,9 +246,7 @@ full_softmax_kernel(const __grid_constant__ CUtensorMap tmapX, const __grid_cons
   const uint32_t tmem = __shfl_sync(0xffffffffu, B->tmem_base, 0);
   bool ok = *abort_flag == 0;
 
-  // item -> (tile of X, piece of the accumulator's columns, split of the streamed axis).  The split is the slow index: blocks that run
-  // together stream the same tiles, which then come from L2.
-  const int base = sc.tx * sc.pieces;
+  FsWalk walk(sc, blockIdx.x, p.grid);
 
   if (warp == 0) {
     // ---------------- TMA producer ----------------
@@ -255,9 +264,8 @@ full_softmax_kernel(const __grid_constant__ CUtensorMap tmapX, const __grid_cons
         ++loads;
         return true;
       };
-      for (int w = blockIdx.x; w < sc.items && ok; w += gridDim.x, ++item) {
-        const int split = w / base, rem = w - split * base, x = rem % sc.tx, piece = rem / sc.tx;
-        const int t0 = split * sc.per, nt = min(sc.ty, t0 + sc.per) - t0;
+      for (; ok && walk.next(sc); ++item) {
+        const int x = walk.item % sc.tx, piece = walk.item / sc.tx, t0 = walk.t0, nt = walk.nt;
         if (p.x_resident && nt > 0) {
           if (item > 0 && !fs_wait(&B->x_empty, (item - 1) & 1, abort_flag, FS_ERR_X)) { ok = false; break; }
           mbar_expect_tx(&B->x_full, p.kb * kFsSlotBytes);
@@ -290,7 +298,7 @@ full_softmax_kernel(const __grid_constant__ CUtensorMap tmapX, const __grid_cons
         for (uint32_t j = loads > units ? loads - units : 0; j < loads; ++j)
           while (!mbar_try_wait(&B->full[j % units], (j / units) & 1) && clock64() - begin < kWaitCycles) {
           }
-        if (p.x_resident && item < uint32_t(sc.items))
+        if (p.x_resident)
           while (!mbar_try_wait(&B->x_full, item & 1) && clock64() - begin < kWaitCycles) {
           }
         if constexpr (MODE == FS_BWD)
@@ -324,9 +332,8 @@ full_softmax_kernel(const __grid_constant__ CUtensorMap tmapX, const __grid_cons
       const uint32_t n0 = min(64 * spu, (p.D + 15) / 16 * 16), n_all = (p.D + 15) / 16 * 16;
       const uint32_t idesc_0 = fs_idesc(n0, true), idesc_1 = fs_idesc(n_all > 128 ? n_all - 128 : 16, true), idesc_all = fs_idesc(n_all & 0x1ff, true);
       const bool two_units = upt == 2, slot_1 = p.kb > 1, slot_3 = p.kb > 3;
-      for (int w = blockIdx.x; w < sc.items && ok; w += gridDim.x, ++item) {
-        const int split = w / base, rem = w - split * base, piece = rem / sc.tx;
-        const int t0 = split * sc.per, nt = min(sc.ty, t0 + sc.per) - t0;
+      for (; ok && walk.next(sc); ++item) {
+        const int piece = walk.item / sc.tx, nt = walk.nt;
         if (p.x_resident && nt > 0 && !wait_all(&B->x_full, item & 1, FS_ERR_X)) { ok = false; break; }
         const int pu0 = piece * (kFsAcc / 128), pu1 = min(upt, pu0 + kFsAcc / 128);
         const int groups = (nt + kPair - 1) / kPair, ahead = kAcc ? int(bufs) - 1 : 0;
@@ -477,11 +484,10 @@ full_softmax_kernel(const __grid_constant__ CUtensorMap tmapX, const __grid_cons
     auto wait_all = [&](uint64_t* bar, uint32_t parity, int code) {
       return __all_sync(0xffffffffu, fs_wait(bar, parity, abort_flag, code)) != 0;
     };
-    for (int w = blockIdx.x; w < sc.items && ok; w += gridDim.x, ++item) {
-      const int split = w / base, rem = w - split * base, x = rem % sc.tx, piece = rem / sc.tx;
-      const int t0 = split * sc.per, nt = min(sc.ty, t0 + sc.per) - t0;
+    for (; ok && walk.next(sc); ++item) {
+      const int x = walk.item % sc.tx, piece = walk.item / sc.tx, t0 = walk.t0, nt = walk.nt;
       const int row = x * kFsTile + q * 32 + lane;  // FWD: compacted row of h; BWD: item
-      const int64_t prow = int64_t(sc.tx) * kFsTile;  // rows of one split's partial results
+      const int r128 = q * 32 + lane;
       int tgt = -1;
       float bias_row = 0.f;
       if constexpr (MODE == FS_BWD) {
@@ -715,8 +721,8 @@ full_softmax_kernel(const __grid_constant__ CUtensorMap tmapX, const __grid_cons
           m2 = mr;
         }
       }
-      if (piece == 0 && (MODE != FS_BWD || BIAS)) {
-        const int64_t at = (int64_t(split) * 2 + half) * prow + row;
+      if (MODE != FS_BWD || (BIAS && piece == 0)) {
+        const int64_t at = (int64_t(walk.slot) * 2 + half) * kFsTile + r128;
         p.part_l[at] = l;
         if constexpr (MODE != FS_BWD) p.part_m[at] = m2;
       }
@@ -726,7 +732,9 @@ full_softmax_kernel(const __grid_constant__ CUtensorMap tmapX, const __grid_cons
           tcgen05_fence_after();
         }
         const int width = min(kFsAcc, p.D - piece * kFsAcc);
-        const bool direct = MODE == FS_BWD && sc.splits == 1;
+        const bool direct = MODE == FS_BWD && walk.all;
+        const int acc_width = min(p.D, kFsAcc);
+        float* part = direct ? nullptr : p.part_acc + (int64_t(MODE == FS_BWD ? walk.slot - sc.whole * p.grid : walk.slot) * kFsTile + r128) * acc_width;
         float scale = 1.f;
         if (direct && !ROWG) scale = *p.dloss / (p.mean ? float(max(n_valid, 1)) : 1.f);
         for (int g = half; g * 32 < width; g += 2) {
@@ -746,7 +754,7 @@ full_softmax_kernel(const __grid_constant__ CUtensorMap tmapX, const __grid_cons
 #pragma unroll
             for (int k = 0; k < 8; ++k) v[k] = __uint_as_float(a[j + k]) * scale;
             if (!direct || p.dw_fp32) {
-              float* o = direct ? reinterpret_cast<float*>(p.dw) + int64_t(row) * p.D + c0 + j : p.part_acc + (int64_t(split) * prow + row) * p.D + c0 + j;
+              float* o = direct ? reinterpret_cast<float*>(p.dw) + int64_t(row) * p.D + c0 + j : part + g * 32 + j;
               *reinterpret_cast<float4*>(o) = make_float4(v[0], v[1], v[2], v[3]);
               *reinterpret_cast<float4*>(o + 4) = make_float4(v[4], v[5], v[6], v[7]);
             } else {
@@ -925,7 +933,7 @@ __global__ void __launch_bounds__(kPrepThreads) full_softmax_prep_kernel(const P
 }
 
 // ---- after the forward: join the splits of every row --------------------------------------------------
-// One block per row: the splits' weights 2^(m_s - max) go to shared memory, then the threads walk (group of splits, 4 columns).  The
+// One block per row: the weights 2^(m_s - max) of its item's parts go to shared memory, then the threads walk (group of parts, 4 columns).  The
 // block that finishes a tile of rows last adds up their losses, and the last of those the tiles', in a fixed order.
 constexpr int kJoinThreads = 128;
 static_assert(kJoinThreads == kFsTile, "a tile's losses are added up by one block, a row per thread");
@@ -946,7 +954,7 @@ struct JoinParams {
 
 template <bool ACC>
 __global__ void __launch_bounds__(kJoinThreads) full_softmax_join_kernel(const JoinParams p) {
-  extern __shared__ __align__(16) float js[];  // [splits] weights, then [threads * 4] partial sums
+  extern __shared__ __align__(16) float js[];  // [slots of an item] weights, then [threads * 4] partial sums
   const int n = p.st.counters[FS_N_VALID], row = blockIdx.x;
   const int padded = (n + kFsTile - 1) / kFsTile * kFsTile;
   if (row >= padded) return;
@@ -966,16 +974,27 @@ __global__ void __launch_bounds__(kJoinThreads) full_softmax_join_kernel(const J
   }
   const float z = p.zt[row];
   {
-    const FsSchedule sc = fs_schedule(n, p.V, p.pieces, p.grid);
-    const int64_t prow = int64_t(sc.tx) * kFsTile;
+    const FsSchedule sc(n, p.V, p.pieces, p.grid);
+    const int x = row / kFsTile, r128 = row % kFsTile, whole = sc.whole * p.grid;
+    // the slots of an item: count of them from the first
+    auto slots = [&](int item, int& first) {
+      if (item < whole) {
+        first = item;
+        return 1;
+      }
+      const int rel = item - whole, c0 = sc.first_run(rel);
+      first = item + c0;
+      return sc.last_run(rel) - c0 + 1;
+    };
+    int first, count = slots(x, first);
     float m = -INFINITY, l = 0.f;
-    for (int s = threadIdx.x; s < 2 * sc.splits; s += kJoinThreads) {
-      const float ms = p.part_m[s * prow + row], ls = p.part_l[s * prow + row];
+    for (int s = threadIdx.x; s < 2 * count; s += kJoinThreads) {
+      const int64_t at = (int64_t(first) * 2 + s) * kFsTile + r128;
+      const float ms = p.part_m[at], ls = p.part_l[at];
       const float mn = fmaxf(m, ms);
       if (mn != -INFINITY) l = l * exp2f(m - mn) + ls * exp2f(ms - mn);
       else l += ls;
       m = mn;
-      if (ACC && !(s & 1)) js[s >> 1] = ms;
     }
     const float mine = m;
     m = warp_max(m);
@@ -984,10 +1003,6 @@ __global__ void __launch_bounds__(kJoinThreads) full_softmax_join_kernel(const J
     m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
     const float ms = m == -INFINITY ? 0.f : m;
     l = block_sum(mine == -INFINITY ? l : l * exp2f(mine - ms));
-    if (ACC) {
-      for (int s = threadIdx.x; s < sc.splits; s += kJoinThreads) js[s] = exp2f(js[s] - ms);
-      __syncthreads();
-    }
     // others' log sum a, target's score z (base 2): lse = max + log2(1 + 2^-|a - z|)
     const float a = ms + log2f(l), d = a - z;
     const float tail = log1pf(exp2f(-fabsf(d)));
@@ -1000,42 +1015,43 @@ __global__ void __launch_bounds__(kJoinThreads) full_softmax_join_kernel(const J
       else p.loss_c[row] = loss;
     }
     if constexpr (ACC) {
-      float4* buf = reinterpret_cast<float4*>(js + ((sc.splits + 3) & ~3));
-      const int vecs = p.D / 4;
-      int lanes = 1;
-      while (lanes < vecs && lanes < kJoinThreads) lanes <<= 1;
-      const int groups = sc.splits > 1 ? kJoinThreads / lanes : 1;
-      const int g = threadIdx.x / lanes, c = threadIdx.x % lanes;
+      float4* buf = reinterpret_cast<float4*>(js + ((p.grid + 7) & ~3));
       const float inv = l > 0.f ? w / l : (l == 0.f ? 0.f : l);
       const int64_t t = p.st.target[row];
-      for (int v0 = 0; v0 < vecs; v0 += lanes) {
-        const int v = v0 + c;
+      const int acc_width = min(p.D, kFsAcc);
+      for (int piece = 0; piece < p.pieces; ++piece) {
+        // every piece was cut on its own
+        if (piece > 0) count = slots(piece * sc.tx + x, first);
+        __syncthreads();
+        for (int s = threadIdx.x; s < count; s += kJoinThreads) js[s] = exp2f(p.part_m[(int64_t(first) + s) * 2 * kFsTile + r128] - ms);
+        __syncthreads();
+        const int vecs = (min(p.D - piece * kFsAcc, kFsAcc)) / 4;  // at most 64
+        int lanes = 1;
+        while (lanes < vecs) lanes <<= 1;
+        const int groups = kJoinThreads / lanes, g = threadIdx.x / lanes, c = threadIdx.x % lanes;
         float4 s4 = f4zero();
-        if (v < vecs && g < groups)
-          for (int s = g; s < sc.splits; s += groups) {
-            const float4 x = *reinterpret_cast<const float4*>(p.part_acc + (s * prow + row) * p.D + v * 4);
+        if (c < vecs)
+          for (int s = g; s < count; s += groups) {
+            const float4 v = *reinterpret_cast<const float4*>(p.part_acc + ((int64_t(first) + s) * kFsTile + r128) * acc_width + c * 4);
             const float f = js[s];
-            s4.x += f * x.x;
-            s4.y += f * x.y;
-            s4.z += f * x.z;
-            s4.w += f * x.w;
+            s4.x += f * v.x;
+            s4.y += f * v.y;
+            s4.z += f * v.z;
+            s4.w += f * v.w;
           }
-        if (groups > 1) {
-          buf[threadIdx.x] = s4;
-          __syncthreads();
-          if (g == 0)
-            for (int k = 1; k < groups; ++k) {
-              const float4 x = buf[k * lanes + c];
-              s4.x += x.x;
-              s4.y += x.y;
-              s4.z += x.z;
-              s4.w += x.w;
-            }
-          __syncthreads();
-        }
-        if (g == 0 && v < vecs) {
-          const float4 wt = Vec4<__nv_bfloat16>::load(p.W + t * p.ldw + v * 4);
-          *reinterpret_cast<float4*>(p.st.unit + int64_t(row) * p.D + v * 4) =
+        buf[threadIdx.x] = s4;
+        __syncthreads();
+        if (g == 0 && c < vecs) {
+          for (int k = 1; k < min(groups, count); ++k) {
+            const float4 v = buf[k * lanes + c];
+            s4.x += v.x;
+            s4.y += v.y;
+            s4.z += v.z;
+            s4.w += v.w;
+          }
+          const int col = piece * kFsAcc + c * 4;
+          const float4 wt = Vec4<__nv_bfloat16>::load(p.W + t * p.ldw + col);
+          *reinterpret_cast<float4*>(p.st.unit + int64_t(row) * p.D + col) =
               make_float4(s4.x * inv - w * wt.x, s4.y * inv - w * wt.y, s4.z * inv - w * wt.z, s4.w * inv - w * wt.w);
         }
       }
@@ -1126,28 +1142,41 @@ __global__ void __launch_bounds__(256) full_softmax_finish_kernel(const FinishPa
     }
   }
   if (p.part_acc == nullptr && p.db == nullptr) return;
-  const FsSchedule sc = fs_schedule(p.V, n, p.pieces, p.grid);
-  const int64_t prow = int64_t(sc.tx) * kFsTile;
-  if (p.part_acc != nullptr && sc.splits > 1) {
-    for (int64_t i = me; i < int64_t(p.V) * vecs; i += step) {
+  const FsSchedule sc(p.V, n, p.pieces, p.grid);
+  const int whole = sc.whole * p.grid;
+  if (p.part_acc != nullptr) {
+    // items left over that were cut (the others were written by the main kernel)
+    const int acc_width = min(p.Dp, kFsAcc), wv = acc_width / 8;
+    for (int64_t i = me; i < int64_t(sc.rest) * kFsTile * wv; i += step) {
+      const int c = int(i % wv) * 8, r128 = int(i / wv % kFsTile), rel = int(i / wv / kFsTile);
+      const int c0 = sc.first_run(rel), c1 = sc.last_run(rel), item = whole + rel, x = item % sc.tx, piece = item / sc.tx;
+      const int64_t row = int64_t(x) * kFsTile + r128;
+      if (c0 == c1 || row >= p.V || piece * kFsAcc + c >= p.Dp) continue;
       float v[8];
 #pragma unroll
       for (int k = 0; k < 8; ++k) v[k] = 0.f;
-      for (int s = 0; s < sc.splits; ++s) {
-        const float4* x = reinterpret_cast<const float4*>(p.part_acc + s * prow * p.Dp + i * 8);
-        const float4 a = x[0], b = x[1];
+      for (int s = c0; s <= c1; ++s) {
+        const float4* x4 = reinterpret_cast<const float4*>(p.part_acc + (int64_t(rel + s) * kFsTile + r128) * acc_width + c);
+        const float4 a = x4[0], b = x4[1];
         v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
         v[4] += b.x; v[5] += b.y; v[6] += b.z; v[7] += b.w;
       }
 #pragma unroll
       for (int k = 0; k < 8; ++k) v[k] *= g_all;
-      fs_store8(reinterpret_cast<TW*>(p.dw) + i * 8, v);
+      fs_store8(reinterpret_cast<TW*>(p.dw) + row * p.Dp + piece * kFsAcc + c, v);
     }
   }
   if (p.db != nullptr)
     for (int64_t v = me; v < p.V; v += step) {
+      const int item = int(v / kFsTile), r128 = int(v % kFsTile);
+      int first = item, count = 1;
+      if (item >= whole) {
+        const int c0 = sc.first_run(item - whole);
+        first = item + c0;
+        count = sc.last_run(item - whole) - c0 + 1;
+      }
       float s = 0.f;
-      for (int k = 0; k < 2 * sc.splits; ++k) s += p.part_l[k * prow + v];
+      for (int k = 0; k < 2 * count; ++k) s += p.part_l[(int64_t(first) * 2 + k) * kFsTile + r128];
       s *= g_all;
       if (p.db_bf16) reinterpret_cast<__nv_bfloat16*>(p.db)[v] = __float2bfloat16(s);
       else reinterpret_cast<float*>(p.db)[v] = s;
@@ -1220,10 +1249,10 @@ std::tuple<at::Tensor, at::Tensor> full_softmax_fwd(const at::Tensor& h, const a
   }
   const int grid = fs_grid(h.device());
   const int pieces = acc ? int((Dp + kFsAcc - 1) / kFsAcc) : 1;
-  const int64_t prows = fs_partial_rows(P, V, grid);
-  at::Tensor part = at::empty({(acc ? prows * Dp : 0) + 4 * prows + 2 * Ppad + Ppad / kFsTile}, f32);  // accumulators, maxima, sums, targets' scores, losses
+  const int64_t prows = (Ppad / kFsTile * pieces + grid) * kFsTile, n_acc = acc ? prows * std::min<int64_t>(Dp, kFsAcc) : 0;  // rows of all slots
+  at::Tensor part = at::empty({n_acc + 4 * prows + 2 * Ppad + Ppad / kFsTile}, f32);  // accumulators, references, sums, targets' scores, losses
   float* part_acc = part.data_ptr<float>();
-  float* part_m = part_acc + (acc ? prows * Dp : 0);
+  float* part_m = part_acc + n_acc;
   float* part_l = part_m + 2 * prows;
   float* zt = part_l + 2 * prows;
   float* loss_c = zt + Ppad;
@@ -1257,7 +1286,7 @@ std::tuple<at::Tensor, at::Tensor> full_softmax_fwd(const at::Tensor& h, const a
   else has_bias ? fs_launch<FS_LSE, true, false>(tx, ty, p, dev) : fs_launch<FS_LSE, false, false>(tx, ty, p, dev);
   const JoinParams j{st, int(V), int(Dp), grid, pieces, int(reduction), part_acc, part_m, part_l, zt, loss_c, loss_c + Ppad, reinterpret_cast<const __nv_bfloat16*>(weight.data_ptr()),
                      weight.stride(0), loss.data_ptr<float>()};
-  const int smem = (kFsItemsPerSm * grid + 8) * 4 + kJoinThreads * 16;
+  const int smem = (grid + 8) * 4 + kJoinThreads * 16;
   if (acc) full_softmax_join_kernel<true><<<unsigned(Ppad), kJoinThreads, smem, stream>>>(j);
   else full_softmax_join_kernel<false><<<unsigned(Ppad), kJoinThreads, 0, stream>>>(j);
   TRB_CUDA_CHECK(cudaGetLastError());
@@ -1294,9 +1323,10 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> full_softmax_bwd(const at::Tensor
   const int grid = fs_grid(device), dev = device.index();
   const bool per_row = reduction == 0, mean = reduction == 1;
   const int pieces = int((Dp + kFsAcc - 1) / kFsAcc);
-  const int64_t prows = fs_partial_rows(V, P, grid);
-  const bool may_split = main && int64_t(kFsItemsPerSm) * grid / (Vpad / kFsTile) > 1 && Ppad > kFsTile;  // mirrors fs_schedule
-  const int64_t n_acc = may_split ? prows * Dp : 0, n_l = main && has_bias ? 2 * prows : 0, n_g = main && per_row ? Ppad : 0;
+  const int64_t items = Vpad / kFsTile * pieces, rest = items % grid;
+  const bool may_split = main && rest > 0 && Ppad > kFsTile;  // items left over, of more than one tile
+  const int64_t n_acc = may_split ? (rest + grid) * kFsTile * std::min<int64_t>(Dp, kFsAcc) : 0, n_l = main && has_bias ? 2 * (items + grid) * kFsTile : 0,
+                n_g = main && per_row ? Ppad : 0;
   at::Tensor part = n_acc + n_l + n_g > 0 ? at::empty({n_acc + n_l + n_g}, f32) : at::Tensor();
   float* part_acc = n_acc ? part.data_ptr<float>() : nullptr;
   float* part_l = n_l ? part.data_ptr<float>() + n_acc : nullptr;
@@ -1329,7 +1359,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> full_softmax_bwd(const at::Tensor
   if (want_h || want_b || may_split) {
     const FinishParams f{st, int(P), int(V), int(D), int(Dp), grid, pieces, per_row, mean, dloss.data_ptr<float>(), per_row ? dloss.stride(0) : 0, part_acc, part_l,
                          want_h ? dh.data_ptr() : nullptr, dw.data_ptr(), want_b ? db.data_ptr() : nullptr, !db_fp32};
-    const int64_t most = std::max<int64_t>({want_h ? P * (Dp / 8) : 0, may_split ? V * (Dp / 8) : 0, want_b ? V : 0});
+    const int64_t most = std::max<int64_t>({want_h ? P * (Dp / 8) : 0, n_acc / 8, want_b ? V : 0});
     const unsigned blocks = unsigned(std::min<int64_t>((most + 255) / 256, 16 * grid));
     if (dh_fp32) dw_fp32 ? full_softmax_finish_kernel<float, float><<<blocks, 256, 0, stream>>>(f) : full_softmax_finish_kernel<float, __nv_bfloat16><<<blocks, 256, 0, stream>>>(f);
     else dw_fp32 ? full_softmax_finish_kernel<__nv_bfloat16, float><<<blocks, 256, 0, stream>>>(f)

@@ -55,6 +55,26 @@ enum FsErr : int { FS_ERR_EMPTY = 1, FS_ERR_FULL = 2, FS_ERR_X = 3, FS_ERR_S = 4
 
 __device__ int g_fs_error = 0;  // one word per device; never allocated, so it may first be touched inside a graph capture
 
+// The kernels of a call are launched so that the next one may begin (and set itself up) before the one in front has ended; what that one
+// wrote is read behind fs_after.  fs_let_next allows the next kernel's blocks in as soon as all of this kernel's have started.
+__device__ __forceinline__ void fs_after() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void fs_let_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+template <typename Kernel, typename... Args>
+static void fs_launch_next(Kernel kernel, unsigned grid, unsigned threads, size_t smem, cudaStream_t stream, Args... args) {
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3(grid);
+  config.blockDim = dim3(threads);
+  config.dynamicSmemBytes = smem;
+  config.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = &attr;
+  config.numAttrs = 1;
+  TRB_CUDA_CHECK(cudaLaunchKernelEx(&config, kernel, args...));
+}
+
 // How the work is dealt to the blocks.  An item is a tile of X and a piece of the accumulator's columns; it streams `ty` tiles of Y.  Every
 // block takes the same number of whole items, and what is left over (fewer items than blocks) is cut along the streamed axis into one equal
 // run per block, which may cross from one item into the next: with whole items alone 313 items keep 148 SMs busy 70 % of the time.
@@ -201,9 +221,6 @@ full_softmax_kernel(const __grid_constant__ CUtensorMap tmapX, const __grid_cons
   volatile int* abort_flag = &B->abort_flag;
   // values that are alike in a warp are taken from lane 0, which tells the compiler so
   const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
-  const int n_valid = __shfl_sync(0xffffffffu, *p.n_valid, 0);
-  const int nx = MODE == FS_BWD ? p.V : n_valid, ny = MODE == FS_BWD ? n_valid : p.V;
-  const FsSchedule sc(nx, ny, kAcc ? (p.D + kFsAcc - 1) / kFsAcc : 1, p.grid);
   // a unit of the ring: two blocks of 64 columns of a tile (one for rows of up to 64), or one block of a pair of tiles
   const int spu = kAcc && p.kb == 1 ? 1 : 2;               // its slots
   const int upt = kAcc ? (p.kb + spu - 1) / spu : p.kb;    // units of a streamed tile or pair
@@ -243,6 +260,10 @@ full_softmax_kernel(const __grid_constant__ CUtensorMap tmapX, const __grid_cons
   tcgen05_fence_before();
   __syncthreads();
   tcgen05_fence_after();
+  fs_after();
+  const int n_valid = __shfl_sync(0xffffffffu, *p.n_valid, 0);
+  const int nx = MODE == FS_BWD ? p.V : n_valid, ny = MODE == FS_BWD ? n_valid : p.V;
+  const FsSchedule sc(nx, ny, kAcc ? (p.D + kFsAcc - 1) / kFsAcc : 1, p.grid);
   const uint32_t tmem = __shfl_sync(0xffffffffu, B->tmem_base, 0);
   bool ok = *abort_flag == 0;
 
@@ -849,6 +870,7 @@ __device__ __forceinline__ int64_t fs_target(int64_t i, const PrepParams& p) {
 __device__ __forceinline__ int64_t fs_target_kind(int64_t t, const PrepParams& p) { return t == p.ignore ? 0 : (t < 0 || t >= p.V ? int64_t(1) << 32 : 1); }
 
 __global__ void __launch_bounds__(kPrepThreads) full_softmax_prep_kernel(const PrepParams p) {
+  fs_let_next();
   if (int(blockIdx.x) >= p.row_blocks) {
     const int64_t vpad = (int64_t(p.V) + kFsTile - 1) / kFsTile * kFsTile;
     for (int64_t v = int64_t(blockIdx.x - p.row_blocks) * kPrepThreads + threadIdx.x; v < vpad; v += int64_t(gridDim.x - p.row_blocks) * kPrepThreads)
@@ -955,7 +977,8 @@ struct JoinParams {
 template <bool ACC>
 __global__ void __launch_bounds__(kJoinThreads) full_softmax_join_kernel(const JoinParams p) {
   extern __shared__ __align__(16) float js[];  // [slots of an item] weights, then [threads * 4] partial sums
-  const int n = p.st.counters[FS_N_VALID], row = blockIdx.x;
+  fs_after();
+  const int n = p.st.counters[FS_N_VALID], n_bad = p.st.counters[FS_N_BAD], row = blockIdx.x;
   const int padded = (n + kFsTile - 1) / kFsTile * kFsTile;
   if (row >= padded) return;
   __shared__ float red[kJoinThreads / 32];
@@ -1080,7 +1103,7 @@ __global__ void __launch_bounds__(kJoinThreads) full_softmax_join_kernel(const J
     for (int k = threadIdx.x; k < tiles; k += kJoinThreads) s += __ldcg(p.tile_loss + k);
     s = block_sum(s);
   }
-  if (threadIdx.x == 0) *p.loss = p.st.counters[FS_N_BAD] > 0 ? __int_as_float(0x7fc00000) : (p.reduction == 1 ? s / float(n) : s);
+  if (threadIdx.x == 0) *p.loss = n_bad > 0 ? __int_as_float(0x7fc00000) : (p.reduction == 1 ? s / float(n) : s);
 }
 
 // ---- backward ---------------------------------------------------------------------------------------------
@@ -1116,6 +1139,7 @@ __device__ __forceinline__ void fs_store8(T* o, const float (&v)[8]) {
 // dh = g * unit at the rows' own places; the splits of dW and db joined in their order
 template <typename TH, typename TW>
 __global__ void __launch_bounds__(256) full_softmax_finish_kernel(const FinishParams p) {
+  fs_after();
   const int n = p.st.counters[FS_N_VALID], vecs = p.Dp / 8;
   const int64_t step = int64_t(gridDim.x) * blockDim.x, me = int64_t(blockIdx.x) * blockDim.x + threadIdx.x;
   const float g_all = p.per_row ? 1.f : *p.dloss / (p.mean ? float(max(n, 1)) : 1.f);
@@ -1194,8 +1218,7 @@ static void fs_launch(const CUtensorMap& tx, const CUtensorMap& ty, const FsPara
     TRB_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kFsSmem));
     if (device < 64) set[device] = true;
   }
-  kernel<<<p.grid, kFsThreads, kFsSmem, at::cuda::getCurrentCUDAStream()>>>(tx, ty, p);
-  TRB_CUDA_CHECK(cudaGetLastError());
+  fs_launch_next(kernel, p.grid, kFsThreads, kFsSmem, at::cuda::getCurrentCUDAStream(), tx, ty, p);
 }
 
 static void fs_shape(FsParams& p, int64_t V, int64_t D, bool acc) {
@@ -1287,9 +1310,8 @@ std::tuple<at::Tensor, at::Tensor> full_softmax_fwd(const at::Tensor& h, const a
   const JoinParams j{st, int(V), int(Dp), grid, pieces, int(reduction), part_acc, part_m, part_l, zt, loss_c, loss_c + Ppad, reinterpret_cast<const __nv_bfloat16*>(weight.data_ptr()),
                      weight.stride(0), loss.data_ptr<float>()};
   const int smem = (grid + 8) * 4 + kJoinThreads * 16;
-  if (acc) full_softmax_join_kernel<true><<<unsigned(Ppad), kJoinThreads, smem, stream>>>(j);
-  else full_softmax_join_kernel<false><<<unsigned(Ppad), kJoinThreads, 0, stream>>>(j);
-  TRB_CUDA_CHECK(cudaGetLastError());
+  if (acc) fs_launch_next(full_softmax_join_kernel<true>, unsigned(Ppad), kJoinThreads, smem, stream, j);
+  else fs_launch_next(full_softmax_join_kernel<false>, unsigned(Ppad), kJoinThreads, 0, stream, j);
   return {loss, state};
 }
 
@@ -1361,10 +1383,14 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> full_softmax_bwd(const at::Tensor
                          want_h ? dh.data_ptr() : nullptr, dw.data_ptr(), want_b ? db.data_ptr() : nullptr, !db_fp32};
     const int64_t most = std::max<int64_t>({want_h ? P * (Dp / 8) : 0, n_acc / 8, want_b ? V : 0});
     const unsigned blocks = unsigned(std::min<int64_t>((most + 255) / 256, 16 * grid));
-    if (dh_fp32) dw_fp32 ? full_softmax_finish_kernel<float, float><<<blocks, 256, 0, stream>>>(f) : full_softmax_finish_kernel<float, __nv_bfloat16><<<blocks, 256, 0, stream>>>(f);
-    else dw_fp32 ? full_softmax_finish_kernel<__nv_bfloat16, float><<<blocks, 256, 0, stream>>>(f)
-                 : full_softmax_finish_kernel<__nv_bfloat16, __nv_bfloat16><<<blocks, 256, 0, stream>>>(f);
-    TRB_CUDA_CHECK(cudaGetLastError());
+    auto finish = dh_fp32 ? (dw_fp32 ? full_softmax_finish_kernel<float, float> : full_softmax_finish_kernel<float, __nv_bfloat16>)
+                          : (dw_fp32 ? full_softmax_finish_kernel<__nv_bfloat16, float> : full_softmax_finish_kernel<__nv_bfloat16, __nv_bfloat16>);
+    if (main) {
+      fs_launch_next(finish, blocks, 256, 0, stream, f);
+    } else {
+      finish<<<blocks, 256, 0, stream>>>(f);
+      TRB_CUDA_CHECK(cudaGetLastError());
+    }
   }
   return {dh, dw, db};
 }

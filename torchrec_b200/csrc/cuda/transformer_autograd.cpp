@@ -1,6 +1,6 @@
 // Autograd nodes of the transformer operators in C++.  For the smallest calls - one position scored, one token turned - the kernels take
 // a few microseconds and the call is bound by the host: a node here saves the interpreter's share of the forward and the backward
-// (one step of 260 rows x 20000 classes x 64 went from 152 to 92 us, a rotation step of 7000 tokens from 131 to 84 us).
+// (a step of 260 rows x 20000 classes x 64 went from 152 to 92 us, a rotation step of 7000 tokens from 131 to 84 us).
 #include <ATen/ATen.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -86,18 +86,22 @@ static void check_full_softmax(const Tensor& h, const Tensor& weight, const c10:
   TORCH_CHECK_VALUE(targets.device() == h.device(), "full_softmax_loss: targets is on ", targets.device(), ", h on ", h.device());
 }
 
-static Tensor full_softmax_loss_autograd(const Tensor& h, const Tensor& weight, const c10::optional<Tensor>& bias, const Tensor& targets, const c10::optional<Tensor>& rounded,
-                                         int64_t ignore_index, int64_t reduction) {
-  check_full_softmax(h, weight, bias, targets);
-  int64_t grad = 0;
-  if (at::GradMode::is_enabled()) grad = h.requires_grad() ? 2 : int64_t(weight.requires_grad() || (bias.has_value() && bias->defined() && bias->requires_grad()));
-  return FullSoftmaxLoss::apply(h, weight, bias, targets, rounded, ignore_index, reduction, grad);
-}
-
 static Tensor full_softmax_loss_plain(const Tensor& h, const Tensor& weight, const c10::optional<Tensor>& bias, const Tensor& targets, const c10::optional<Tensor>& rounded,
                                       int64_t ignore_index, int64_t reduction) {
   check_full_softmax(h, weight, bias, targets);
   return std::get<0>(full_softmax_fwd(h, kernel_rows(weight, rounded), targets, bias, ignore_index, reduction, 0));
+}
+
+static Tensor full_softmax_loss_autograd(const Tensor& h, const Tensor& weight, const c10::optional<Tensor>& bias, const Tensor& targets, const c10::optional<Tensor>& rounded,
+                                         int64_t ignore_index, int64_t reduction) {
+  int64_t grad = 0;
+  if (at::GradMode::is_enabled()) grad = h.requires_grad() ? 2 : int64_t(weight.requires_grad() || (bias.has_value() && bias->defined() && bias->requires_grad()));
+  if (grad == 0) {  // no node
+    at::AutoDispatchBelowADInplaceOrView below;
+    return full_softmax_loss_plain(h, weight, bias, targets, rounded, ignore_index, reduction);
+  }
+  check_full_softmax(h, weight, bias, targets);
+  return FullSoftmaxLoss::apply(h, weight, bias, targets, rounded, ignore_index, reduction, grad);
 }
 
 // ---- norm and rotation of queries and keys ------------------------------------------------------------------
@@ -178,16 +182,21 @@ static Tensor check_rotary(const Tensor& qkv, const c10::optional<Tensor>& qw, c
 
 static Tensor frequencies(const Tensor& f) { return f.detach().to(at::kDouble).contiguous(); }
 
-static Tensor qk_norm_rotary_autograd(const Tensor& qkv, const Tensor& positions, const Tensor& inv_freq, const c10::optional<Tensor>& qw, const c10::optional<Tensor>& kw,
-                                      at::IntArrayRef sections, int64_t heads, int64_t kv_heads, double eps, bool norm, bool interleaved) {
-  const Tensor pos = check_rotary(qkv, qw, kw, positions, inv_freq, sections, heads, kv_heads, eps);
-  return QKNormRotary::apply(qkv, qw, kw, pos, frequencies(inv_freq), sections, heads, kv_heads, eps, norm, interleaved);
-}
-
 static Tensor qk_norm_rotary_plain(const Tensor& qkv, const Tensor& positions, const Tensor& inv_freq, const c10::optional<Tensor>& qw, const c10::optional<Tensor>& kw,
                                    at::IntArrayRef sections, int64_t heads, int64_t kv_heads, double eps, bool norm, bool interleaved) {
   const Tensor pos = check_rotary(qkv, qw, kw, positions, inv_freq, sections, heads, kv_heads, eps);
   return qk_norm_rotary_fwd(rows16(qkv), pos, frequencies(inv_freq), fp32(qw), fp32(kw), sections, heads, kv_heads, eps, norm, interleaved);
+}
+
+static Tensor qk_norm_rotary_autograd(const Tensor& qkv, const Tensor& positions, const Tensor& inv_freq, const c10::optional<Tensor>& qw, const c10::optional<Tensor>& kw,
+                                      at::IntArrayRef sections, int64_t heads, int64_t kv_heads, double eps, bool norm, bool interleaved) {
+  auto wants = [](const c10::optional<Tensor>& t) { return t.has_value() && t->defined() && t->requires_grad(); };
+  if (!at::GradMode::is_enabled() || !(qkv.requires_grad() || wants(qw) || wants(kw))) {  // no node
+    at::AutoDispatchBelowADInplaceOrView below;
+    return qk_norm_rotary_plain(qkv, positions, inv_freq, qw, kw, sections, heads, kv_heads, eps, norm, interleaved);
+  }
+  const Tensor pos = check_rotary(qkv, qw, kw, positions, inv_freq, sections, heads, kv_heads, eps);
+  return QKNormRotary::apply(qkv, qw, kw, pos, frequencies(inv_freq), sections, heads, kv_heads, eps, norm, interleaved);
 }
 
 }  // namespace trb

@@ -18,7 +18,7 @@ from typing import Optional, Sequence, Tuple
 
 import torch
 
-from torchrec_b200.ops import _ext
+from torchrec_b200.ops import _ext, dense_ops
 
 _seed_counter = itertools.count(0x5EED)
 
@@ -386,8 +386,6 @@ def full_softmax_loss(h: torch.Tensor, weight: torch.Tensor, targets: torch.Tens
     if reduction not in _REDUCTIONS:
         raise ValueError(f"full_softmax_loss: reduction is one of {sorted(_REDUCTIONS)}, got {reduction!r}")
     if h.is_cuda and h.dim() == 2 and h.shape[1] <= FULL_SOFTMAX_MAX_DIM and weight.dtype in _KERNEL_TYPES and (bias is None or bias.dtype in _KERNEL_TYPES):
-        from torchrec_b200.ops import dense_ops
-
         if (h.dtype == torch.bfloat16 or (h.dtype == torch.float32 and dense_ops.fused_dense_enabled(h))) and _ext.use_cuda_kernel(h, "full_softmax_loss"):
             # fp32 parameters go through the cache that the dense layers use: rounded once per optimizer step
             rounded = dense_ops.bf16_cache.get(weight) if weight.dtype == torch.float32 and weight.is_cuda and isinstance(weight, torch.nn.Parameter) else None

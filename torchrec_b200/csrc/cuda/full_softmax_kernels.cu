@@ -21,9 +21,9 @@
 // All sums run in a fixed order: pieces of the streamed axis go to a workspace and are joined by a second kernel.
 // Every wait is bounded (tcgen05.cuh); a block that gives up raises an error word and returns.
 //
-// Measured (B200, 18944 rows x 40000 classes, whole forward or backward): D = 256 forward with dh 640 us (1.21 PFLOP/s), backward 566 us
-// (1.37), value only 380 us (1.02); D = 64 420, 310 and 336 us, where the 16384 exponentials of a tile take 1.0 to 1.3 us; D = 512 (half the
-// rows) 980, 912 and 286 us, with the scores computed once per 256 columns.  At 16384 x 131071 x 256 a step takes 4.25 ms: 8 P V D at 1.04
+// Measured (B200, 18944 rows x 40000 classes, whole forward or backward): D = 256 forward with dh 644 us (1.20 PFLOP/s), backward 557 us
+// (1.39), value only 370 us (1.05); D = 64 422, 311 and 336 us, where the 16384 exponentials of a tile take 1.0 to 1.3 us; D = 512 (half the
+// rows) 881, 831 and 276 us, with the scores computed once per 256 columns.  At 16384 x 131071 x 256 a step takes 4.21 ms: 8 P V D at 1.04
 // PFLOP/s under the power cap (the library product alone sustains 1.40).  What bounds it: the score product reads both operands from
 // shared memory, which also receives the streamed tile; for narrow rows the softmax warps, at 60 % of the special-function rate (neither
 // more warps, nor paired arithmetic, nor a polynomial for a part of the exponentials changed that).
@@ -421,7 +421,11 @@ full_softmax_kernel(const __grid_constant__ CUtensorMap tmapX, const __grid_cons
           }
           continue;
         }
-        for (int t = 0; t < groups + ahead && ok; ++t) {
+        // wider rows, or no accumulator: blocks are given back as soon as they were multiplied, and loaded again for the accumulator
+        const uint32_t n_first = min(128, (p.D - pu0 * 128 + 15) / 16 * 16), n_second = min(128, (p.D - pu0 * 128 - 128 + 15) / 16 * 16);
+        const uint32_t idesc_first = fs_idesc(n_first, true), idesc_second = fs_idesc(n_second, true);
+        const bool second = pu1 - pu0 == 2;
+        for (int t = 0; t < groups + ahead; ++t) {
           if (t < groups) {
             // the buffer's previous tile: with ACC its E was consumed by an MMA issued before this one; without, its readers must be done
             if constexpr (!kAcc) {
@@ -429,8 +433,8 @@ full_softmax_kernel(const __grid_constant__ CUtensorMap tmapX, const __grid_cons
               tcgen05_fence_after();
             }
             const uint32_t d = tmem + sb * kFsTile;
+            uint64_t dx = desc_k + x16;
             for (int u = 0; u < upt; ++u) {
-              uint64_t dx = desc_k + x16 + u * (kAcc ? unit16 : kSlot16);
               const uint32_t xs = r.stage;
               if (!p.x_resident) {
                 if (!wait_all(&B->full[xs], r.phase, FS_ERR_FULL)) { ok = false; break; }
@@ -441,22 +445,11 @@ full_softmax_kernel(const __grid_constant__ CUtensorMap tmapX, const __grid_cons
               if (!wait_all(&B->full[ys], r.phase, FS_ERR_FULL)) { ok = false; break; }
               r.next();
               const uint64_t dy = desc_k + ring16 + ys * unit16;
-              const int steps = kAcc ? min(4 * spu, (p.D - u * spu * 64 + 15) / 16) : min(4, (p.D - u * 64 + 15) / 16);  // 16 columns each
-              if (steps == (kAcc ? 8 : 4)) {
-#pragma unroll
-                for (int i = 0; i < (kAcc ? 8 : 4); ++i) {
-                  const uint32_t off = (i >> 2) * kSlot16 + (i & 3) * 2;
-                  umma_bf16_by(leader, d, dx + off, dy + off, idesc_s, (i > 0 || u > 0) ? 1u : 0u);
-                }
-              } else {
-#pragma unroll 1
-                for (int i = 0; i < steps; ++i) {
-                  const uint32_t off = (i >> 2) * kSlot16 + (i & 3) * 2;
-                  umma_bf16_by(leader, d, dx + off, dy + off, idesc_s, (i > 0 || u > 0) ? 1u : 0u);
-                }
-              }
+              score_block(d, dx, dy, u == 0);
+              if (kAcc && 2 * u + 1 < p.kb) score_block(d, dx + kSlot16, dy + kSlot16, false);
               if (!p.x_resident) tcgen05_commit_by(leader, &B->empty[xs]);
               tcgen05_commit_by(leader, &B->empty[ys]);
+              dx += kAcc ? unit16 : kSlot16;
             }
             if (!ok) break;
             tcgen05_commit_by(leader, &B->s_full[sb]);
@@ -469,23 +462,26 @@ full_softmax_kernel(const __grid_constant__ CUtensorMap tmapX, const __grid_cons
             }
           }
           if (kAcc && t >= ahead) {
-            const bool first = t == ahead;
-            if (first && item > 0 && !wait_all(&B->o_empty, (item - 1) & 1, FS_ERR_ACC)) { ok = false; break; }
+            const uint32_t more = t == ahead ? 0u : 1u;
+            if (more == 0 && item > 0 && !wait_all(&B->o_empty, (item - 1) & 1, FS_ERR_ACC)) { ok = false; break; }
             if (!wait_all(&B->p_full[eb], eb_phase, FS_ERR_P)) { ok = false; break; }
             tcgen05_fence_after();
             const uint32_t e = tmem + eb * kFsTile;
-            for (int u = pu0; u < pu1; ++u) {
-              const uint32_t ys = r.stage;
-              if (!wait_all(&B->full[ys], r.phase, FS_ERR_FULL)) { ok = false; break; }
-              r.next();
-              const int n = min(64 * spu, (p.D - u * 64 * spu + 15) / 16 * 16);
-              const uint32_t idesc = fs_idesc(n, true), d = tmem + o_col + (u - pu0) * 128;
-              const uint64_t dy = desc_mn + ring16 + ys * unit16;
+            if (!wait_all(&B->full[r.stage], r.phase, FS_ERR_FULL)) { ok = false; break; }
+            uint64_t dy = desc_mn + ring16 + r.stage * unit16;
 #pragma unroll
-              for (int i = 0; i < 8; ++i) umma_bf16_ts_by(leader, d, e + i * 8, dy + i * 128, idesc, (i > 0 || !first) ? 1u : 0u);
-              tcgen05_commit_by(leader, &B->empty[ys]);
+            for (int i = 0; i < 8; ++i) umma_bf16_ts_by(leader, tmem + o_col, e + i * 8, dy + i * 128, idesc_first, i > 0 ? 1u : more);
+            tcgen05_commit_by(leader, &B->empty[r.stage]);
+            r.next();
+            if (second) {
+              if (!wait_all(&B->full[r.stage], r.phase, FS_ERR_FULL)) { ok = false; break; }
+              dy = desc_mn + ring16 + r.stage * unit16;
+#pragma unroll
+              for (int i = 0; i < 8; ++i) umma_bf16_ts_by(leader, tmem + o_col + 128, e + i * 8, dy + i * 128, idesc_second, i > 0 ? 1u : more);
+              tcgen05_commit_by(leader, &B->empty[r.stage]);
+              r.next();
             }
-            if (ok) tcgen05_commit_by(leader, &B->acc_done[tc & 3]);
+            tcgen05_commit_by(leader, &B->acc_done[tc & 3]);
             ++tc;
             if (++eb == bufs) {
               eb = 0;

@@ -49,7 +49,7 @@ constexpr int kFsSlots = 14;                        // X and the ring of streame
 constexpr int kFsMaxUnits = 13;
 constexpr int kFsMaxD = 1024;
 constexpr int kFsAcc = 256;                         // accumulator columns
-constexpr int kFsExtra = 3 * 1024;                     // per-column values of a tile, exchange of maxima, barriers
+constexpr int kFsExtra = 3 * 1024;                  // per-column values of a tile, exchange of maxima, barriers
 constexpr int kFsSmem = kFsSlots * kFsSlotBytes + kFsExtra;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -544,7 +544,7 @@ full_softmax_kernel(const __grid_constant__ CUtensorMap tmapX, const __grid_cons
         tmem_ld_32x32_issue(ts, r);
         if constexpr (MODE == FS_BWD) {
           const int v0 = x * kFsTile + q * 32;
-          int tg = __ldg(p.target + col0 + lane);  // targets of 32 rows of h, one per lane
+          int tg = p.target[col0 + lane];  // targets of 32 rows of h, one per lane
           const uint32_t cb = tc & (kCols - 1);
           if (!wait_all(&B->c_full[cb], (tc >> kColShift) & 1, FS_ERR_COL)) { ok = false; break; }
 #pragma unroll 1
@@ -567,7 +567,7 @@ full_softmax_kernel(const __grid_constant__ CUtensorMap tmapX, const __grid_cons
             const int tg_now = tg;
             if (c < 3) {
               tmem_ld_32x32_issue(ts + (c + 1) * 32, r);
-              tg = __ldg(p.target + col0 + (c + 1) * 32 + lane);
+              tg = p.target[col0 + (c + 1) * 32 + lane];
             }
 #pragma unroll
             for (int j = 0; j < 32; ++j) z[j] = fs_ex2(z[j]);
@@ -575,7 +575,7 @@ full_softmax_kernel(const __grid_constant__ CUtensorMap tmapX, const __grid_cons
               const int j = __ffs(hits) - 1;
               hits &= hits - 1;
               if (__shfl_sync(0xffffffffu, tg_now, j) == v0 + lane) {
-                const float v = -__ldg(p.wex + col0 + c * 32 + j);
+                const float v = -p.wex[col0 + c * 32 + j];
 #pragma unroll
                 for (int k = 0; k < 32; ++k) z[k] = k == j ? v : z[k];
               }
@@ -639,7 +639,7 @@ full_softmax_kernel(const __grid_constant__ CUtensorMap tmapX, const __grid_cons
               const float4* bp = reinterpret_cast<const float4*>(p.bias + col0 + c * 32);
 #pragma unroll
               for (int j = 0; j < 8; ++j) {
-                const float4 v = __ldg(bp + j);
+                const float4 v = bp[j];  // (written by the kernel in front, during this one's life: not through the read-only path)
                 z[4 * j] += v.x;
                 z[4 * j + 1] += v.y;
                 z[4 * j + 2] += v.z;
@@ -792,6 +792,10 @@ full_softmax_kernel(const __grid_constant__ CUtensorMap tmapX, const __grid_cons
         __syncwarp();
         if (lane == 0) mbar_arrive(&B->o_empty);
       }
+    }
+    if (!ok) {  // reads and writes of tensor memory on their way must end before it is freed
+      asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+      tmem_st_wait();
     }
   }
 

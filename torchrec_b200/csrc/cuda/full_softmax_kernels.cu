@@ -16,7 +16,9 @@
 // Both products want the streamed tile, once K-major (S) and once MN-major (ACC); one copy in shared memory serves both up to
 // D = 256, where ACC takes the 256 TMEM columns that two S tiles leave.  Wider rows are cut into pieces of 256 columns that
 // recompute S (and load the tile twice).
-// The maximum is raised lazily: ACC and the sums are rescaled only when a row's maximum grew by more than 2^40.
+// The reference of a row's exponentials is raised lazily: ACC and the sums are rescaled only when a row's maximum grew by more than 2^40.
+// It is a whole power of two next to zero, and counts from one of the row's own scores where those are far from zero (FsRef): classes masked
+// by a large finite bias give no infinities, and a row in which all of them are masked alike is the uniform softmax that it is.
 // Ignored rows are left out at the start (their h is never multiplied, so NaN or infinity in padding does not spread) and cost nothing.
 // All sums run in a fixed order: pieces of the streamed axis go to a workspace and are joined by a second kernel.
 // Every wait is bounded (tcgen05.cuh); a block that gives up raises an error word and returns.
@@ -35,6 +37,7 @@
 #include <torch/library.h>
 
 #include <cmath>
+#include <type_traits>
 
 #include "common.cuh"
 #include "tcgen05.cuh"
@@ -56,6 +59,10 @@ constexpr float kLn2 = 0.6931471805599453f;
 // Base-2 growth of a row's maximum that forces a rescale.  The terms have bf16's and fp32's exponents: 2^40 over 2^31 columns is far
 // from overflow, and what is flushed lies 2^86 below the largest term.
 constexpr float kRaise = 40.f;
+
+// Scores beyond this size are compared with a score of the row before they are scaled to base 2: z log2(e) and its rounding, which the
+// reference would be, lie up to 2^-24 |z| apart, for a mask of -1e10 hundreds of powers of two.  Below it the reference is an exact whole number.
+constexpr float kFar = 4194304.f;  // 2^22
 
 enum FsMode : int { FS_LSE = 0, FS_FWD = 1, FS_BWD = 2 };
 enum FsErr : int { FS_ERR_EMPTY = 1, FS_ERR_FULL = 2, FS_ERR_X = 3, FS_ERR_S = 4, FS_ERR_P = 5, FS_ERR_ACC = 6, FS_ERR_COL = 7, FS_ERR_XCH = 8, FS_ERR_SMEM = 9, FS_ERR_TARGET = 16 };
@@ -145,10 +152,12 @@ struct FsParams {
   const int* target;       // [Ppad] targets of the compacted rows
   const float* bias;       // [Vpad] (-inf behind V), or null
   float* part_acc;         // [slots, 128, min(D, 256)]; BWD: of the items left over only
-  float* part_m;           // [slots, 2, 128]  reference (base 2) of either group of warps
+  float2* part_m;          // [slots, 2, 128]  reference (k, base) of either group of warps
   float* part_l;           // [slots, 2, 128]  their sums; BWD: db
-  float* zt;               // [Ppad] score of the target (base 2)
-  const float* lse2;       // BWD [Ppad] (+inf behind n_valid)
+  float* zt;               // [Ppad] score of the target
+  const float* lse2;       // BWD [Ppad] log sum less its base, base 2 (+inf behind n_valid)
+  const float* lbase;      // BWD [Ppad] base of the log sum
+  const int* far;          // BWD: not 0 when some row's base is not
   const float* wex;        // BWD [Ppad] 1 - p_t
   const float* gcol;       // BWD [Ppad] upstream gradient of every row, or null
   const float* dloss;      // BWD scalar upstream gradient (with gcol: unused)
@@ -161,6 +170,37 @@ __device__ __forceinline__ float fs_ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// A row's reference: a term is 2^((z - base) log2(e) - k).  k is a whole number and base 0 unless the row's scores lie beyond kFar, so that
+// rescaling by the difference of two references is exact.  (Beyond it the scores themselves are a quarter and more apart.)
+struct FsRef {
+  float k = -INFINITY, base = 0.f;
+  __device__ __forceinline__ bool is(const FsRef& o) const { return k == o.k && base == o.base; }
+  // the largest score that may stand under it
+  __device__ __forceinline__ float limit() const { return fmaf(k + kRaise, kLn2, base); }
+};
+__device__ __forceinline__ float fs_gap(const FsRef& a, const FsRef& b) { return fmaf(a.base - b.base, kLog2e, a.k - b.k); }
+// what terms under `from` are multiplied by to stand under `to`
+__device__ __forceinline__ float fs_factor(const FsRef& from, const FsRef& to) { return from.is(to) ? 1.f : fs_ex2(fs_gap(from, to)); }
+// the same in either order
+__device__ __forceinline__ FsRef fs_higher(const FsRef& a, const FsRef& b) {
+  const float g = fs_gap(a, b);
+  return g > 0.f || (g == 0.f && a.base > b.base) ? a : b;
+}
+// the reference at `top`, a score above the old one
+__device__ __forceinline__ FsRef fs_raised(const FsRef& r, float top) {
+  FsRef n;
+  if (fabsf(top) < kFar) {
+    n.k = ceilf(top * kLog2e);
+  } else if (r.base != 0.f && fabsf(top - r.base) < kFar) {
+    n.base = r.base;
+    n.k = ceilf((top - r.base) * kLog2e);
+  } else {
+    n.base = top;
+    n.k = 0.f;
+  }
+  return n;
 }
 
 __device__ __forceinline__ uint32_t fs_pack(float lo, float hi) {
@@ -223,7 +263,7 @@ full_softmax_kernel(const __grid_constant__ CUtensorMap tmapX, const __grid_cons
   constexpr uint32_t kCols = ROWG ? 2 : 4, kColShift = ROWG ? 1 : 2;  // tiles whose per-column values are in shared memory
   constexpr int kPair = kAcc ? 1 : 2;  // without an accumulator two tiles are one product of 256 columns, which reads X half as often
   extern __shared__ __align__(1024) uint8_t fs_smem[];
-  float* cols = reinterpret_cast<float*>(fs_smem + kFsSlots * kFsSlotBytes);  // FWD: the rows' maxima [128]; BWD: lse2 [4][128], or lse2 [2][128], g [2][128]
+  float* cols = reinterpret_cast<float*>(fs_smem + kFsSlots * kFsSlotBytes);  // FWD: the rows' references, k [128], base [128]; BWD: lse2 [4][128], or lse2 [2][128], g [2][128]
   FsBars* B = reinterpret_cast<FsBars*>(cols + 512);
   volatile int* abort_flag = &B->abort_flag;
   // values that are alike in a warp are taken from lane 0, which tells the compiler so
@@ -514,12 +554,14 @@ full_softmax_kernel(const __grid_constant__ CUtensorMap tmapX, const __grid_cons
       const int r128 = q * 32 + lane;
       int tgt = -1;
       float bias_row = 0.f;
+      const bool far = MODE == FS_BWD && __shfl_sync(0xffffffffu, *p.far, 0) != 0;
       if constexpr (MODE == FS_BWD) {
-        if constexpr (BIAS) bias_row = p.bias[row] * kLog2e;  // padded to whole tiles
+        if constexpr (BIAS) bias_row = far ? 0.f : p.bias[row] * kLog2e;  // padded to whole tiles
       } else {
         tgt = p.target[row];
       }
-      float m2 = -INFINITY, l = 0.f;  // m2: reference of the exponentials, a whole number, so that rescaling is exact
+      FsRef ref;
+      float l = 0.f, limit = -INFINITY;
       const uint32_t tc0 = tc, tc1 = tc + (nt + kPair - 1) / kPair * kPair;
       tc += (tc ^ half) & 1;
       uint32_t b = tc % bufs, ph = (tc / bufs) & 1;  // the tile's buffer
@@ -547,63 +589,80 @@ full_softmax_kernel(const __grid_constant__ CUtensorMap tmapX, const __grid_cons
           int tg = p.target[col0 + lane];  // targets of 32 rows of h, one per lane
           const uint32_t cb = tc & (kCols - 1);
           if (!wait_all(&B->c_full[cb], (tc >> kColShift) & 1, FS_ERR_COL)) { ok = false; break; }
+          auto tile = [&](auto far_rows) {
 #pragma unroll 1
-          for (int c = 0; c < 4; ++c) {
-            float z[32];
-            tmem_ld_wait(r);
-            const float4* lp = reinterpret_cast<const float4*>(cols + cb * 128 + c * 32);
+            for (int c = 0; c < 4; ++c) {
+              float z[32];
+              tmem_ld_wait(r);
+              const float4* lp = reinterpret_cast<const float4*>(cols + cb * 128 + c * 32);
+              if constexpr (decltype(far_rows)::value) {  // scores less the base of their row's log sum
+                const float4* fp = reinterpret_cast<const float4*>(p.lbase + col0 + c * 32);
+                const float bias_far = BIAS ? p.bias[row] : 0.f;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              const float4 v = lp[j];
-              const float s4[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                const float s = __uint_as_float(r[4 * j + k]);
-                z[4 * j + k] = BIAS ? fmaf(s, kLog2e, bias_row) - s4[k] : fmaf(s, kLog2e, -s4[k]);
+                for (int j = 0; j < 8; ++j) {
+                  const float4 v = fp[j];
+                  r[4 * j] = __float_as_uint(__uint_as_float(r[4 * j]) + bias_far - v.x);
+                  r[4 * j + 1] = __float_as_uint(__uint_as_float(r[4 * j + 1]) + bias_far - v.y);
+                  r[4 * j + 2] = __float_as_uint(__uint_as_float(r[4 * j + 2]) + bias_far - v.z);
+                  r[4 * j + 3] = __float_as_uint(__uint_as_float(r[4 * j + 3]) + bias_far - v.w);
+                }
               }
-            }
-            // entries (item, row of h) with the row's target: p - 1 = -(1 - p_t)
-            uint32_t hits = __ballot_sync(0xffffffffu, tg >= v0 && tg < v0 + 32);
-            const int tg_now = tg;
-            if (c < 3) {
-              tmem_ld_32x32_issue(ts + (c + 1) * 32, r);
-              tg = p.target[col0 + (c + 1) * 32 + lane];
-            }
-#pragma unroll
-            for (int j = 0; j < 32; ++j) z[j] = fs_ex2(z[j]);
-            while (hits) {
-              const int j = __ffs(hits) - 1;
-              hits &= hits - 1;
-              if (__shfl_sync(0xffffffffu, tg_now, j) == v0 + lane) {
-                const float v = -p.wex[col0 + c * 32 + j];
-#pragma unroll
-                for (int k = 0; k < 32; ++k) z[k] = k == j ? v : z[k];
-              }
-              __syncwarp();
-            }
-            if constexpr (ROWG) {
-              const float4* gp = reinterpret_cast<const float4*>(cols + 256 + cb * 128 + c * 32);
 #pragma unroll
               for (int j = 0; j < 8; ++j) {
-                const float4 v = gp[j];
-                z[4 * j] *= v.x;
-                z[4 * j + 1] *= v.y;
-                z[4 * j + 2] *= v.z;
-                z[4 * j + 3] *= v.w;
+                const float4 v = lp[j];
+                const float s4[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                  const float s = __uint_as_float(r[4 * j + k]);
+                  z[4 * j + k] = BIAS ? fmaf(s, kLog2e, bias_row) - s4[k] : fmaf(s, kLog2e, -s4[k]);
+                }
               }
-            }
-            if constexpr (BIAS) {
-              float sum[4] = {0.f, 0.f, 0.f, 0.f};
+              // entries (item, row of h) with the row's target: p - 1 = -(1 - p_t)
+              uint32_t hits = __ballot_sync(0xffffffffu, tg >= v0 && tg < v0 + 32);
+              const int tg_now = tg;
+              if (c < 3) {
+                tmem_ld_32x32_issue(ts + (c + 1) * 32, r);
+                tg = p.target[col0 + (c + 1) * 32 + lane];
+              }
 #pragma unroll
-              for (int j = 0; j < 32; ++j) sum[j & 3] += z[j];
-              l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-            }
-            // E of these columns over score columns that this thread has read already
-            uint32_t e[16];
+              for (int j = 0; j < 32; ++j) z[j] = fs_ex2(z[j]);
+              while (hits) {
+                const int j = __ffs(hits) - 1;
+                hits &= hits - 1;
+                if (__shfl_sync(0xffffffffu, tg_now, j) == v0 + lane) {
+                  const float v = -p.wex[col0 + c * 32 + j];
 #pragma unroll
-            for (int j = 0; j < 16; ++j) e[j] = fs_pack(z[2 * j], z[2 * j + 1]);
-            tmem_st_32x16(ts + c * 16, e);
-          }
+                  for (int k = 0; k < 32; ++k) z[k] = k == j ? v : z[k];
+                }
+                __syncwarp();
+              }
+              if constexpr (ROWG) {
+                const float4* gp = reinterpret_cast<const float4*>(cols + 256 + cb * 128 + c * 32);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                  const float4 v = gp[j];
+                  z[4 * j] *= v.x;
+                  z[4 * j + 1] *= v.y;
+                  z[4 * j + 2] *= v.z;
+                  z[4 * j + 3] *= v.w;
+                }
+              }
+              if constexpr (BIAS) {
+                float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int j = 0; j < 32; ++j) sum[j & 3] += z[j];
+                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+              }
+              // E of these columns over score columns that this thread has read already
+              uint32_t e[16];
+#pragma unroll
+              for (int j = 0; j < 16; ++j) e[j] = fs_pack(z[2 * j], z[2 * j + 1]);
+              tmem_st_32x16(ts + c * 16, e);
+            }
+          };
+          // (with the rare case inside the loop of the other one: 324 -> 363 us, 18944 x 40000 x 64 with a bias)
+          if (far) tile(std::true_type());
+          else tile(std::false_type());
           __syncwarp();
           if (lane == 0) mbar_arrive(&B->c_empty[cb]);
         } else {
@@ -626,7 +685,9 @@ full_softmax_kernel(const __grid_constant__ CUtensorMap tmapX, const __grid_cons
           if constexpr (MODE == FS_FWD) {
             if (t == 1) {  // this group's first tile: the row's reference comes from the tile before
               if (!wait_all(&B->m_done[q], (tc - 1) & 1, FS_ERR_XCH)) { ok = false; break; }
-              m2 = cols[q * 32 + lane];
+              ref.k = cols[r128];
+              ref.base = cols[128 + r128];
+              limit = ref.base != 0.f ? -INFINITY : ref.limit();
             }
           }
 #pragma unroll 1
@@ -658,21 +719,27 @@ full_softmax_kernel(const __grid_constant__ CUtensorMap tmapX, const __grid_cons
                 zt = j == at ? z[j] : zt;
                 z[j] = j == at ? -INFINITY : z[j];
               }
-              if (piece == 0 && tgt >= 0 && at >= 0 && at < 32) p.zt[row] = zt * kLog2e;
+              if (piece == 0 && tgt >= 0 && at >= 0 && at < 32) p.zt[row] = zt;
               __syncwarp();
             }
             float mx[4] = {z[0], z[1], z[2], z[3]};
 #pragma unroll
             for (int j = 4; j < 32; ++j) mx[j & 3] = fmaxf(mx[j & 3], z[j]);
-            const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * kLog2e;
-            if (__builtin_expect(__any_sync(0xffffffffu, top > m2 + kRaise), 0)) {
-              const float mn = top > m2 + kRaise ? ceilf(top) : m2;
-              const float f = mn == m2 ? 1.f : fs_ex2(m2 - mn);
-              m2 = mn;
-              l *= f;
-              if constexpr (kAcc) rescale_terms(c, f);
+            const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+            if (__builtin_expect(__any_sync(0xffffffffu, top > limit), 0)) {  // rows whose base is not 0 always come here
+              const bool raise = top > ref.limit();
+              if (__any_sync(0xffffffffu, raise)) {
+                const FsRef now = raise ? fs_raised(ref, top) : ref;
+                const float f = fs_factor(ref, now);
+                ref = now;
+                limit = ref.base != 0.f ? -INFINITY : ref.limit();
+                l *= f;
+                if constexpr (kAcc) rescale_terms(c, f);
+              }
+#pragma unroll
+              for (int j = 0; j < 32; ++j) z[j] -= ref.base;
             }
-            const float ms = m2 == -INFINITY ? 0.f : m2;
+            const float ms = ref.k == -INFINITY ? 0.f : ref.k;
 #pragma unroll
             for (int j = 0; j < 32; ++j) z[j] = fmaf(z[j], kLog2e, -ms);
             if (c < 3) tmem_ld_32x32_issue(ts + (c + 1) * 32, r);
@@ -695,20 +762,23 @@ full_softmax_kernel(const __grid_constant__ CUtensorMap tmapX, const __grid_cons
             // The accumulator and both groups' sums refer to one maximum per row, kept in shared memory: a tile is published after the
             // tile before it, by when that one's decision is known.
             if (t == 0) {
-              cols[q * 32 + lane] = m2;
+              cols[r128] = ref.k;
+              cols[128 + r128] = ref.base;
             } else {
               if (t > 1 && !wait_all(&B->m_done[q], (tc - 1) & 1, FS_ERR_XCH)) { ok = false; break; }
-              const float mr = cols[q * 32 + lane];
-              if (__builtin_expect(__any_sync(0xffffffffu, mr != m2), 0)) {
-                const float mn = fmaxf(mr, m2);
-                const float fe = mn == m2 ? 1.f : fs_ex2(m2 - mn);
+              FsRef acc_ref;
+              acc_ref.k = cols[r128];
+              acc_ref.base = cols[128 + r128];
+              if (__builtin_expect(__any_sync(0xffffffffu, !acc_ref.is(ref)), 0)) {
+                const FsRef now = fs_higher(acc_ref, ref);
+                const float fe = fs_factor(ref, now);
                 l *= fe;
                 rescale_terms(4, fe);
-                if (__any_sync(0xffffffffu, mn != mr)) {
+                if (__any_sync(0xffffffffu, !now.is(acc_ref))) {
                   // every ACC up to the previous tile has to be complete; this tile's has not been issued
                   if (!wait_all(&B->acc_done[(tc - 1) & 3], ((tc - 1) >> 2) & 1, FS_ERR_ACC)) { ok = false; break; }
                   tcgen05_fence_after();
-                  const float f = mr == mn ? 1.f : fs_ex2(mr - mn);
+                  const float f = fs_factor(acc_ref, now);
                   const int groups = (min(kFsAcc, p.D - piece * kFsAcc) + 15) / 16;
 #pragma unroll 1
                   for (int g = 0; g < groups; ++g) {
@@ -720,9 +790,11 @@ full_softmax_kernel(const __grid_constant__ CUtensorMap tmapX, const __grid_cons
                     for (int j = 0; j < 16; ++j) a[j] = __float_as_uint(__uint_as_float(a[j]) * f);
                     tmem_st_32x16(to, a);
                   }
-                  cols[q * 32 + lane] = mn;
+                  cols[r128] = now.k;
+                  cols[128 + r128] = now.base;
                 }
-                m2 = mn;
+                ref = now;
+                limit = ref.base != 0.f ? -INFINITY : ref.limit();
               }
             }
             __syncwarp();
@@ -740,15 +812,17 @@ full_softmax_kernel(const __grid_constant__ CUtensorMap tmapX, const __grid_cons
       if constexpr (MODE == FS_FWD) {
         if (nt > 0 && ((tc - 1) & 1) != uint32_t(half)) {  // the other group had the last tile
           if (!wait_all(&B->m_done[q], (tc - 1) & 1, FS_ERR_XCH)) { ok = false; break; }
-          const float mr = cols[q * 32 + lane];
-          if (m2 != mr) l *= fs_ex2(m2 - mr);
-          m2 = mr;
+          FsRef acc_ref;
+          acc_ref.k = cols[r128];
+          acc_ref.base = cols[128 + r128];
+          l *= fs_factor(ref, acc_ref);
+          ref = acc_ref;
         }
       }
       if (MODE != FS_BWD || (BIAS && piece == 0)) {
         const int64_t at = (int64_t(walk.slot) * 2 + half) * kFsTile + r128;
         p.part_l[at] = l;
-        if constexpr (MODE != FS_BWD) p.part_m[at] = m2;
+        if constexpr (MODE != FS_BWD) p.part_m[at] = make_float2(ref.k, ref.base);
       }
       if constexpr (kAcc) {
         if (nt > 0) {
@@ -810,14 +884,15 @@ full_softmax_kernel(const __grid_constant__ CUtensorMap tmapX, const __grid_cons
 // ---- workspace ----------------------------------------------------------------------------------------
 // What the forward leaves for the backward, in one allocation: counters, targets, the rows' places, statistics, the padded bias, the
 // compacted rows of h and (with a gradient of h wanted) dh without the upstream factor.
-enum FsCounter : int { FS_N_VALID = 0, FS_N_BAD = 1, FS_JOINED = 2, FS_COUNTERS = 8 };
+enum FsCounter : int { FS_N_VALID = 0, FS_N_BAD = 1, FS_JOINED = 2, FS_FAR = 3, FS_COUNTERS = 8 };
 
 struct FsState {
   int* counters;        // [FS_COUNTERS + Ppad / 128]: joined rows of every tile behind the first ones
   int* target;          // [Ppad] of the compacted rows, -1 behind the last
   int* orig;            // [Ppad] their rows of h
   int* slot;            // [P] place of every row of h, or -1
-  float* lse2;          // [Ppad] log sum (base 2), +inf behind the last
+  float* lse2;          // [Ppad] log sum less its base (base 2), +inf behind the last
+  float* lbase;         // [Ppad] base of the log sum, in the scores' units
   float* wex;           // [Ppad] 1 - p_t
   float* bias;          // [Vpad], or null
   __nv_bfloat16* hc;    // [Ppad, Dp]
@@ -837,6 +912,7 @@ struct FsState {
     orig = reinterpret_cast<int*>(take(4 * Ppad));
     slot = reinterpret_cast<int*>(take(4 * P));
     lse2 = reinterpret_cast<float*>(take(4 * Ppad));
+    lbase = reinterpret_cast<float*>(take(4 * Ppad));
     wex = reinterpret_cast<float*>(take(4 * Ppad));
     bias = has_bias ? reinterpret_cast<float*>(take(4 * Vpad)) : nullptr;
     hc = reinterpret_cast<__nv_bfloat16*>(take(2 * Ppad * Dp));
@@ -933,6 +1009,7 @@ __global__ void __launch_bounds__(kPrepThreads) full_softmax_prep_kernel(const P
       p.st.counters[FS_N_VALID] = n;
       p.st.counters[FS_N_BAD] = n_bad;
       p.st.counters[FS_JOINED] = 0;
+      p.st.counters[FS_FAR] = 0;
       if (p.reduction != 0 && n == 0) *p.loss = n_bad > 0 ? __int_as_float(0x7fc00000) : 0.f;
     }
     if (n + int(threadIdx.x) < padded) p.st.target[n + threadIdx.x] = -1;
@@ -962,7 +1039,7 @@ __global__ void __launch_bounds__(kPrepThreads) full_softmax_prep_kernel(const P
 }
 
 // ---- after the forward: join the splits of every row --------------------------------------------------
-// One block per row: the weights 2^(m_s - max) of its item's parts go to shared memory, then the threads walk (group of parts, 4 columns).  The
+// One block per row: the factors of its item's parts (to the highest of their references) go to shared memory, then the threads walk (group of parts, 4 columns).  The
 // block that finishes a tile of rows last adds up their losses, and the last of those the tiles', in a fixed order.
 constexpr int kJoinThreads = 128;
 static_assert(kJoinThreads == kFsTile, "a tile's losses are added up by one block, a row per thread");
@@ -971,7 +1048,7 @@ struct JoinParams {
   FsState st;
   int V, D, grid, pieces, reduction;
   const float* part_acc;
-  const float* part_m;
+  const float2* part_m;
   const float* part_l;
   const float* zt;
   float* loss_c;     // [Ppad]
@@ -989,6 +1066,7 @@ __global__ void __launch_bounds__(kJoinThreads) full_softmax_join_kernel(const J
   const int padded = (n + kFsTile - 1) / kFsTile * kFsTile;
   if (row >= padded) return;
   __shared__ float red[kJoinThreads / 32];
+  __shared__ float2 refs[kJoinThreads / 32];
   __shared__ int arrived;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   auto block_sum = [&](float v) {
@@ -999,7 +1077,10 @@ __global__ void __launch_bounds__(kJoinThreads) full_softmax_join_kernel(const J
     return (red[0] + red[1]) + (red[2] + red[3]);
   };
   if (row >= n) {  // a streamed row of zeros: exp(0 - inf) = 0
-    if (threadIdx.x == 0) p.st.lse2[row] = INFINITY;
+    if (threadIdx.x == 0) {
+      p.st.lse2[row] = INFINITY;
+      p.st.lbase[row] = 0.f;
+    }
     return;
   }
   const float z = p.zt[row];
@@ -1017,29 +1098,54 @@ __global__ void __launch_bounds__(kJoinThreads) full_softmax_join_kernel(const J
       return sc.last_run(rel) - c0 + 1;
     };
     int first, count = slots(x, first);
-    float m = -INFINITY, l = 0.f;
+    auto load_ref = [&](int64_t at) {
+      const float2 v = p.part_m[at];
+      FsRef r;
+      r.k = v.x;
+      r.base = v.y;
+      return r;
+    };
+    FsRef m;
+    float l = 0.f;
     for (int s = threadIdx.x; s < 2 * count; s += kJoinThreads) {
       const int64_t at = (int64_t(first) * 2 + s) * kFsTile + r128;
-      const float ms = p.part_m[at], ls = p.part_l[at];
-      const float mn = fmaxf(m, ms);
-      if (mn != -INFINITY) l = l * exp2f(m - mn) + ls * exp2f(ms - mn);
+      const FsRef ms = load_ref(at);
+      const float ls = p.part_l[at];
+      const FsRef mn = fs_higher(m, ms);
+      if (mn.k != -INFINITY) l = l * fs_factor(m, mn) + ls * fs_factor(ms, mn);
       else l += ls;
       m = mn;
     }
-    const float mine = m;
-    m = warp_max(m);
-    if (lane == 0) red[warp] = m;
+    const FsRef mine = m;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      FsRef other;
+      other.k = __shfl_xor_sync(0xffffffffu, m.k, o);
+      other.base = __shfl_xor_sync(0xffffffffu, m.base, o);
+      m = fs_higher(m, other);
+    }
+    if (lane == 0) refs[warp] = make_float2(m.k, m.base);
     __syncthreads();
-    m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-    const float ms = m == -INFINITY ? 0.f : m;
-    l = block_sum(mine == -INFINITY ? l : l * exp2f(mine - ms));
-    // others' log sum a, target's score z (base 2): lse = max + log2(1 + 2^-|a - z|)
-    const float a = ms + log2f(l), d = a - z;
-    const float tail = log1pf(exp2f(-fabsf(d)));
-    const float w = d > 0.f ? 1.f / (1.f + exp2f(-d)) : exp2f(d) / (1.f + exp2f(d));  // 1 - p_t
+    m = FsRef();
+#pragma unroll
+    for (int w = 0; w < kJoinThreads / 32; ++w) {
+      FsRef other;
+      other.k = refs[w].x;
+      other.base = refs[w].y;
+      m = fs_higher(m, other);
+    }
+    if (m.k == -INFINITY) m.k = 0.f;  // no terms: every factor is 0
+    l = block_sum(mine.k == -INFINITY ? l : l * fs_factor(mine, m));
+    // others' log sum (base + a2 in base 2) and the target's score z: d = others - z, lse = max + log(1 + e^-|d|)
+    const float a2 = m.k + log2f(l), d = fmaf(a2, kLn2, m.base - z), d2 = d * kLog2e;
+    const float tail = log1pf(exp2f(-fabsf(d2)));
+    const float w = d > 0.f ? 1.f / (1.f + exp2f(-d2)) : exp2f(d2) / (1.f + exp2f(d2));  // 1 - p_t
     if (threadIdx.x == 0) {
-      const float loss = d != d ? d : (d > 0.f ? d * kLn2 : 0.f) + tail;
-      p.st.lse2[row] = fmaxf(a, z) + tail * kLog2e;
+      const float loss = d != d ? d : (d > 0.f ? d : 0.f) + tail;
+      const float base = d > 0.f ? m.base : (fabsf(z) < kFar ? 0.f : z);
+      p.st.lse2[row] = (d > 0.f ? a2 : (z - base) * kLog2e) + tail * kLog2e;
+      p.st.lbase[row] = base;
+      if (base != 0.f) p.st.counters[FS_FAR] = 1;  // every writer's value is the same
       p.st.wex[row] = w;
       if (p.reduction == 0) p.loss[p.st.orig[row]] = loss;
       else p.loss_c[row] = loss;
@@ -1053,7 +1159,7 @@ __global__ void __launch_bounds__(kJoinThreads) full_softmax_join_kernel(const J
         // every piece was cut on its own
         if (piece > 0) count = slots(piece * sc.tx + x, first);
         __syncthreads();
-        for (int s = threadIdx.x; s < count; s += kJoinThreads) js[s] = exp2f(p.part_m[(int64_t(first) + s) * 2 * kFsTile + r128] - ms);
+        for (int s = threadIdx.x; s < count; s += kJoinThreads) js[s] = fs_factor(load_ref((int64_t(first) + s) * 2 * kFsTile + r128), m);
         __syncthreads();
         const int vecs = (min(p.D - piece * kFsAcc, kFsAcc)) / 4;  // at most 64
         int lanes = 1;
@@ -1280,10 +1386,10 @@ std::tuple<at::Tensor, at::Tensor> full_softmax_fwd(const at::Tensor& h, const a
   const int grid = fs_grid(h.device());
   const int pieces = acc ? int((Dp + kFsAcc - 1) / kFsAcc) : 1;
   const int64_t prows = (Ppad / kFsTile * pieces + grid) * kFsTile, n_acc = acc ? prows * std::min<int64_t>(Dp, kFsAcc) : 0;  // rows of all slots
-  at::Tensor part = at::empty({n_acc + 4 * prows + 2 * Ppad + Ppad / kFsTile}, f32);  // accumulators, references, sums, targets' scores, losses
+  at::Tensor part = at::empty({n_acc + 6 * prows + 2 * Ppad + Ppad / kFsTile}, f32);  // accumulators, references, sums, targets' scores, losses
   float* part_acc = part.data_ptr<float>();
-  float* part_m = part_acc + n_acc;
-  float* part_l = part_m + 2 * prows;
+  float2* part_m = reinterpret_cast<float2*>(part_acc + n_acc);
+  float* part_l = part_acc + n_acc + 4 * prows;
   float* zt = part_l + 2 * prows;
   float* loss_c = zt + Ppad;
   {
@@ -1374,6 +1480,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> full_softmax_bwd(const at::Tensor
     p.part_acc = part_acc;
     p.part_l = part_l;
     p.lse2 = st.lse2;
+    p.lbase = st.lbase;
+    p.far = st.counters + FS_FAR;
     p.wex = st.wex;
     p.gcol = gcol;
     p.dloss = dloss.data_ptr<float>();

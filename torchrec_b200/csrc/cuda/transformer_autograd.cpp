@@ -25,6 +25,11 @@ static variable_list once(variable_list grads, const variable_list& upstream, co
   return (*error)(std::move(in));
 }
 
+// A dual tensor need not require a gradient, so that a call without a node would drop its tangent: a derivative of zero.
+static void refuse_forward_mode(std::initializer_list<const Tensor*> inputs, const char* name) {
+  for (const Tensor* t : inputs) TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(0).defined(), name, " has no forward-mode derivative on CUDA");
+}
+
 static c10::optional<Tensor> opt(const Tensor& t) { return t.defined() ? c10::optional<Tensor>(t) : c10::nullopt; }
 
 // ---- softmax over the whole catalogue ---------------------------------------------------------------------
@@ -94,8 +99,10 @@ static Tensor full_softmax_loss_plain(const Tensor& h, const Tensor& weight, con
 
 static Tensor full_softmax_loss_autograd(const Tensor& h, const Tensor& weight, const c10::optional<Tensor>& bias, const Tensor& targets, const c10::optional<Tensor>& rounded,
                                          int64_t ignore_index, int64_t reduction) {
+  const Tensor b = bias.value_or(Tensor());
+  refuse_forward_mode({&h, &weight, &b}, "full_softmax_loss");
   int64_t grad = 0;
-  if (at::GradMode::is_enabled()) grad = h.requires_grad() ? 2 : int64_t(weight.requires_grad() || (bias.has_value() && bias->defined() && bias->requires_grad()));
+  if (at::GradMode::is_enabled()) grad = h.requires_grad() ? 2 : int64_t(weight.requires_grad() || (b.defined() && b.requires_grad()));
   if (grad == 0) {  // no node
     at::AutoDispatchBelowADInplaceOrView below;
     return full_softmax_loss_plain(h, weight, bias, targets, rounded, ignore_index, reduction);
@@ -190,8 +197,10 @@ static Tensor qk_norm_rotary_plain(const Tensor& qkv, const Tensor& positions, c
 
 static Tensor qk_norm_rotary_autograd(const Tensor& qkv, const Tensor& positions, const Tensor& inv_freq, const c10::optional<Tensor>& qw, const c10::optional<Tensor>& kw,
                                       at::IntArrayRef sections, int64_t heads, int64_t kv_heads, double eps, bool norm, bool interleaved) {
-  auto wants = [](const c10::optional<Tensor>& t) { return t.has_value() && t->defined() && t->requires_grad(); };
-  if (!at::GradMode::is_enabled() || !(qkv.requires_grad() || wants(qw) || wants(kw))) {  // no node
+  const Tensor q = qw.value_or(Tensor()), k = kw.value_or(Tensor());
+  refuse_forward_mode({&qkv, &q, &k}, "qk_norm_rotary");
+  auto wants = [](const Tensor& t) { return t.defined() && t.requires_grad(); };
+  if (!at::GradMode::is_enabled() || !(qkv.requires_grad() || wants(q) || wants(k))) {  // no node
     at::AutoDispatchBelowADInplaceOrView below;
     return qk_norm_rotary_plain(qkv, positions, inv_freq, qw, kw, sections, heads, kv_heads, eps, norm, interleaved);
   }

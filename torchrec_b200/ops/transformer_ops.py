@@ -17,6 +17,7 @@ import itertools
 from typing import Optional, Sequence, Tuple
 
 import torch
+import torch.autograd.forward_ad as fwAD
 
 from torchrec_b200.ops import _ext, dense_ops
 
@@ -174,6 +175,11 @@ def rotary_inv_freq(rotary_dim: int, base: float = 10000.0, device: Optional[tor
     return base ** (torch.arange(rotary_dim // 2, dtype=torch.float64, device=device) * (-2.0 / rotary_dim))
 
 
+def _has_tangent(*tensors: Optional[torch.Tensor]) -> bool:
+    """Whether one of the tensors carries a forward-mode tangent."""
+    return fwAD._current_level >= 0 and any(t is not None and fwAD.unpack_dual(t).tangent is not None for t in tensors)
+
+
 def _qk_norm_rotary_plain(qkv, positions, inv_freq, q_weight, k_weight, cfg):
     """Oracle / fallback in plain torch: fp32 (fp64 for fp64 ``qkv``) with fp64 angles, one rounding at the end."""
     sections, heads, kv_heads, eps, norm, interleaved = cfg
@@ -208,10 +214,10 @@ def qk_norm_rotary(qkv: torch.Tensor, positions: torch.Tensor, inv_freq: torch.T
     Positions are int32 or int64, below ``2 ** 53`` in magnitude.
 
     Gradients reach ``qkv`` and the weights.  CUDA tensors in bf16, fp16 or fp32 with a head dimension that is a multiple of 8 up to 256
-    run in one kernel; others in plain torch."""
+    run in one kernel; others, and calls that carry forward-mode tangents, in plain torch."""
     kv_heads = num_heads if num_kv_heads is None else num_kv_heads
     sections = [inv_freq.shape[0] if inv_freq.dim() else 0] if sections is None else [int(n) for n in sections]
-    if qkv.is_cuda and qkv.dtype in _ROTARY_TYPES and qkv.dim() == 2 and num_heads + 2 * kv_heads > 0:
+    if qkv.is_cuda and qkv.dtype in _ROTARY_TYPES and qkv.dim() == 2 and num_heads + 2 * kv_heads > 0 and not _has_tangent(qkv, q_weight, k_weight):
         dim = qkv.shape[1] // (num_heads + 2 * kv_heads)
         if dim % 8 == 0 and dim <= ROTARY_MAX_HEAD_DIM and _ext.use_cuda_kernel(qkv, "qk_norm_rotary"):  # arguments are checked there
             return torch.ops.trb200.qk_norm_rotary(qkv, positions, inv_freq, q_weight, k_weight, sections, num_heads, kv_heads, eps, norm, interleaved)
@@ -382,7 +388,8 @@ def full_softmax_loss(h: torch.Tensor, weight: torch.Tensor, targets: torch.Tens
     On CUDA bf16 ``h`` (and fp32 ``h`` while the dense compute type is bf16, ``dense_ops.set_dense_compute_dtype``) with ``D <= 1024`` runs
     on the tensor cores with bf16 operands and fp32 sums; an fp32 ``weight`` is rounded to bf16 for the products and gets an fp32
     gradient.  Everything else is computed in fp32 (fp64 for fp64 ``h``), a piece of the rows at a time.  A target outside ``[0, V)``
-    raises on the CPU; on CUDA it makes the row's loss NaN and its gradient zero, and ``full_softmax_error`` reports it."""
+    raises on the CPU; on CUDA it makes the row's loss NaN and its gradient zero, and ``full_softmax_error`` reports it.  Forward-mode
+    derivatives are refused."""
     if reduction not in _REDUCTIONS:
         raise ValueError(f"full_softmax_loss: reduction is one of {sorted(_REDUCTIONS)}, got {reduction!r}")
     if h.is_cuda and h.dim() == 2 and h.shape[1] <= FULL_SOFTMAX_MAX_DIM and weight.dtype in _KERNEL_TYPES and (bias is None or bias.dtype in _KERNEL_TYPES):

@@ -340,11 +340,12 @@ class _FullSoftmaxPieces(torch.autograd.Function):
         t = torch.where(keep, targets, 0)
         step = max(1, _FullSoftmaxPieces.PIECE // V)
         lse, rows = h.new_zeros(P, dtype=acc), h.new_zeros(P, dtype=acc)
-        for lo in range(0, P, step):
-            hi = min(P, lo + step)
-            _, z = _FullSoftmaxPieces._scores(h, weight, bias, keep, lo, hi, acc)
-            lse[lo:hi] = torch.logsumexp(z, 1)
-            rows[lo:hi] = lse[lo:hi] - z.gather(1, t[lo:hi, None]).squeeze(1)
+        with torch.autocast(h.device.type, enabled=False):  # the products in `acc` in either direction, whatever region the call stands in
+            for lo in range(0, P, step):
+                hi = min(P, lo + step)
+                _, z = _FullSoftmaxPieces._scores(h, weight, bias, keep, lo, hi, acc)
+                lse[lo:hi] = torch.logsumexp(z, 1)
+                rows[lo:hi] = lse[lo:hi] - z.gather(1, t[lo:hi, None]).squeeze(1)
         rows = torch.where(keep, rows, 0).masked_fill(bad, float("nan"))
         count = keep.sum().clamp(min=1)
         ctx.save_for_backward(h, weight, bias, t, keep, lse, count)
@@ -363,16 +364,17 @@ class _FullSoftmaxPieces(torch.autograd.Function):
         dh = torch.zeros_like(h)
         dw = weight.new_zeros(weight.shape, dtype=acc)
         db = None if bias is None else bias.new_zeros(bias.shape, dtype=acc)
-        for lo in range(0, P, step):
-            hi = min(P, lo + step)
-            x, z = _FullSoftmaxPieces._scores(h, weight, bias, keep, lo, hi, acc)
-            p = torch.exp(z - lse[lo:hi, None])
-            p.scatter_add_(1, t[lo:hi, None], p.new_full((hi - lo, 1), -1.0))
-            p = torch.where(keep[lo:hi, None], p * scale[lo:hi, None], 0)
-            dh[lo:hi] = (p @ w).to(h.dtype)
-            dw += p.t() @ x
-            if db is not None:
-                db += p.sum(0)
+        with torch.autocast(h.device.type, enabled=False):
+            for lo in range(0, P, step):
+                hi = min(P, lo + step)
+                x, z = _FullSoftmaxPieces._scores(h, weight, bias, keep, lo, hi, acc)
+                p = torch.exp(z - lse[lo:hi, None])
+                p.scatter_add_(1, t[lo:hi, None], p.new_full((hi - lo, 1), -1.0))
+                p = torch.where(keep[lo:hi, None], p * scale[lo:hi, None], 0)
+                dh[lo:hi] = (p @ w).to(h.dtype)
+                dw += p.t() @ x
+                if db is not None:
+                    db += p.sum(0)
         return dh, dw.to(weight.dtype), None if db is None else db.to(bias.dtype), None, None, None
 
 

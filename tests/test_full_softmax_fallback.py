@@ -1,5 +1,7 @@
 """Softmax loss over the whole catalogue where no kernel takes it (the CPU here; types, widths and compute types that the kernel does not take
-on CUDA): inside an autocast region."""
+on CUDA): inside an autocast region, with masks."""
+import math
+
 import pytest
 import torch
 
@@ -32,3 +34,36 @@ def test_autocast_changes_nothing(device, where):
         assert x.dtype == y.dtype and torch.equal(x, y)
     # a row's gradients of the scores add up to zero: 500 terms of at most 1 in fp32, 64 rows
     assert abs(float(got_g[2].sum())) <= 64 * 500 * 2.0**-24
+
+
+@devices
+@pytest.mark.parametrize("mask", [-1e9, -1e20, torch.finfo(torch.float32).min])
+def test_rows_whose_mask_leaves_nothing(device, mask):
+    """Every class behind the same finite mask, which swallows the products: a uniform softmax, as cross_entropy of these scores."""
+    h, w, b, t = _inputs(20, 70, 8, device)
+    with torch.no_grad():
+        b.fill_(mask)
+    loss = full_softmax_loss(h, w, t, b, reduction="none")
+    grads = torch.autograd.grad(loss.sum(), (h, w, b))
+    want = torch.nn.functional.cross_entropy(h @ w.t() + b, t, reduction="none")
+    want_g = torch.autograd.grad(want.sum(), (h, w, b))
+    torch.testing.assert_close(loss, want, rtol=1e-6, atol=1e-6)
+    assert abs(float(loss[0].detach()) - math.log(70)) < 1e-5
+    for x, y in zip(grads, want_g):
+        torch.testing.assert_close(x, y, rtol=1e-5, atol=1e-5)
+
+
+def test_infinite_masks():
+    h, w, b, t = _inputs(6, 9, 4, "cpu")
+    with torch.no_grad():
+        b[:4] = float("-inf")
+    t = torch.tensor([4, 5, 6, 7, 8, 0])  # the last target cannot be reached
+    rows = full_softmax_loss(h, w, t, b, reduction="none")
+    want = torch.nn.functional.cross_entropy(h @ w.t() + b, t, reduction="none")
+    torch.testing.assert_close(rows, want)
+    assert float(rows[5].detach()) == float("inf")
+    one = torch.full((9,), float("-inf"))
+    one[5] = 0.5
+    loss = full_softmax_loss(h, w, torch.full((6,), 5), one, reduction="sum")
+    (dh,) = torch.autograd.grad(loss, h)
+    assert float(loss.detach()) == 0 and float(dh.abs().max()) == 0

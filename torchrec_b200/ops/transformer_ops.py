@@ -339,23 +339,27 @@ class _FullSoftmaxPieces(torch.autograd.Function):
         keep = keep & ~bad
         t = torch.where(keep, targets, 0)
         step = max(1, _FullSoftmaxPieces.PIECE // V)
-        lse, rows = h.new_zeros(P, dtype=acc), h.new_zeros(P, dtype=acc)
+        # the log sum is kept as a score of the row and the rest: next to a mask of -1e9 their sum would lose log V
+        top, lse, rows = (h.new_zeros(P, dtype=acc) for _ in range(3))
         with torch.autocast(h.device.type, enabled=False):  # the products in `acc` in either direction, whatever region the call stands in
             for lo in range(0, P, step):
                 hi = min(P, lo + step)
                 _, z = _FullSoftmaxPieces._scores(h, weight, bias, keep, lo, hi, acc)
-                lse[lo:hi] = torch.logsumexp(z, 1)
+                m = z.amax(1, keepdim=True)
+                m = torch.where(m == float("-inf"), 0, m)
+                z -= m
+                top[lo:hi], lse[lo:hi] = m.squeeze(1), torch.logsumexp(z, 1)
                 rows[lo:hi] = lse[lo:hi] - z.gather(1, t[lo:hi, None]).squeeze(1)
         rows = torch.where(keep, rows, 0).masked_fill(bad, float("nan"))
         count = keep.sum().clamp(min=1)
-        ctx.save_for_backward(h, weight, bias, t, keep, lse, count)
+        ctx.save_for_backward(h, weight, bias, t, keep, top, lse, count)
         ctx.cfg = (reduction, acc)
         return rows if reduction == 0 else rows.sum() if reduction == 2 else rows.sum() / count
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
-        h, weight, bias, t, keep, lse, count = ctx.saved_tensors
+        h, weight, bias, t, keep, top, lse, count = ctx.saved_tensors
         reduction, acc = ctx.cfg
         P, V = h.shape[0], weight.shape[0]
         scale = torch.where(keep, (g / count if reduction == 1 else g).to(acc), 0)
@@ -368,7 +372,7 @@ class _FullSoftmaxPieces(torch.autograd.Function):
             for lo in range(0, P, step):
                 hi = min(P, lo + step)
                 x, z = _FullSoftmaxPieces._scores(h, weight, bias, keep, lo, hi, acc)
-                p = torch.exp(z - lse[lo:hi, None])
+                p = torch.exp((z - top[lo:hi, None]) - lse[lo:hi, None])
                 p.scatter_add_(1, t[lo:hi, None], p.new_full((hi - lo, 1), -1.0))
                 p = torch.where(keep[lo:hi, None], p * scale[lo:hi, None], 0)
                 dh[lo:hi] = (p @ w).to(h.dtype)

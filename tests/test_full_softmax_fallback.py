@@ -1,5 +1,5 @@
 """Softmax loss over the whole catalogue where no kernel takes it (the CPU here; types, widths and compute types that the kernel does not take
-on CUDA): inside an autocast region, with masks."""
+on CUDA): inside an autocast region, with masks, with confident rows."""
 import math
 
 import pytest
@@ -67,3 +67,29 @@ def test_infinite_masks():
     loss = full_softmax_loss(h, w, torch.full((6,), 5), one, reduction="sum")
     (dh,) = torch.autograd.grad(loss, h)
     assert float(loss.detach()) == 0 and float(dh.abs().max()) == 0
+
+
+@devices
+def test_confident_rows_keep_their_accuracy(device):
+    """1 - p of a target that has almost everything: relative to itself, not to 1.  Scores are off by at most d = D 2^-23 sum |h w|, the rest
+    by a dozen roundings, which is the relative error of a loss that small and of its gradient."""
+    h, w, b, t = _inputs(60, 200, 32, device)
+    with torch.no_grad():
+        h.copy_(w[t] * torch.linspace(0.5, 1.5, 60, device=device)[:, None])
+    b = None
+    loss = full_softmax_loss(h, w, t, b, reduction="none")
+    (dh,) = torch.autograd.grad(loss.sum(), h)
+    z = h.detach().double() @ w.detach().double().t()
+    zt = z.gather(1, t[:, None])[:, 0]
+    others = torch.logsumexp(z.scatter(1, t[:, None], float("-inf")), 1) - zt
+    want = torch.nn.functional.softplus(others, threshold=1e9)
+    want = torch.where(others < -30, torch.exp(others), want)
+    d = 32 * 2.0**-23 * float((h.detach().double().abs() @ w.detach().double().abs().t()).max()) + 2.0**-20
+    rel = torch.expm1(torch.tensor(2 * d)).item() + 2.0**-20
+    assert float(want.min()) < 1e-9  # there are such rows
+    assert bool(((loss.detach().double() - want).abs() <= rel * want + 1e-37).all())
+    G = torch.exp(z - zt[:, None] - want[:, None])
+    G[torch.arange(60, device=device), t] = -torch.sigmoid(others)
+    wd = w.detach().double()
+    limit = (rel + 200 * 2.0**-23) * (G.abs() @ wd.abs()) + 1e-37
+    assert bool(((dh.double() - G @ wd).abs() <= limit).all())

@@ -339,8 +339,9 @@ class _FullSoftmaxPieces(torch.autograd.Function):
         keep = keep & ~bad
         t = torch.where(keep, targets, 0)
         step = max(1, _FullSoftmaxPieces.PIECE // V)
-        # the log sum is kept as a score of the row and the rest: next to a mask of -1e9 their sum would lose log V
-        top, lse, rows = (h.new_zeros(P, dtype=acc) for _ in range(3))
+        # the log sum is kept as a score of the row and the rest: next to a mask of -1e9 their sum would lose log V; the other classes'
+        # distance to the target gives 1 - p of a confident row, which is no difference of two rounded numbers then
+        top, lse, gap, rows = (h.new_zeros(P, dtype=acc) for _ in range(4))
         with torch.autocast(h.device.type, enabled=False):  # the products in `acc` in either direction, whatever region the call stands in
             for lo in range(0, P, step):
                 hi = min(P, lo + step)
@@ -348,18 +349,20 @@ class _FullSoftmaxPieces(torch.autograd.Function):
                 m = z.amax(1, keepdim=True)
                 m = torch.where(m == float("-inf"), 0, m)
                 z -= m
-                top[lo:hi], lse[lo:hi] = m.squeeze(1), torch.logsumexp(z, 1)
-                rows[lo:hi] = lse[lo:hi] - z.gather(1, t[lo:hi, None]).squeeze(1)
+                zt = z.gather(1, t[lo:hi, None]).squeeze(1)
+                others = torch.logsumexp(z.scatter_(1, t[lo:hi, None], float("-inf")), 1)
+                top[lo:hi], lse[lo:hi], gap[lo:hi] = m.squeeze(1), torch.logaddexp(others, zt), others - zt
+                rows[lo:hi] = torch.logaddexp(gap[lo:hi], torch.zeros_like(zt))
         rows = torch.where(keep, rows, 0).masked_fill(bad, float("nan"))
         count = keep.sum().clamp(min=1)
-        ctx.save_for_backward(h, weight, bias, t, keep, top, lse, count)
+        ctx.save_for_backward(h, weight, bias, t, keep, top, lse, gap, count)
         ctx.cfg = (reduction, acc)
         return rows if reduction == 0 else rows.sum() if reduction == 2 else rows.sum() / count
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
-        h, weight, bias, t, keep, top, lse, count = ctx.saved_tensors
+        h, weight, bias, t, keep, top, lse, gap, count = ctx.saved_tensors
         reduction, acc = ctx.cfg
         P, V = h.shape[0], weight.shape[0]
         scale = torch.where(keep, (g / count if reduction == 1 else g).to(acc), 0)
@@ -373,7 +376,7 @@ class _FullSoftmaxPieces(torch.autograd.Function):
                 hi = min(P, lo + step)
                 x, z = _FullSoftmaxPieces._scores(h, weight, bias, keep, lo, hi, acc)
                 p = torch.exp((z - top[lo:hi, None]) - lse[lo:hi, None])
-                p.scatter_add_(1, t[lo:hi, None], p.new_full((hi - lo, 1), -1.0))
+                p.scatter_(1, t[lo:hi, None], -torch.sigmoid(gap[lo:hi, None]))
                 p = torch.where(keep[lo:hi, None], p * scale[lo:hi, None], 0)
                 dh[lo:hi] = (p @ w).to(h.dtype)
                 dw += p.t() @ x

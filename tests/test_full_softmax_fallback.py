@@ -1,5 +1,5 @@
 """Softmax loss over the whole catalogue where no kernel takes it (the CPU here; types, widths and compute types that the kernel does not take
-on CUDA): inside an autocast region, with masks, with confident rows."""
+on CUDA): inside an autocast region, with masks, with confident rows, with targets outside the classes."""
 import math
 
 import pytest
@@ -93,3 +93,21 @@ def test_confident_rows_keep_their_accuracy(device):
     wd = w.detach().double()
     limit = (rel + 200 * 2.0**-23) * (G.abs() @ wd.abs()) + 1e-37
     assert bool(((dh.double() - G @ wd).abs() <= limit).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.float64])
+def test_targets_outside_the_classes_are_reported_on_cuda(dtype):
+    from torchrec_b200.ops.transformer_ops import full_softmax_error
+
+    h, w, b, t = _inputs(20, 30, 8, "cuda")
+    h = h.detach().to(dtype).requires_grad_(True)
+    assert full_softmax_error(h.device) == 0
+    full_softmax_loss(h, w, t, b, reduction="none")
+    assert full_softmax_error(h.device) == 0
+    t[3], t[11], t[12] = 30, -1, -100
+    rows = full_softmax_loss(h, w, t, b, reduction="none")
+    rows.sum().backward()
+    assert rows.isnan().nonzero().flatten().tolist() == [3, 11]
+    assert float(h.grad[[3, 11, 12]].abs().max()) == 0 and bool(torch.isfinite(h.grad).all())
+    assert full_softmax_error(h.device) == 16 and full_softmax_error(h.device) == 0

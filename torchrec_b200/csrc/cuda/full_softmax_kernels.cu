@@ -1510,6 +1510,23 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> full_softmax_bwd(const at::Tensor
   return {dh, dw, db};
 }
 
+// Raises the error word for targets outside [0, classes): calls that no kernel takes report them as the others do, without a look from the host.
+__global__ void full_softmax_targets_kernel(const int64_t* __restrict__ targets, int64_t n, int64_t stride, int64_t classes, int64_t ignore) {
+  for (int64_t i = int64_t(blockIdx.x) * blockDim.x + threadIdx.x; i < n; i += int64_t(gridDim.x) * blockDim.x) {
+    const int64_t t = targets[i * stride];
+    if (t != ignore && (t < 0 || t >= classes)) atomicCAS(&g_fs_error, 0, FS_ERR_TARGET);
+  }
+}
+
+void full_softmax_check_targets(const at::Tensor& targets, int64_t classes, int64_t ignore_index) {
+  TORCH_CHECK_VALUE(targets.is_cuda() && targets.dim() == 1 && targets.scalar_type() == at::kLong, "full_softmax_check_targets: targets is an int64 [P]");
+  if (targets.numel() == 0) return;
+  c10::cuda::CUDAGuard guard(targets.device());
+  const unsigned blocks = unsigned(std::min<int64_t>((targets.numel() + 255) / 256, 4 * fs_grid(targets.device())));
+  full_softmax_targets_kernel<<<blocks, 256, 0, at::cuda::getCurrentCUDAStream()>>>(targets.data_ptr<int64_t>(), targets.numel(), targets.stride(0), classes, ignore_index);
+  TRB_CUDA_CHECK(cudaGetLastError());
+}
+
 // non-zero after a launch gave up waiting (1..9) or met a target outside [0, V) (16); reading it synchronises and resets it
 int64_t full_softmax_status() {
   int v = 0;
@@ -1526,12 +1543,14 @@ TORCH_LIBRARY_FRAGMENT(trb200, m) {
   m.def("full_softmax_fwd(Tensor h, Tensor weight, Tensor targets, Tensor? bias, int ignore_index, int reduction, int grad) -> (Tensor, Tensor)");
   m.def("full_softmax_bwd(Tensor dloss, Tensor weight, Tensor state, int P, int D, bool has_bias, int reduction, bool has_unit, bool want_h, bool want_w, bool want_b, "
         "bool dh_fp32, bool dw_fp32, bool db_fp32) -> (Tensor, Tensor, Tensor)");
+  m.def("full_softmax_check_targets(Tensor targets, int classes, int ignore_index) -> ()");
   m.def("full_softmax_status() -> int");
 }
 
 TORCH_LIBRARY_IMPL(trb200, CUDA, m) {
   m.impl("full_softmax_fwd", &trb::full_softmax_fwd);
   m.impl("full_softmax_bwd", &trb::full_softmax_bwd);
+  m.impl("full_softmax_check_targets", &trb::full_softmax_check_targets);
 }
 
 TORCH_LIBRARY_IMPL(trb200, CompositeExplicitAutograd, m) { m.impl("full_softmax_status", &trb::full_softmax_status); }

@@ -336,6 +336,8 @@ class _FullSoftmaxPieces(torch.autograd.Function):
         bad = keep & ((targets < 0) | (targets >= V))
         if not targets.is_cuda and bool(bad.any()):
             raise IndexError(f"full_softmax_loss: target {int(targets[bad][0])} is out of bounds for {V} classes")
+        if targets.is_cuda and _ext.has_cuda_ext():
+            torch.ops.trb200.full_softmax_check_targets(targets, V, ignore_index)
         keep = keep & ~bad
         t = torch.where(keep, targets, 0)
         step = max(1, _FullSoftmaxPieces.PIECE // V)

@@ -14,11 +14,10 @@ using at::Tensor;
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
-// Gradients of a backward that is itself recorded (create_graph): differentiating them again is an error, not silently zero.
-static variable_list once(variable_list grads, const variable_list& upstream, const char* name) {
-  bool any = false;
-  for (const auto& g : upstream) any = any || (g.defined() && g.requires_grad());
-  if (!at::GradMode::is_enabled() || !any) return grads;
+// Gradients of a backward that is itself recorded (create_graph): differentiating them again is an error, not silently zero.  They depend on
+// the inputs whether or not the upstream gradient, often the constant one, is recorded too.
+static variable_list once(variable_list grads, const char* name) {
+  if (!at::GradMode::is_enabled()) return grads;
   variable_list in;
   for (auto& g : grads) in.push_back(g.defined() ? g.detach().set_requires_grad(true) : g);
   auto error = std::make_shared<torch::autograd::DelayedError>(std::string("the gradient of ") + name + " cannot be differentiated again", int(in.size()));
@@ -74,7 +73,7 @@ struct FullSoftmaxLoss : public torch::autograd::Function<FullSoftmaxLoss> {
     if (want_h) out[0] = dh;
     if (want_w) out[1] = dw;
     if (want_b) out[2] = db;
-    return once(std::move(out), grads, "full_softmax_loss");
+    return once(std::move(out), "full_softmax_loss");
   }
 };
 
@@ -152,7 +151,7 @@ struct QKNormRotary : public torch::autograd::Function<QKNormRotary> {
       if (want_k) out[2] = dw.select(0, 1).to(at::ScalarType(ints[5]));
     }
     if (ctx->needs_input_grad(0)) out[0] = dqkv;
-    return once(std::move(out), grads, "qk_norm_rotary");
+    return once(std::move(out), "qk_norm_rotary");
   }
 };
 

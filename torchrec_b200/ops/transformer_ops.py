@@ -362,8 +362,16 @@ class _FullSoftmaxPieces(torch.autograd.Function):
         return rows if reduction == 0 else rows.sum() if reduction == 2 else rows.sum() / count
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, g):
+        with torch.no_grad():
+            grads = _FullSoftmaxPieces._gradients(ctx, g)
+        if torch.is_grad_enabled():  # create_graph: an error when they are differentiated again, whatever `g` is (once_differentiable asks `g` alone)
+            fail = torch._C._functions.DelayedError(b"the gradient of full_softmax_loss cannot be differentiated again", len(grads))
+            grads = fail(*(None if x is None else x.detach().requires_grad_(True) for x in grads))
+        return grads[0], grads[1], grads[2], None, None, None
+
+    @staticmethod
+    def _gradients(ctx, g):
         h, weight, bias, t, keep, top, lse, gap, count = ctx.saved_tensors
         reduction, acc = ctx.cfg
         P, V = h.shape[0], weight.shape[0]
@@ -384,7 +392,7 @@ class _FullSoftmaxPieces(torch.autograd.Function):
                 dw += p.t() @ x
                 if db is not None:
                     db += p.sum(0)
-        return dh, dw.to(weight.dtype), None if db is None else db.to(bias.dtype), None, None, None
+        return dh, dw.to(weight.dtype), None if db is None else db.to(bias.dtype)
 
 
 def full_softmax_loss(h: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, bias: Optional[torch.Tensor] = None, ignore_index: int = -100,
@@ -400,7 +408,7 @@ def full_softmax_loss(h: torch.Tensor, weight: torch.Tensor, targets: torch.Tens
     on the tensor cores with bf16 operands and fp32 sums; an fp32 ``weight`` is rounded to bf16 for the products and gets an fp32
     gradient.  Everything else is computed in fp32 (fp64 for fp64 ``h``), a piece of the rows at a time.  A target outside ``[0, V)``
     raises on the CPU; on CUDA it makes the row's loss NaN and its gradient zero, and ``full_softmax_error`` reports it.  Forward-mode
-    derivatives are refused."""
+    and second derivatives are refused."""
     if reduction not in _REDUCTIONS:
         raise ValueError(f"full_softmax_loss: reduction is one of {sorted(_REDUCTIONS)}, got {reduction!r}")
     if h.is_cuda and h.dim() == 2 and h.shape[1] <= FULL_SOFTMAX_MAX_DIM and weight.dtype in _KERNEL_TYPES and (bias is None or bias.dtype in _KERNEL_TYPES):

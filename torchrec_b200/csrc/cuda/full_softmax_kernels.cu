@@ -21,7 +21,8 @@
 // by a large finite bias give no infinities, and a row in which all of them are masked alike is the uniform softmax that it is.
 // Ignored rows are left out at the start (their h is never multiplied, so NaN or infinity in padding does not spread) and cost nothing.
 // All sums run in a fixed order: pieces of the streamed axis go to a workspace and are joined by a second kernel.
-// Every wait is bounded (tcgen05.cuh); a block that gives up raises an error word and returns.
+// Every wait is bounded (tcgen05.cuh); a block that gives up raises an error word, marks the call's state and returns, and the kernels behind
+// it give NaN for the loss and every gradient of that call.
 //
 // Measured (B200, 18944 rows x 40000 classes, whole forward or backward): D = 256 forward with dh 644 us (1.20 PFLOP/s), backward 557 us
 // (1.39), value only 370 us (1.05); D = 64 422, 311 and 336 us, where the 16384 exponentials of a tile take 1.0 to 1.3 us; D = 512 (half the
@@ -158,6 +159,7 @@ struct FsParams {
   const float* lse2;       // BWD [Ppad] log sum less its base, base 2 (+inf behind n_valid)
   const float* lbase;      // BWD [Ppad] base of the log sum
   const int* far;          // BWD: not 0 when some row's base is not
+  int* gave_up;            // set by a block that gave up
   const float* wex;        // BWD [Ppad] 1 - p_t
   const float* gcol;       // BWD [Ppad] upstream gradient of every row, or null
   const float* dloss;      // BWD scalar upstream gradient (with gcol: unused)
@@ -875,6 +877,7 @@ full_softmax_kernel(const __grid_constant__ CUtensorMap tmapX, const __grid_cons
 
   tcgen05_fence_before();
   __syncthreads();
+  if (threadIdx.x == 0 && *abort_flag != 0) *p.gave_up = 1;
   if (warp == 1) {
     tcgen05_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
@@ -884,7 +887,7 @@ full_softmax_kernel(const __grid_constant__ CUtensorMap tmapX, const __grid_cons
 // ---- workspace ----------------------------------------------------------------------------------------
 // What the forward leaves for the backward, in one allocation: counters, targets, the rows' places, statistics, the padded bias, the
 // compacted rows of h and (with a gradient of h wanted) dh without the upstream factor.
-enum FsCounter : int { FS_N_VALID = 0, FS_N_BAD = 1, FS_JOINED = 2, FS_FAR = 3, FS_COUNTERS = 8 };
+enum FsCounter : int { FS_N_VALID = 0, FS_N_BAD = 1, FS_JOINED = 2, FS_FAR = 3, FS_GAVE_UP = 4, FS_COUNTERS = 8 };
 
 struct FsState {
   int* counters;        // [FS_COUNTERS + Ppad / 128]: joined rows of every tile behind the first ones
@@ -944,6 +947,7 @@ struct PrepParams {
   int bias_bf16;
   int rows;  // of a block: a multiple of 32
   int row_blocks;
+  int gave_up;  // what FS_GAVE_UP starts at
 };
 
 __device__ __forceinline__ int64_t fs_target(int64_t i, const PrepParams& p) {
@@ -1010,6 +1014,7 @@ __global__ void __launch_bounds__(kPrepThreads) full_softmax_prep_kernel(const P
       p.st.counters[FS_N_BAD] = n_bad;
       p.st.counters[FS_JOINED] = 0;
       p.st.counters[FS_FAR] = 0;
+      p.st.counters[FS_GAVE_UP] = p.gave_up;
       if (p.reduction != 0 && n == 0) *p.loss = n_bad > 0 ? __int_as_float(0x7fc00000) : 0.f;
     }
     if (n + int(threadIdx.x) < padded) p.st.target[n + threadIdx.x] = -1;
@@ -1141,7 +1146,7 @@ __global__ void __launch_bounds__(kJoinThreads) full_softmax_join_kernel(const J
     const float tail = log1pf(exp2f(-fabsf(d2)));
     const float w = d > 0.f ? 1.f / (1.f + exp2f(-d2)) : exp2f(d2) / (1.f + exp2f(d2));  // 1 - p_t
     if (threadIdx.x == 0) {
-      const float loss = d != d ? d : (d > 0.f ? d : 0.f) + tail;
+      const float loss = p.st.counters[FS_GAVE_UP] != 0 ? __int_as_float(0x7fc00000) : d != d ? d : (d > 0.f ? d : 0.f) + tail;
       const float base = d > 0.f ? m.base : (fabsf(z) < kFar ? 0.f : z);
       p.st.lse2[row] = (d > 0.f ? a2 : (z - base) * kLog2e) + tail * kLog2e;
       p.st.lbase[row] = base;
@@ -1234,7 +1239,8 @@ struct FinishParams {
   const float* part_acc;  // or null: dW was written by the main kernel
   const float* part_l;
   void* dh;               // [P, D] or null
-  void* dw;               // [V, Dp]
+  void* dw;               // [dw_rows, Dp]
+  int64_t dw_rows;        // V, or 0
   void* db;               // [V] or null
   int db_bf16;
 };
@@ -1254,6 +1260,7 @@ template <typename TH, typename TW>
 __global__ void __launch_bounds__(256) full_softmax_finish_kernel(const FinishParams p) {
   fs_after();
   const int n = p.st.counters[FS_N_VALID], vecs = p.Dp / 8;
+  const bool gave_up = p.st.counters[FS_GAVE_UP] != 0;  // in this pass or in the forward: what the blocks left is not to be used
   const int64_t step = int64_t(gridDim.x) * blockDim.x, me = int64_t(blockIdx.x) * blockDim.x + threadIdx.x;
   const float g_all = p.per_row ? 1.f : *p.dloss / (p.mean ? float(max(n, 1)) : 1.f);
   if (p.dh != nullptr) {
@@ -1269,6 +1276,10 @@ __global__ void __launch_bounds__(256) full_softmax_finish_kernel(const FinishPa
         const float4 a = u[0], b = u[1];
         v[0] = a.x * g; v[1] = a.y * g; v[2] = a.z * g; v[3] = a.w * g;
         v[4] = b.x * g; v[5] = b.y * g; v[6] = b.z * g; v[7] = b.w * g;
+        if (gave_up) {
+#pragma unroll
+          for (int k = 0; k < 8; ++k) v[k] = __int_as_float(0x7fc00000);
+        }
       }
       TH* o = reinterpret_cast<TH*>(p.dh) + row * p.D + c;
       if (p.D == p.Dp) {
@@ -1277,6 +1288,17 @@ __global__ void __launch_bounds__(256) full_softmax_finish_kernel(const FinishPa
         for (int k = 0; k < 8 && c + k < p.D; ++k) o[k] = TH(v[k]);
       }
     }
+  }
+  if (gave_up) {
+    const float nan = __int_as_float(0x7fc00000);
+    const float v[8] = {nan, nan, nan, nan, nan, nan, nan, nan};
+    for (int64_t i = me; i < p.dw_rows * vecs; i += step) fs_store8(reinterpret_cast<TW*>(p.dw) + i * 8, v);
+    if (p.db != nullptr)
+      for (int64_t i = me; i < p.V; i += step) {
+        if (p.db_bf16) reinterpret_cast<__nv_bfloat16*>(p.db)[i] = __float2bfloat16(nan);
+        else reinterpret_cast<float*>(p.db)[i] = nan;
+      }
+    return;
   }
   if (p.part_acc == nullptr && p.db == nullptr) return;
   const FsSchedule sc(p.V, n, p.pieces, p.grid);
@@ -1354,9 +1376,9 @@ static void fs_check_weight(const at::Tensor& w) {
 
 // h [P, D] bf16 or fp32 (any strides), weight [V, Dp] bf16 with Dp = D rounded up to 8 (zero columns behind D), targets [P] int64 or
 // int32, bias [V] fp32 or bf16 or none.  reduction: 0 none, 1 mean, 2 sum.  grad: 0 loss only, 1 prepare the backward of W and b, 2 of h
-// too.  Returns the loss and the state for the backward.
+// too.  Returns the loss and the state for the backward.  gave_up: not 0 gives what a call gives in which a block gave up its wait.
 std::tuple<at::Tensor, at::Tensor> full_softmax_fwd(const at::Tensor& h, const at::Tensor& weight, const at::Tensor& targets, const c10::optional<at::Tensor>& bias,
-                                                    int64_t ignore_index, int64_t reduction, int64_t grad) {
+                                                    int64_t ignore_index, int64_t reduction, int64_t grad, int64_t gave_up) {
   fs_check_weight(weight);
   TORCH_CHECK_VALUE(h.is_cuda() && h.dim() == 2 && (h.scalar_type() == at::kBFloat16 || h.scalar_type() == at::kFloat), "full_softmax: h is a bf16 or fp32 CUDA tensor [P, D]");
   TORCH_CHECK_VALUE(targets.is_cuda() && targets.dim() == 1 && (targets.scalar_type() == at::kLong || targets.scalar_type() == at::kInt) && targets.size(0) == h.size(0),
@@ -1401,13 +1423,14 @@ std::tuple<at::Tensor, at::Tensor> full_softmax_fwd(const at::Tensor& h, const a
     const bool vec = !fp32 && D == Dp && h.stride(1) == 1 && h.stride(0) % 8 == 0 && reinterpret_cast<uintptr_t>(h.data_ptr()) % 16 == 0;
     const PrepParams q{h.data_ptr(), h.stride(0), h.stride(1), fp32, vec, targets.data_ptr(), targets.stride(0), ignore_index, targets.scalar_type() == at::kInt,
                        int(P), int(V), int(D), int(Dp), st, loss.data_ptr<float>(), int(reduction), has_bias ? bias->data_ptr() : nullptr, has_bias ? bias->stride(0) : 0,
-                       has_bias && bias->scalar_type() == at::kBFloat16, rows, row_blocks};
+                       has_bias && bias->scalar_type() == at::kBFloat16, rows, row_blocks, gave_up != 0};
     full_softmax_prep_kernel<<<row_blocks + bias_blocks, kPrepThreads, 0, stream>>>(q);
     TRB_CUDA_CHECK(cudaGetLastError());
   }
   FsParams p{};
   fs_shape(p, V, Dp, acc);
   p.n_valid = st.counters + FS_N_VALID;
+  p.gave_up = st.counters + FS_GAVE_UP;
   p.grid = grid;
   p.target = st.target;
   p.bias = st.bias;
@@ -1474,6 +1497,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> full_softmax_bwd(const at::Tensor
     FsParams p{};
     fs_shape(p, V, Dp, true);
     p.n_valid = st.counters + FS_N_VALID;
+    p.gave_up = st.counters + FS_GAVE_UP;
     p.grid = grid;
     p.target = st.target;
     p.bias = st.bias;
@@ -1493,10 +1517,10 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> full_softmax_bwd(const at::Tensor
     if (has_bias) per_row ? fs_launch<FS_BWD, true, true>(tx, ty, p, dev) : fs_launch<FS_BWD, true, false>(tx, ty, p, dev);
     else per_row ? fs_launch<FS_BWD, false, true>(tx, ty, p, dev) : fs_launch<FS_BWD, false, false>(tx, ty, p, dev);
   }
-  if (want_h || want_b || may_split) {
+  if (want_h || main) {  // (behind every main kernel: it looks whether a block gave up)
     const FinishParams f{st, int(P), int(V), int(D), int(Dp), grid, pieces, per_row, mean, dloss.data_ptr<float>(), per_row ? dloss.stride(0) : 0, part_acc, part_l,
-                         want_h ? dh.data_ptr() : nullptr, dw.data_ptr(), want_b ? db.data_ptr() : nullptr, !db_fp32};
-    const int64_t most = std::max<int64_t>({want_h ? P * (Dp / 8) : 0, n_acc / 8, want_b ? V : 0});
+                         want_h ? dh.data_ptr() : nullptr, dw.data_ptr(), main ? V : 0, want_b ? db.data_ptr() : nullptr, !db_fp32};
+    const int64_t most = std::max<int64_t>({want_h ? P * (Dp / 8) : 0, n_acc / 8, want_b ? V : 0, 1});
     const unsigned blocks = unsigned(std::min<int64_t>((most + 255) / 256, 16 * grid));
     auto finish = dh_fp32 ? (dw_fp32 ? full_softmax_finish_kernel<float, float> : full_softmax_finish_kernel<float, __nv_bfloat16>)
                           : (dw_fp32 ? full_softmax_finish_kernel<__nv_bfloat16, float> : full_softmax_finish_kernel<__nv_bfloat16, __nv_bfloat16>);
@@ -1540,7 +1564,7 @@ int64_t full_softmax_status() {
 }  // namespace trb
 
 TORCH_LIBRARY_FRAGMENT(trb200, m) {
-  m.def("full_softmax_fwd(Tensor h, Tensor weight, Tensor targets, Tensor? bias, int ignore_index, int reduction, int grad) -> (Tensor, Tensor)");
+  m.def("full_softmax_fwd(Tensor h, Tensor weight, Tensor targets, Tensor? bias, int ignore_index, int reduction, int grad, int gave_up=0) -> (Tensor, Tensor)");
   m.def("full_softmax_bwd(Tensor dloss, Tensor weight, Tensor state, int P, int D, bool has_bias, int reduction, bool has_unit, bool want_h, bool want_w, bool want_b, "
         "bool dh_fp32, bool dw_fp32, bool db_fp32) -> (Tensor, Tensor, Tensor)");
   m.def("full_softmax_check_targets(Tensor targets, int classes, int ignore_index) -> ()");

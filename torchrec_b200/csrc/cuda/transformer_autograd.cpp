@@ -45,7 +45,7 @@ struct FullSoftmaxLoss : public torch::autograd::Function<FullSoftmaxLoss> {
   static Tensor forward(AutogradContext* ctx, const Tensor& h, const Tensor& weight, const c10::optional<Tensor>& bias, const Tensor& targets,
                         const c10::optional<Tensor>& rounded, int64_t ignore_index, int64_t reduction, int64_t grad) {
     const Tensor w = kernel_rows(weight, rounded);
-    auto [loss, state] = full_softmax_fwd(h, w, targets, bias, ignore_index, reduction, grad);
+    auto [loss, state] = full_softmax_fwd(h, w, targets, bias, ignore_index, reduction, grad, 0);
     if (grad > 0) {
       // the caller's weight is saved too where the kernel read a copy, so that a change in place is noticed
       ctx->save_for_backward({state, weight, w.is_same(weight) ? Tensor() : w});
@@ -93,7 +93,7 @@ static void check_full_softmax(const Tensor& h, const Tensor& weight, const c10:
 static Tensor full_softmax_loss_plain(const Tensor& h, const Tensor& weight, const c10::optional<Tensor>& bias, const Tensor& targets, const c10::optional<Tensor>& rounded,
                                       int64_t ignore_index, int64_t reduction) {
   check_full_softmax(h, weight, bias, targets);
-  return std::get<0>(full_softmax_fwd(h, kernel_rows(weight, rounded), targets, bias, ignore_index, reduction, 0));
+  return std::get<0>(full_softmax_fwd(h, kernel_rows(weight, rounded), targets, bias, ignore_index, reduction, 0, 0));
 }
 
 static Tensor full_softmax_loss_autograd(const Tensor& h, const Tensor& weight, const c10::optional<Tensor>& bias, const Tensor& targets, const c10::optional<Tensor>& rounded,

@@ -9,7 +9,7 @@ namespace trb {
 
 // full_softmax_kernels.cu
 std::tuple<at::Tensor, at::Tensor> full_softmax_fwd(const at::Tensor& h, const at::Tensor& weight, const at::Tensor& targets, const c10::optional<at::Tensor>& bias,
-                                                    int64_t ignore_index, int64_t reduction, int64_t grad);
+                                                    int64_t ignore_index, int64_t reduction, int64_t grad, int64_t gave_up);
 std::tuple<at::Tensor, at::Tensor, at::Tensor> full_softmax_bwd(const at::Tensor& dloss, const at::Tensor& weight, const at::Tensor& state, int64_t P, int64_t D, bool has_bias,
                                                                 int64_t reduction, bool has_unit, bool want_h, bool want_w, bool want_b, bool dh_fp32, bool dw_fp32, bool db_fp32);
 

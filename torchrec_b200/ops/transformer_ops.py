@@ -308,7 +308,8 @@ _KERNEL_TYPES = (torch.bfloat16, torch.float32)
 
 def full_softmax_error(device: torch.device) -> int:
     """Non-zero after a ``full_softmax_loss`` launch on ``device`` met a target outside ``[0, V)`` that is not ``ignore_index`` (16: the
-    loss of that row is NaN, its gradient zero) or gave up waiting for its own copies (1..9).  Reading it synchronises and resets it."""
+    loss of that row is NaN, its gradient zero) or gave up waiting for its own copies (1..9: the loss and all gradients of that call are NaN).
+    Reading it synchronises and resets it."""
     device = torch.device(device)
     if device.type != "cuda" or not _ext.has_cuda_ext():
         return 0

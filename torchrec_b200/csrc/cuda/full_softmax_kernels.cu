@@ -926,10 +926,13 @@ struct FsState {
 
 // ---- before the forward -----------------------------------------------------------------------------
 // Blocks 0..row_blocks-1 put the rows whose target counts one behind the other (in their order), as bf16 with zero columns up to Dp.
-// The remaining blocks copy the bias with -inf behind V.  Every row block counts the targets before its own itself: P targets are at
-// most a few hundred KB in L2, cheaper than another launch.  A block takes 32 to 512 rows, so that two blocks per SM share the copying
-// (4096 rows of 512: 39 us with 512 rows a block).
+// The remaining blocks copy the bias with -inf behind V.  Every row block counts the targets before its own itself, from the start of its
+// stretch of kPrepStretch rows: up to that many rows a few hundred KB in L2, cheaper than another launch.  More rows have their stretches
+// counted by a kernel in front, so that the reading grows with the rows and not with their square (a call with all of its rows ignored:
+// 65537 rows 61 us without that kernel and 69 with it, 450563 rows 449 and 295 us, 16 M rows 294 and 10 ms).  A block takes 32 to 512 rows, so that
+// two blocks per SM share the copying (4096 rows of 512: 39 us with 512 rows a block).
 constexpr int kPrepThreads = 512;
+constexpr int64_t kPrepStretch = 65536;  // a multiple of every block's rows
 
 struct PrepParams {
   const void* h;
@@ -947,6 +950,7 @@ struct PrepParams {
   int bias_bf16;
   int rows;  // of a block: a multiple of 32
   int row_blocks;
+  int64_t* stretches;  // targets of every whole stretch (as fs_target_kind sums them), or null: there is only one
   int gave_up;  // what FS_GAVE_UP starts at
 };
 
@@ -955,6 +959,22 @@ __device__ __forceinline__ int64_t fs_target(int64_t i, const PrepParams& p) {
 }
 // 0 ignored, 1 counts, 1 << 32 outside the classes (so that a sum counts both)
 __device__ __forceinline__ int64_t fs_target_kind(int64_t t, const PrepParams& p) { return t == p.ignore ? 0 : (t < 0 || t >= p.V ? int64_t(1) << 32 : 1); }
+
+// one block per stretch
+__global__ void __launch_bounds__(kPrepThreads) full_softmax_count_kernel(const PrepParams p) {
+  __shared__ int64_t sums[kPrepThreads / 32];
+  const int64_t begin = int64_t(blockIdx.x) * kPrepStretch, end = min(begin + kPrepStretch, int64_t(p.P));
+  int64_t n = 0;
+  for (int64_t i = begin + threadIdx.x; i < end; i += kPrepThreads) n += fs_target_kind(fs_target(i, p), p);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+  if ((threadIdx.x & 31) == 0) sums[threadIdx.x >> 5] = n;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < kPrepThreads / 32; ++w) n += sums[w];
+    p.stretches[blockIdx.x] = n;
+  }
+}
 
 __global__ void __launch_bounds__(kPrepThreads) full_softmax_prep_kernel(const PrepParams p) {
   fs_let_next();
@@ -972,7 +992,9 @@ __global__ void __launch_bounds__(kPrepThreads) full_softmax_prep_kernel(const P
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t begin = int64_t(blockIdx.x) * p.rows, row = int(threadIdx.x) < p.rows ? begin + threadIdx.x : p.P;  // P: no row
   int64_t before = 0;
-  for (int64_t i = threadIdx.x; i < begin; i += kPrepThreads) before += fs_target_kind(fs_target(i, p), p);
+  const int64_t stretch = p.stretches != nullptr ? begin / kPrepStretch : 0;
+  for (int64_t i = threadIdx.x; i < stretch; i += kPrepThreads) before += p.stretches[i];
+  for (int64_t i = stretch * kPrepStretch + threadIdx.x; i < begin; i += kPrepThreads) before += fs_target_kind(fs_target(i, p), p);
   const int64_t t = row < p.P ? fs_target(row, p) : p.ignore;
   const int64_t kind = fs_target_kind(t, p);
   const uint32_t mine = __ballot_sync(0xffffffffu, kind == 1), bad = __ballot_sync(0xffffffffu, kind > 1);
@@ -1408,12 +1430,16 @@ std::tuple<at::Tensor, at::Tensor> full_softmax_fwd(const at::Tensor& h, const a
   const int grid = fs_grid(h.device());
   const int pieces = acc ? int((Dp + kFsAcc - 1) / kFsAcc) : 1;
   const int64_t prows = (Ppad / kFsTile * pieces + grid) * kFsTile, n_acc = acc ? prows * std::min<int64_t>(Dp, kFsAcc) : 0;  // rows of all slots
-  at::Tensor part = at::empty({n_acc + 6 * prows + 2 * Ppad + Ppad / kFsTile}, f32);  // accumulators, references, sums, targets' scores, losses
+  const int64_t n_stretch = P > kPrepStretch ? (P + kPrepStretch - 1) / kPrepStretch : 0;
+  // accumulators, references, sums, targets' scores, losses, counts of the stretches (on 8 bytes), losses of the tiles
+  at::Tensor part = at::empty({n_acc + 6 * prows + 2 * Ppad + 2 * n_stretch + Ppad / kFsTile}, f32);
   float* part_acc = part.data_ptr<float>();
   float2* part_m = reinterpret_cast<float2*>(part_acc + n_acc);
   float* part_l = part_acc + n_acc + 4 * prows;
   float* zt = part_l + 2 * prows;
   float* loss_c = zt + Ppad;
+  int64_t* stretches = n_stretch > 0 ? reinterpret_cast<int64_t*>(loss_c + Ppad) : nullptr;
+  float* tile_loss = loss_c + Ppad + 2 * n_stretch;
   {
     int rows = 32;
     while (rows < kPrepThreads && int64_t(rows) * 2 * grid < P) rows *= 2;
@@ -1423,7 +1449,11 @@ std::tuple<at::Tensor, at::Tensor> full_softmax_fwd(const at::Tensor& h, const a
     const bool vec = !fp32 && D == Dp && h.stride(1) == 1 && h.stride(0) % 8 == 0 && reinterpret_cast<uintptr_t>(h.data_ptr()) % 16 == 0;
     const PrepParams q{h.data_ptr(), h.stride(0), h.stride(1), fp32, vec, targets.data_ptr(), targets.stride(0), ignore_index, targets.scalar_type() == at::kInt,
                        int(P), int(V), int(D), int(Dp), st, loss.data_ptr<float>(), int(reduction), has_bias ? bias->data_ptr() : nullptr, has_bias ? bias->stride(0) : 0,
-                       has_bias && bias->scalar_type() == at::kBFloat16, rows, row_blocks, gave_up != 0};
+                       has_bias && bias->scalar_type() == at::kBFloat16, rows, row_blocks, stretches, gave_up != 0};
+    if (n_stretch > 0) {
+      full_softmax_count_kernel<<<unsigned(n_stretch), kPrepThreads, 0, stream>>>(q);
+      TRB_CUDA_CHECK(cudaGetLastError());
+    }
     full_softmax_prep_kernel<<<row_blocks + bias_blocks, kPrepThreads, 0, stream>>>(q);
     TRB_CUDA_CHECK(cudaGetLastError());
   }
@@ -1443,7 +1473,7 @@ std::tuple<at::Tensor, at::Tensor> full_softmax_fwd(const at::Tensor& h, const a
   const int dev = h.device().index();
   if (acc) has_bias ? fs_launch<FS_FWD, true, false>(tx, ty, p, dev) : fs_launch<FS_FWD, false, false>(tx, ty, p, dev);
   else has_bias ? fs_launch<FS_LSE, true, false>(tx, ty, p, dev) : fs_launch<FS_LSE, false, false>(tx, ty, p, dev);
-  const JoinParams j{st, int(V), int(Dp), grid, pieces, int(reduction), part_acc, part_m, part_l, zt, loss_c, loss_c + Ppad, reinterpret_cast<const __nv_bfloat16*>(weight.data_ptr()),
+  const JoinParams j{st, int(V), int(Dp), grid, pieces, int(reduction), part_acc, part_m, part_l, zt, loss_c, tile_loss, reinterpret_cast<const __nv_bfloat16*>(weight.data_ptr()),
                      weight.stride(0), loss.data_ptr<float>()};
   const int smem = (grid + 8) * 4 + kJoinThreads * 16;
   if (acc) fs_launch_next(full_softmax_join_kernel<true>, unsigned(Ppad), kJoinThreads, smem, stream, j);

@@ -51,10 +51,11 @@ class QKNormRotary(nn.Module):
 
 
 def packed_token_positions(offsets: torch.Tensor, num_tokens: int) -> torch.Tensor:
-    """Place of every packed token in its own sequence, ``[num_tokens]`` (no host synchronisation)."""
+    """Place of every packed token in its own sequence, ``[num_tokens]`` (no host synchronisation).  Tokens behind the last sequence, as in a
+    buffer of a fixed size, are counted from its end."""
     offsets = offsets.to(torch.int64)
-    first = torch.repeat_interleave(offsets[:-1], offsets[1:] - offsets[:-1], output_size=num_tokens)
-    return torch.arange(num_tokens, device=offsets.device) - first
+    token = torch.arange(num_tokens, device=offsets.device)
+    return token - offsets.index_select(0, torch.searchsorted(offsets[1:].contiguous(), token, right=True))
 
 
 def supports(encoder: nn.TransformerEncoder) -> bool:

@@ -41,9 +41,11 @@ class QKNormRotary(nn.Module):
         self.register_buffer("inv_freq", rotary_inv_freq(self.rotary_dim, base, device), persistent=False)
 
     def _apply(self, fn, recurse: bool = True):
+        freq = self.inv_freq
         super()._apply(fn, recurse)
-        # a cast of the module must not round the frequencies, and a move off the meta device has to fill them
-        self.inv_freq = rotary_inv_freq(self.rotary_dim, self.base, self.q_weight.device)
+        # a cast of the module must not round the frequencies (which may have been set to others), and a move off the meta device has to fill them
+        device = self.q_weight.device
+        self.inv_freq = rotary_inv_freq(self.rotary_dim, self.base, device) if freq.is_meta else freq.to(device)
         return self
 
     def forward(self, qkv: torch.Tensor, positions: torch.Tensor, num_heads: int, num_kv_heads: Optional[int] = None) -> torch.Tensor:

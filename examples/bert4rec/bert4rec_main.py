@@ -1,7 +1,7 @@
 """Masked-item training of BERT4Rec on synthetic sessions with a sharded item table.
 
     python examples/bert4rec/bert4rec_main.py --num_iterations 5
-    python examples/bert4rec/bert4rec_main.py --full_softmax --rotary
+    python examples/bert4rec/bert4rec_main.py --full_softmax --rotary --bf16
     torchrun --standalone --local-addr 127.0.0.1 --nproc-per-node 8 examples/bert4rec/bert4rec_main.py --sharding column_wise
 
 (cf. ``examples/bert4rec/bert4rec_main.py`` of the reference.)"""
@@ -21,6 +21,7 @@ from torchrec_b200.distributed.embedding import EmbeddingCollectionSharder  # no
 from torchrec_b200.distributed.model_parallel import DistributedModelParallel  # noqa: E402
 from torchrec_b200.distributed.types import ShardingEnv, ShardingPlan  # noqa: E402
 from torchrec_b200.models.bert4rec import BERT4Rec  # noqa: E402
+from torchrec_b200.ops import dense_ops  # noqa: E402
 from torchrec_b200.optim.apply_optimizer_in_backward import apply_optimizer_in_backward  # noqa: E402
 from torchrec_b200.optim.keyed import CombinedOptimizer, KeyedOptimizerWrapper  # noqa: E402
 from torchrec_b200.optim.optimizers import in_backward_optimizer_filter  # noqa: E402
@@ -56,6 +57,7 @@ def main() -> None:
     p.add_argument("--lr", type=float, default=1e-3)
     p.add_argument("--full_softmax", action="store_true", help="cross entropy over the whole vocabulary instead of sampled negatives")
     p.add_argument("--rotary", action="store_true", help="normalised, position-rotated queries and keys instead of learned position embeddings")
+    p.add_argument("--bf16", action="store_true", help="bf16 products with fp32 sums in the dense layers and the loss (on a GPU: their tensor-core kernels); fp32 without")
     p.add_argument("--sharding", default="row_wise", choices=["table_wise", "row_wise", "column_wise", "data_parallel"])
     a = p.parse_args()
     rank, world = int(os.environ.get("RANK", 0)), int(os.environ.get("WORLD_SIZE", 1))
@@ -69,6 +71,8 @@ def main() -> None:
         os.environ.setdefault("MASTER_ADDR", "127.0.0.1")
         os.environ.setdefault("MASTER_PORT", "29551")
         dist.init_process_group(backend, rank=rank, world_size=world)
+    if a.bf16:
+        dense_ops.set_dense_compute_dtype(torch.bfloat16)
     torch.manual_seed(0)
     model = BERT4Rec(a.vocab_size, a.max_len, a.emb_dim, a.nhead, a.num_layers, rotary=a.rotary).to(device)
     apply_optimizer_in_backward(torch.optim.Adam, model.history.ec.parameters(), {"lr": a.lr})

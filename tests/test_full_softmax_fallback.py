@@ -5,7 +5,18 @@ import math
 import pytest
 import torch
 
+from torchrec_b200.ops import dense_ops
 from torchrec_b200.ops.transformer_ops import full_softmax_loss
+
+
+@pytest.fixture(autouse=True)
+def fp32_compute_type():
+    """Another test of the process may have left bf16, with which fp32 tensors go to the tensor-core kernels."""
+    prev = dense_ops.get_dense_compute_dtype()
+    dense_ops.set_dense_compute_dtype(torch.float32)
+    yield
+    dense_ops.set_dense_compute_dtype(prev)
+
 
 devices = pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
 

@@ -4,6 +4,17 @@ import torch
 
 from torchrec_b200.models.bert4rec import BERT4Rec
 from torchrec_b200.modules.jagged_transformer import jagged_encoder_forward, packed_token_positions
+from torchrec_b200.ops import dense_ops
+
+
+@pytest.fixture(autouse=True)
+def fp32_compute_type():
+    """Another test of the process may have left bf16, with which fp32 tensors go to the tensor-core kernels."""
+    prev = dense_ops.get_dense_compute_dtype()
+    dense_ops.set_dense_compute_dtype(torch.float32)
+    yield
+    dense_ops.set_dense_compute_dtype(prev)
+
 
 devices = pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
 

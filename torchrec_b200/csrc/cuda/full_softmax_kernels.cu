@@ -13,6 +13,10 @@
 // The target's own term never enters the rounded sums: with w = 1 - p_t (from the sum over the others), dh = w (ACC / sum - W_t) and
 // G_it = -w, so rows that the model already predicts well keep their relative accuracy.
 //
+// E, and G in the backward, are rounded to bf16 (by at most 2^-8 of a term) in front of the second product, as the first one's operands are:
+// the terms need an exponent range that fp16 has not, and a tf32 product would run at half the rate and want W and h in 32 bits too.  The sums
+// are of the terms before that rounding, and like ACC in fp32; gradients that leave in fp32 hold the same rounded terms.
+//
 // Both products want the streamed tile, once K-major (S) and once MN-major (ACC); one copy in shared memory serves both up to
 // D = 256, where ACC takes the 256 TMEM columns that two S tiles leave.  Wider rows are cut into pieces of 256 columns that
 // recompute S (and load the tile twice).
@@ -24,12 +28,13 @@
 // Every wait is bounded (tcgen05.cuh); a block that gives up raises an error word, marks the call's state and returns, and the kernels behind
 // it give NaN for the loss and every gradient of that call.
 //
-// Measured (B200, 18944 rows x 40000 classes, whole forward or backward): D = 256 forward with dh 644 us (1.20 PFLOP/s), backward 557 us
-// (1.39), value only 370 us (1.05); D = 64 422, 311 and 336 us, where the 16384 exponentials of a tile take 1.0 to 1.3 us; D = 512 (half the
-// rows) 881, 831 and 276 us, with the scores computed once per 256 columns.  At 16384 x 131071 x 256 a step takes 4.21 ms: 8 P V D at 1.04
-// PFLOP/s under the power cap (the library product alone sustains 1.40).  What bounds it: the score product reads both operands from
-// shared memory, which also receives the streamed tile; for narrow rows the softmax warps, at 60 % of the special-function rate (neither
-// more warps, nor paired arithmetic, nor a polynomial for a part of the exponentials changed that).
+// Measured (B200, 18944 rows x 40000 classes, whole forward or backward): D = 256 forward with dh 657 us (1.18 PFLOP/s), backward 576 us
+// (1.35), value only 380 us (1.02); D = 64 448, 328 and 372 us; D = 512 (half the rows) 907, 933 and 277 us, with the scores computed once per
+// 256 columns, and D = 1024 (a quarter) 1860, 1803 and 380 us.  At 16384 x 131071 x 256 a step takes 4.27 ms: 8 P V D at 1.03 PFLOP/s under the
+// power cap (the library product alone sustains 1.40).  What bounds it: the score product reads both operands from shared memory, which
+// also receives the streamed tile.  Narrow rows and values alone take 1.1 to 1.2 us a tile whatever D is; what bounds them is not known: the
+// special-function pipe is 47 to 56 % busy, 0.45 instructions are issued a cycle, most stalls are the fixed latency between dependent
+// instructions, and more warps, paired arithmetic or a polynomial for a part of the exponentials each left the time as it was.
 //
 // (The reference ends BERT4Rec in a dense projection over the vocabulary and nn.CrossEntropyLoss, examples/bert4rec/bert4rec_main.py.)
 #include <ATen/ATen.h>

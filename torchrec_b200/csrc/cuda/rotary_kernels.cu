@@ -11,9 +11,10 @@
 // head costs its loads, one sum over the group and two products per value; the partner's values come from the neighbouring lanes.  (With a
 // warp per token and the factors fetched anew for every head, the kernel issued 600 to 900 instructions per token of 12 heads and was
 // bound by that.)  Statistics and sums are fp32, one rounding at the end.
-// Measured (B200): 450563 tokens of 12 heads of 64 bf16 forward 251 us (5.5 TB/s of 6.5), backward 450 us (4.1 TB/s, bound by issue and
-// latency at 24 warps an SM); 20011 tokens of 20 heads of 128 fp32 70 us (5.8 TB/s) and 113 us (5.3 TB/s).  Heads whose half of the rotated
-// part is not a multiple of eight fetch their partners one by one: 2.2 to 2.5 TB/s.
+// Measured (B200): 450563 tokens of 12 heads of 64 bf16 forward 253 us (5.5 TB/s of 6.5), backward 456 us (4.0 TB/s: 0.54 instructions a
+// cycle at the 24 warps an SM that its registers are bounded for); 20011 tokens of 20 heads of 128 fp32 73 us (5.6 TB/s) and 114 us
+// (5.3 TB/s).  Heads whose half of the rotated part is not a multiple of eight fetch their partners one by one: 2.4 TB/s (131075 tokens of
+// 24 heads of 48, 24 of them turned, fp16: 252 us, backward 333 us).
 // dw is summed per token in registers, over a thread's tokens in shared memory, then over the block and by a second kernel over the
 // blocks, in a fixed order.
 #include <ATen/ATen.h>

@@ -206,7 +206,8 @@ def qk_norm_rotary(qkv: torch.Tensor, positions: torch.Tensor, inv_freq: torch.T
                    sections: Optional[Sequence[int]] = None, interleaved: bool = False, norm: bool = True) -> torch.Tensor:
     """Queries and keys of the packed ``qkv [T, (num_heads + 2 * num_kv_heads) * head_dim]`` (``q | k | v`` along the columns) with every head
     divided by its root mean square (``norm``), scaled by ``q_weight`` / ``k_weight [head_dim]`` and turned by its token's position; ``v``
-    unchanged.  Returns a new tensor of the same shape and type, ready for :func:`packed_attention`.
+    unchanged.  Returns a new tensor of the same shape and type; with equal head counts, heads of 64 and bf16 it is what :func:`packed_attention`
+    takes (shared key heads are for an attention of the caller's).
 
     The first ``2 * len(inv_freq)`` values of a head are turned, pair ``j`` by ``positions[t] * inv_freq[j]`` (:func:`rotary_inv_freq`; the
     angle is formed in fp64): value ``j`` with value ``j + len(inv_freq)``, or neighbours ``2 j, 2 j + 1`` with ``interleaved``.  With several
@@ -406,8 +407,8 @@ def full_softmax_loss(h: torch.Tensor, weight: torch.Tensor, targets: torch.Tens
     none), ``"sum"`` or ``"none"`` (``[P]``, 0 at ignored rows).
 
     On CUDA bf16 ``h`` (and fp32 ``h`` while the dense compute type is bf16, ``dense_ops.set_dense_compute_dtype``) with ``D <= 1024`` runs
-    on the tensor cores with bf16 operands and fp32 sums; an fp32 ``weight`` is rounded to bf16 for the products and gets an fp32
-    gradient.  Everything else is computed in fp32 (fp64 for fp64 ``h``), a piece of the rows at a time.  A target outside ``[0, V)``
+    on the tensor cores with bf16 operands (the softmax terms of the gradients among them) and fp32 sums; an fp32 ``weight`` is rounded to
+    bf16 for the products and gets an fp32 gradient (a parameter once per version, as in the dense layers).  Everything else is computed in fp32 (fp64 for fp64 ``h``), a piece of the rows at a time.  A target outside ``[0, V)``
     raises on the CPU; on CUDA it makes the row's loss NaN and its gradient zero, and ``full_softmax_error`` reports it.  Forward-mode
     and second derivatives are refused."""
     if reduction not in _REDUCTIONS:

@@ -46,3 +46,31 @@ def test_second_derivatives_of_the_rotation_are_never_dropped(device, dtype):
     else:
         with pytest.raises(RuntimeError, match="differentiated again"):
             (g.float().square().sum() + leaves[0].float().sum()).backward()
+
+
+@devices
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("which", [0, 1, 2])
+def test_second_derivatives_of_the_loss_along_another_path(device, dtype, which):
+    """torch.autograd.grad walks only the paths to the inputs that it is asked for: the gradient has to lie on one."""
+    *x, t = _loss_inputs(device, dtype)
+    leaves = [v.requires_grad_(True) for v in x]
+    grads = torch.autograd.grad(full_softmax_loss(leaves[0], leaves[1], t, leaves[2]), leaves, create_graph=True)
+    for g in grads:
+        with pytest.raises(RuntimeError, match="differentiated again"):
+            torch.autograd.grad(g.float().square().sum() + leaves[which].float().sum(), leaves[which], retain_graph=True)
+    with pytest.raises(RuntimeError, match="differentiated again"):
+        torch.autograd.functional.hessian(lambda v: full_softmax_loss(v, leaves[1].detach(), t), leaves[0].detach())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("which", [0, 1, 2])
+def test_second_derivatives_of_the_rotation_along_another_path(dtype, which):
+    x = _rotary_inputs("cuda", dtype)
+    leaves = [v.requires_grad_(True) for v in x[:3]]
+    out = qk_norm_rotary(leaves[0], x[3], x[4], 1, q_weight=leaves[1], k_weight=leaves[2])
+    grads = torch.autograd.grad(out.float().square().sum(), leaves, create_graph=True)
+    for g in grads:
+        with pytest.raises(RuntimeError, match="differentiated again"):
+            torch.autograd.grad(g.float().square().sum() + leaves[which].float().sum(), leaves[which], retain_graph=True)

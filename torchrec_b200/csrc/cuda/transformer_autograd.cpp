@@ -4,6 +4,7 @@
 #include <ATen/ATen.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/library.h>
 
 #include "transformer_ops.h"
@@ -15,13 +16,20 @@ using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
 // Gradients of a backward that is itself recorded (create_graph): differentiating them again is an error, not silently zero.  They depend on
-// the inputs whether or not the upstream gradient, often the constant one, is recorded too.
+// the inputs whether or not the upstream gradient, often the constant one, is recorded too, and the error lies on the way to every input
+// (an engine that is asked for one input's gradient walks no other way).
 static variable_list once(variable_list grads, const char* name) {
   if (!at::GradMode::is_enabled()) return grads;
-  variable_list in;
-  for (auto& g : grads) in.push_back(g.defined() ? g.detach().set_requires_grad(true) : g);
-  auto error = std::make_shared<torch::autograd::DelayedError>(std::string("the gradient of ") + name + " cannot be differentiated again", int(in.size()));
-  return (*error)(std::move(in));
+  torch::autograd::edge_list inputs;
+  for (const auto& edge : torch::autograd::get_current_node()->next_edges())
+    if (edge.is_valid()) inputs.push_back(edge);
+  auto error = std::make_shared<torch::autograd::Error>(std::string("the gradient of ") + name + " cannot be differentiated again", std::move(inputs));
+  for (auto& g : grads)
+    if (g.defined()) {
+      g = g.detach();
+      torch::autograd::set_history(g, error);
+    }
+  return grads;
 }
 
 // A dual tensor need not require a gradient, so that a call without a node would drop its tangent: a derivative of zero.

@@ -318,6 +318,18 @@ def full_softmax_error(device: torch.device) -> int:
         return int(torch.ops.trb200.full_softmax_status())
 
 
+class _OnlyOnce(torch.autograd.Function):
+    """The gradients of a backward that is itself recorded (``create_graph``), with an error on the way from them to every input."""
+
+    @staticmethod
+    def forward(ctx, dh, dw, db, h, weight, bias):
+        return tuple(None if x is None else x.view_as(x) for x in (dh, dw, db))
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError("the gradient of full_softmax_loss cannot be differentiated again")
+
+
 class _FullSoftmaxPieces(torch.autograd.Function):
     """The same loss in plain torch, a piece of the rows at a time (never the whole ``[P, V]`` scores), recomputed in the backward:
     CPU tensors, types and widths the kernel does not take, and the oracle of the small tests."""
@@ -367,9 +379,8 @@ class _FullSoftmaxPieces(torch.autograd.Function):
     def backward(ctx, g):
         with torch.no_grad():
             grads = _FullSoftmaxPieces._gradients(ctx, g)
-        if torch.is_grad_enabled():  # create_graph: an error when they are differentiated again, whatever `g` is (once_differentiable asks `g` alone)
-            fail = torch._C._functions.DelayedError(b"the gradient of full_softmax_loss cannot be differentiated again", len(grads))
-            grads = fail(*(None if x is None else x.detach().requires_grad_(True) for x in grads))
+        if torch.is_grad_enabled():
+            grads = _OnlyOnce.apply(*grads, *ctx.saved_tensors[:3])
         return grads[0], grads[1], grads[2], None, None, None
 
     @staticmethod
